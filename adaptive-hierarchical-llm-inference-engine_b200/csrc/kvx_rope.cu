@@ -1,0 +1,535 @@
+// kvx_rope.cu -- rotary positions (kvx_rope) and the ragged, rotated append
+// into fp16 / fp32 / int8 pages (kvx_rope_append).
+//
+// Both are bound by the bytes of their rows.  One CTA per token: its
+// (cos, sin) pairs are worked out once into shared memory (rotary/2 sincospi
+// for heads * rotary/2 pairs), each thread keeps one item of a row -- a
+// 16-byte vector, or the two that pair up in the half layout -- with its
+// cosines in registers and walks the token's rows.
+#include <math.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "kvx_common.cuh"
+#include "kvx_rope.cuh"
+
+namespace kvx {
+namespace {
+
+constexpr int kMaxRopeDim = 1024;
+constexpr int kRopeThreads = 256;
+constexpr int kRowsInFlight = 4;  // rows whose loads a thread issues together
+
+struct RopeTensor {
+    const void *in;
+    void *out;
+    int heads;
+    int64_t in_token, in_head, out_token, out_head;
+};
+
+struct RopeParams {
+    const uint64_t *turns;
+    const int32_t *positions;
+    RopeTensor x[2];
+    int rotary, items;
+    float amplitude, sine_sign;
+};
+
+// The token's (cos, sin) pairs into shared memory.
+__device__ __forceinline__ void fill_cs(float2 *cs, const uint64_t *turns, int pairs, int64_t pos, float amplitude,
+                                        float sine_sign) {
+    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+        float2 v = rope_turn(turns[i], pos, amplitude);
+        v.y *= sine_sign;
+        cs[i] = v;
+    }
+}
+
+// Rows row0, row0 + step, ... < rows of the tensors, this thread's item of each.
+template <typename Item, typename T, typename Address>
+__device__ __forceinline__ void rope_rows(const Item &item, int row0, int step, int rows, Address at) {
+    for (int r = row0; r < rows; r += kRowsInFlight * step) {
+        typename Item::Data d[kRowsInFlight];
+        const T *src[kRowsInFlight];
+        T *dst[kRowsInFlight];
+        bool turn[kRowsInFlight];
+#pragma unroll
+        for (int u = 0; u < kRowsInFlight; ++u) {
+            dst[u] = nullptr;
+            if (r + u * step < rows) {
+                at(r + u * step, src[u], dst[u], turn[u]);
+                if (dst[u]) item.load(src[u], d[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kRowsInFlight; ++u)
+            if (dst[u]) {
+                if (turn[u]) item.turn(d[u]);
+                item.store(dst[u], d[u]);
+            }
+    }
+}
+
+template <typename T, bool kHalf, bool kVec>
+__global__ void __launch_bounds__(kVec ? kRopeThreads : kMaxRopeDim) rope_kernel(const __grid_constant__ RopeParams p) {
+    __shared__ float2 cs[kMaxRopeDim / 2];
+    const int64_t t = blockIdx.x;
+    fill_cs(cs, p.turns, p.rotary / 2, p.positions[t], p.amplitude, p.sine_sign);
+    __syncthreads();
+    const int step = blockDim.x / p.items, row0 = threadIdx.x / p.items;
+    if (row0 >= step) return;  // threads left over by whole rows
+    const RopeItem<T, kHalf, kVec> item(threadIdx.x % p.items, p.rotary, cs);
+    rope_rows<RopeItem<T, kHalf, kVec>, T>(
+        item, row0, step, p.x[0].heads + p.x[1].heads, [&](int r, const T *&src, T *&dst, bool &turn) {
+            const int which = r >= p.x[0].heads;
+            const RopeTensor &x = p.x[which];
+            const int64_t h = which ? r - p.x[0].heads : r;
+            src = static_cast<const T *>(x.in) + t * x.in_token + h * x.in_head;
+            dst = static_cast<T *>(x.out) + t * x.out_token + h * x.out_head;
+            turn = true;
+        });
+}
+
+// ---------------------------------------------------------------------------
+// kvx_rope_append
+
+struct RopeAppendParams {
+    uint8_t *pool;
+    float *stats;
+    const int32_t *block_table, *q_start, *positions;
+    int32_t *error_flag;
+    const uint64_t *turns;  // null: no rotation
+    const void *q, *k, *v;
+    void *q_out;
+    int64_t q_stride, k_stride, v_stride;
+    int batch, total, hq, hkv, max_pages, num_pages, rotary, items;
+    int half_layout;
+    float amplitude;
+    int kv_blocks, tokens_per_block;  // int8: CTAs that write pages, and the tokens each looks at
+};
+
+// The sequence that owns packed row t, or -1: all threads look at the
+// boundaries at once (one round trip for up to blockDim sequences).
+__device__ __forceinline__ int find_sequence(const int32_t *q_start, int batch, int t, int *slot) {
+    if (threadIdx.x == 0) *slot = -1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < batch; i += blockDim.x)
+        if (q_start[i] <= t && t < q_start[i + 1]) *slot = i;
+    __syncthreads();
+    return *slot;
+}
+
+// Token blockIdx: rotate q, and (fp16 / fp32 pools) rotate k and store k, v.
+template <typename T, bool kHalf, bool kVec>
+__device__ __forceinline__ void rope_append_rows(const RopeAppendParams &p, int t, bool with_kv, float2 *cs, int *slot) {
+    const int s = find_sequence(p.q_start, p.batch, t, slot);
+    if (s < 0) return;
+    const int off = t - p.q_start[s];
+    const long long pos = (long long)p.positions[s] + off;
+    if (p.turns) {
+        fill_cs(cs, p.turns, p.rotary / 2, pos, p.amplitude, 1.f);
+        __syncthreads();
+    }
+    T *page_row = nullptr;  // K row of head 0 at the token's slot
+    if (with_kv) {
+        const long long lp = pos >> 4;
+        const int phys = p.positions[s] >= 0 && lp < p.max_pages ? p.block_table[(size_t)s * p.max_pages + lp] : -1;
+        if (phys >= 0 && phys < p.num_pages)
+            page_row = reinterpret_cast<T *>(p.pool) + ((size_t)phys * 2 * p.hkv * kPageTokens + (pos & 15)) * kHeadDim;
+        else if (p.error_flag && threadIdx.x == 0)
+            atomicOr(p.error_flag, 2);
+    }
+    const int step = blockDim.x / p.items, row0 = threadIdx.x / p.items;
+    if (row0 >= step) return;
+    const RopeItem<T, kHalf, kVec> item(threadIdx.x % p.items, p.rotary, cs);
+    const bool turning = p.turns != nullptr;
+    rope_rows<RopeItem<T, kHalf, kVec>, T>(
+        item, row0, step, p.hq + (page_row ? 2 * p.hkv : 0), [&](int r, const T *&src, T *&dst, bool &turn) {
+            turn = turning;
+            if (r < p.hq) {
+                src = static_cast<const T *>(p.q) + (int64_t)t * p.q_stride + r * kHeadDim;
+                dst = static_cast<T *>(p.q_out) + ((int64_t)t * p.hq + r) * kHeadDim;
+                return;
+            }
+            r -= p.hq;
+            dst = page_row + (size_t)r * kPageTokens * kHeadDim;  // K heads, then V heads of the page
+            if (r < p.hkv) {
+                src = static_cast<const T *>(p.k) + (int64_t)t * p.k_stride + r * kHeadDim;
+            } else {
+                src = static_cast<const T *>(p.v) + (int64_t)t * p.v_stride + (r - p.hkv) * kHeadDim;
+                turn = false;
+            }
+        });
+}
+
+// Without a table the item geometry is that of rotary_dim 2 * kRopeVec in the
+// interleaved layout (any that covers a row would do) and nothing turns.
+template <typename T, bool kHalf, bool kVec>
+__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_constant__ RopeAppendParams p) {
+    __shared__ float2 cs[kHeadDim / 2];
+    __shared__ int slot;
+    rope_append_rows<T, kHalf, kVec>(p, blockIdx.x, true, cs, &slot);
+}
+
+// ---- int8 pages
+
+constexpr float kTieLimit = 0.5f - 4.0e-5f;  // as in kvx_quant.cu: nearer to a half-integer, divide exactly
+constexpr float kTwo23 = 8388608.0f;
+
+// code + 128 of x: clamp(round((x - mn) / scale), 0, 255), NaN -> 0.  The
+// product with the reciprocal decides except next to a half-integer (or
+// where scale or its reciprocal is not finite), where the division does.
+__device__ __forceinline__ uint32_t level(float x, float mn, float scale, float rcp) {
+    const float t = __fmul_rn(__fsub_rn(x, mn), rcp);
+    const float s = __fadd_rn(t, kTwo23);
+    if (fabsf(__fsub_rn(t, __fsub_rn(s, kTwo23))) <= kTieLimit && t >= -0.5f && t <= 255.5f)
+        return __float_as_uint(s) & 0xffu;
+    const float r = roundf(__fdiv_rn(__fsub_rn(x, mn), scale));
+    return r >= 255.f && r < 2147483648.f ? 255u : (r > 0.f && r < 255.f ? (uint32_t)r : 0u);
+}
+
+__device__ __forceinline__ uint32_t code4(const float *x, float mn, float scale, float rcp) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w |= level(x[k], mn, scale, rcp) << (8 * k);
+    return w ^ 0x80808080u;
+}
+
+template <typename T> __device__ __forceinline__ void load4(const T *p, float *f);
+template <> __device__ __forceinline__ void load4<float>(const float *p, float *f) {
+    const float4 v = *reinterpret_cast<const float4 *>(p);
+    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+}
+template <> __device__ __forceinline__ void load4<__half>(const __half *p, float *f) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    const float2 a = h2_to_f2(v.x), b = h2_to_f2(v.y);
+    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+}
+
+// One warp: the new rows (n from slot `slot0`) of one (page, K|V, head)
+// block.  Lane: elements 4 lane .. 4 lane + 3 of every row, held in registers
+// between the range and the codes.  cs: (cos, sin) of row i's pairs at
+// cs + i * rotary/2, null for V and without a table.
+template <typename T>
+__device__ __forceinline__ void append_block_i8(const T *src, int64_t stride, uint8_t *codes, float *stats, int slot0,
+                                                int n, const float2 *cs, int rotary, bool half_layout) {
+    const int lane = threadIdx.x & 31, d = 4 * lane, half = rotary / 2;
+    const float4 old = *reinterpret_cast<const float4 *>(stats);
+    float x[kPageTokens][4];
+    float mn = INFINITY, mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kPageTokens; ++i)
+        if (i < n) load4<T>(src + i * stride + d, x[i]);
+    if (cs && d < rotary) {
+        if (!half_layout) {
+#pragma unroll
+            for (int i = 0; i < kPageTokens; ++i)
+                if (i < n) {
+                    const float2 *c = cs + i * half + d / 2;
+                    rope_pair(x[i][0], x[i][1], c[0]);
+                    if (d + 2 < rotary) rope_pair(x[i][2], x[i][3], c[1]);
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPageTokens; ++i)
+                if (i < n) {
+                    const T *row = src + i * stride;
+                    float y[4];
+                    if (half % 4 == 0) {
+                        load4<T>(row + (d < half ? d + half : d - half), y);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            y[k] = d + k < rotary ? io_traits<T>::load(row + (d + k < half ? d + k + half : d + k - half)) : 0.f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (d + k < half)
+                            rope_pair(x[i][k], y[k], cs[i * half + d + k]);
+                        else if (d + k < rotary)
+                            rope_pair(y[k], x[i][k], cs[i * half + d + k - half]);
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPageTokens; ++i)
+        if (i < n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                mn = fminf(mn, x[i][k]);
+                mx = fmaxf(mx, x[i][k]);
+            }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    if (slot0 > 0) {
+        mn = fminf(mn, old.x);
+        mx = fmaxf(mx, old.y);
+    }
+    if (!(mn <= mx)) mn = mx = NAN;  // nothing but NaN
+    float scale = __fdiv_rn(__fsub_rn(mx, mn), 255.f);
+    if (scale == 0.f) scale = 1.f;
+    const float rcp = __frcp_rn(scale);
+    uint32_t *rows = reinterpret_cast<uint32_t *>(codes) + lane;
+    if (slot0 > 0 && !(mn == old.x && mx == old.y)) {  // earlier rows in the wider range
+#pragma unroll 4
+        for (int r = 0; r < slot0; ++r) {
+            const uint32_t u = rows[r * 32] ^ 0x80808080u;
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = __fadd_rn(old.w, __fmul_rn((float)((u >> (8 * k)) & 0xffu), old.z));
+            rows[r * 32] = code4(v, mn, scale, rcp);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPageTokens; ++i)
+        if (i < n) rows[(slot0 + i) * 32] = code4(x[i], mn, scale, rcp);
+    if (lane == 0) *reinterpret_cast<float4 *>(stats) = make_float4(mn, mx, scale, mn);
+}
+
+// CTAs 0 .. kv_blocks-1 write pages, the others rotate the q rows of one
+// token each.  A page is written by whoever holds its first new token (the
+// sequence's first, or one at a page start) among its tokens_per_block packed
+// rows: one token a CTA while tokens are few (a decode step, where every
+// token leads), 16 when they fill the GPU anyway.
+template <typename T, bool kHalf, bool kVec>
+__global__ void __launch_bounds__(kRopeThreads) rope_append_i8_kernel(const __grid_constant__ RopeAppendParams p) {
+    __shared__ float2 cs[kPageTokens * kHeadDim / 2];
+    __shared__ int slot, found;
+    __shared__ int2 lead[kPageTokens];  // (sequence, packed row)
+    if (blockIdx.x >= p.kv_blocks) {
+        rope_append_rows<T, kHalf, kVec>(p, blockIdx.x - p.kv_blocks, false, cs, &slot);
+        return;
+    }
+    const int r0 = blockIdx.x * p.tokens_per_block, r1 = min(r0 + p.tokens_per_block, p.total);
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    for (int s = threadIdx.x; s < p.batch; s += blockDim.x) {
+        const int a = p.q_start[s], b = min(p.q_start[s + 1], p.total);
+        const int lo = max(a, r0), hi = min(b, r1);
+        if (a < 0 || lo >= hi) continue;
+        const int pos = p.positions[s];
+        if (pos < 0) {
+            if (p.error_flag) atomicOr(p.error_flag, 2);
+            continue;
+        }
+        for (int t = lo; t < hi;) {
+            const int in_page = (int)(((long long)pos + t - a) & 15);
+            if (t == a || in_page == 0) {
+                const int i = atomicAdd(&found, 1);
+                if (i < kPageTokens) lead[i] = make_int2(s, t);
+            }
+            t += 16 - in_page;
+        }
+    }
+    __syncthreads();
+    const int n_lead = min(found, kPageTokens), warp = threadIdx.x >> 5, half = p.rotary / 2;
+    for (int i = 0; i < n_lead; ++i) {
+        const int s = lead[i].x, t = lead[i].y;
+        const int a = p.q_start[s], b = min(p.q_start[s + 1], p.total);
+        const long long pos = (long long)p.positions[s] + t - a, lp = pos >> 4;
+        const int slot0 = (int)(pos & 15), n = min(kPageTokens - slot0, b - t);
+        const int phys = lp < p.max_pages ? p.block_table[(size_t)s * p.max_pages + lp] : -1;
+        if (phys < 0 || phys >= p.num_pages) {
+            if (p.error_flag && threadIdx.x == 0) atomicOr(p.error_flag, 2);
+            continue;
+        }
+        if (p.turns) {
+            __syncthreads();  // the previous page's rows are rotated
+            for (int j = threadIdx.x; j < n * half; j += blockDim.x)
+                cs[j] = rope_turn(p.turns[j % half], pos + j / half, p.amplitude);
+            __syncthreads();
+        }
+        for (int task = warp; task < 2 * p.hkv; task += kRopeThreads / 32) {
+            const bool is_v = task >= p.hkv;
+            const int h = is_v ? task - p.hkv : task;
+            const int64_t stride = is_v ? p.v_stride : p.k_stride;
+            const T *src = static_cast<const T *>(is_v ? p.v : p.k) + t * stride + h * kHeadDim;
+            const size_t block = (size_t)phys * 2 * p.hkv + task;
+            append_block_i8<T>(src, stride, p.pool + block * kPageTokens * kHeadDim, p.stats + block * 4, slot0, n,
+                               !is_v && p.turns ? cs : nullptr, p.rotary, p.half_layout);
+        }
+    }
+}
+
+template <typename T>
+int launch_rope(const RopeParams &p, int tokens, int threads, bool half, bool vec, cudaStream_t st) {
+    auto kern = half ? (vec ? rope_kernel<T, true, true> : rope_kernel<T, true, false>)
+                     : (vec ? rope_kernel<T, false, true> : rope_kernel<T, false, false>);
+    kern<<<(unsigned)tokens, threads, 0, st>>>(p);
+    return launch_status();
+}
+
+template <typename T>
+int launch_rope_append(const RopeAppendParams &p, bool i8, bool half, bool vec, cudaStream_t st) {
+    if (i8) {
+        auto kern = half ? (vec ? rope_append_i8_kernel<T, true, true> : rope_append_i8_kernel<T, true, false>)
+                         : (vec ? rope_append_i8_kernel<T, false, true> : rope_append_i8_kernel<T, false, false>);
+        kern<<<(unsigned)p.kv_blocks + (p.hq ? (unsigned)p.total : 0u), kRopeThreads, 0, st>>>(p);
+    } else {
+        auto kern = half ? (vec ? rope_append_kernel<T, true, true> : rope_append_kernel<T, true, false>)
+                         : (vec ? rope_append_kernel<T, false, true> : rope_append_kernel<T, false, false>);
+        kern<<<(unsigned)p.total, kRopeThreads, 0, st>>>(p);
+    }
+    return launch_status();
+}
+
+bool table_ok(const kvx_rope_table *t, int head_dim) {
+    return t->turns && !(reinterpret_cast<uintptr_t>(t->turns) & 7) && t->rotary_dim >= 2 && t->rotary_dim % 2 == 0 &&
+           t->rotary_dim <= head_dim && (t->layout == KVX_ROPE_HALF || t->layout == KVX_ROPE_INTERLEAVED);
+}
+
+}  // namespace
+}  // namespace kvx
+
+using namespace kvx;
+
+extern "C" KVX_API int kvx_rope_frequencies(const kvx_rope_config *cfg, uint64_t *turns, float *amplitude) {
+    if (!cfg || !turns || !amplitude) return KVX_EINVAL;
+    const int d = cfg->rotary_dim, kind = cfg->scaling;
+    if (d < 2 || d % 2 || d > kMaxRopeDim || kind < KVX_ROPE_NONE || kind > KVX_ROPE_YARN) return KVX_EINVAL;
+    if (!(cfg->base > 0) || !std::isfinite(cfg->base)) return KVX_EINVAL;
+    const double factor = kind == KVX_ROPE_NONE ? 1.0 : cfg->factor;
+    if (!(factor >= 1) || !std::isfinite(factor)) return KVX_EINVAL;
+    const bool bands = kind == KVX_ROPE_LLAMA3 || kind == KVX_ROPE_YARN;
+    if (bands && (!(cfg->low > 0) || !(cfg->high > cfg->low) || !std::isfinite(cfg->high) ||
+                  !(cfg->original_context > 0) || !std::isfinite(cfg->original_context)))
+        return KVX_EINVAL;
+    if (kind == KVX_ROPE_YARN && !(cfg->base > 1)) return KVX_EINVAL;
+    constexpr double two_pi = 6.283185307179586476925286766559;
+    double base = cfg->base;
+    if (kind == KVX_ROPE_NTK && d > 2) base *= std::pow(factor, (double)d / (d - 2));
+    double first = 0, last = 0;  // YaRN: pairs the ramp runs between
+    if (kind == KVX_ROPE_YARN) {
+        auto pair_of = [&](double n) { return d * std::log(cfg->original_context / (n * two_pi)) / (2 * std::log(base)); };
+        first = std::max(std::floor(pair_of(cfg->high)), 0.0);
+        last = std::min(std::ceil(pair_of(cfg->low)), (double)(d - 1));
+    }
+    for (int i = 0; i < d / 2; ++i) {
+        double f = std::pow(base, -2.0 * i / d);
+        if (kind == KVX_ROPE_LINEAR) f /= factor;
+        if (kind == KVX_ROPE_LLAMA3) {
+            const double mix = (cfg->original_context * f / two_pi - cfg->low) / (cfg->high - cfg->low);
+            const double m = std::min(std::max(mix, 0.0), 1.0);
+            f = (1 - m) * f / factor + m * f;
+        }
+        if (kind == KVX_ROPE_YARN) {
+            const double r = std::min(std::max((i - first) / std::max(last - first, 0.001), 0.0), 1.0);
+            f = f * (1 - r) + f / factor * r;
+        }
+        // fraction of a turn in units of 2^-64 (whole turns drop out at every
+        // integer position)
+        const long double turn = (long double)f / 6.283185307179586476925286766559L;
+        const long double frac = turn - std::floor(turn);
+        const long double units = std::floor(frac * 18446744073709551616.0L + 0.5L);
+        turns[i] = units >= 18446744073709551616.0L ? 0 : (uint64_t)units;
+    }
+    *amplitude = kind == KVX_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return KVX_OK;
+}
+
+extern "C" KVX_API int kvx_rope(const kvx_rope_table *table, const int32_t *positions, int32_t tokens,
+                                int32_t head_dim, int32_t dtype, const kvx_rope_rows *rows, int32_t num_rows,
+                                int32_t inverse, void *stream) {
+    if (!table || !rows || num_rows < 1 || num_rows > 2 || tokens < 0 || head_dim <= 0) return KVX_EINVAL;
+    if (inverse != 0 && inverse != 1) return KVX_EINVAL;
+    if (dtype != KVX_F16 && dtype != KVX_F32) return KVX_EUNSUPPORTED;
+    if (head_dim > kMaxRopeDim) return KVX_EUNSUPPORTED;
+    if (!table_ok(table, head_dim)) return KVX_EINVAL;
+    const int size = dtype == KVX_F16 ? 2 : 4;
+    const bool half = table->layout == KVX_ROPE_HALF;
+    RopeParams p{};
+    int64_t total = 0;
+    bool vec = rope_vector_sizes(head_dim, table->rotary_dim, half, 16 / size);
+    for (int i = 0; i < num_rows; ++i) {
+        const kvx_rope_rows &r = rows[i];
+        if (r.heads < 0 || r.heads > (1 << 20)) return KVX_EINVAL;
+        if (r.heads == 0 || tokens == 0) continue;
+        if (!r.in || !r.out) return KVX_EINVAL;
+        if (r.in == r.out && (r.in_token_stride != r.out_token_stride || r.in_head_stride != r.out_head_stride))
+            return KVX_EINVAL;
+        const uintptr_t at = reinterpret_cast<uintptr_t>(r.in) | reinterpret_cast<uintptr_t>(r.out);
+        const int64_t strides = r.in_token_stride | r.in_head_stride | r.out_token_stride | r.out_head_stride;
+        if (at & (size - 1)) return KVX_EINVAL;
+        if ((at & 15) || ((strides * size) & 15)) vec = false;
+        p.x[i] = {r.in, r.out, r.heads, r.in_token_stride, r.in_head_stride, r.out_token_stride, r.out_head_stride};
+        total += r.heads;
+    }
+    if (total == 0 || tokens == 0) return KVX_OK;
+    if (!positions) return KVX_EINVAL;
+    p.turns = table->turns;
+    p.positions = positions;
+    p.rotary = table->rotary_dim;
+    p.items = rope_items(head_dim, table->rotary_dim, half, vec ? 16 / size : 1);
+    p.amplitude = table->amplitude;
+    p.sine_sign = inverse ? -1.f : 1.f;
+    // as many threads as one token's rows have items, 256 at most (beyond
+    // that a row has to fit: scalar rows of up to 1024 items)
+    const int64_t want = std::max<int64_t>(p.items, std::min<int64_t>(total * p.items, kRopeThreads));
+    const int threads = (int)((want + 31) / 32 * 32);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dtype == KVX_F16 ? launch_rope<__half>(p, tokens, threads, half, vec, st)
+                            : launch_rope<float>(p, tokens, threads, half, vec, st);
+}
+
+extern "C" KVX_API int kvx_rope_append(const kvx_paged *kv, const int32_t *block_table, int32_t max_pages,
+                                       const int32_t *q_start, const int32_t *positions, int32_t batch,
+                                       int32_t total_tokens, const kvx_rope_table *table, int32_t io_dtype,
+                                       const void *q, int64_t q_stride, void *q_out, int32_t num_q_heads,
+                                       const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                                       int32_t *error_flag, void *stream) {
+    if (!kv || !kv->pool || !block_table || !q_start || !positions) return KVX_EINVAL;
+    if (batch < 0 || total_tokens < 0 || max_pages <= 0 || kv->num_kv_heads <= 0 || kv->num_pages <= 0 ||
+        num_q_heads < 0)
+        return KVX_EINVAL;
+    if (kv->dtype != KVX_F32 && kv->dtype != KVX_F16 && kv->dtype != KVX_I8) return KVX_EINVAL;
+    if (kv->page_tokens != kPageTokens || kv->head_dim != kHeadDim) return KVX_EUNSUPPORTED;
+    if (io_dtype != KVX_F16 && io_dtype != KVX_F32) return KVX_EINVAL;
+    const bool i8 = kv->dtype == KVX_I8;
+    if (!i8 && io_dtype != kv->dtype) return KVX_EUNSUPPORTED;
+    if (i8 && !kv->stats) return KVX_EINVAL;
+    if (kv->num_kv_heads > (1 << 16) || num_q_heads > (1 << 16)) return KVX_EUNSUPPORTED;
+    if (table && !table_ok(table, kHeadDim)) return KVX_EINVAL;
+    if (batch == 0 || total_tokens == 0) return KVX_OK;
+    if (!k || !v || (num_q_heads > 0 && (!q || !q_out))) return KVX_EINVAL;
+    const int size = io_dtype == KVX_F16 ? 2 : 4;
+    if (k_stride < (int64_t)kv->num_kv_heads * kHeadDim || v_stride < (int64_t)kv->num_kv_heads * kHeadDim ||
+        (num_q_heads > 0 && q_stride < (int64_t)num_q_heads * kHeadDim))
+        return KVX_EINVAL;
+    if (num_q_heads > 0 && q == q_out && q_stride != (int64_t)num_q_heads * kHeadDim) return KVX_EINVAL;
+    const int64_t strides = k_stride | v_stride | (num_q_heads > 0 ? q_stride : 0);
+    if (((reinterpret_cast<uintptr_t>(kv->pool) | reinterpret_cast<uintptr_t>(kv->stats) | reinterpret_cast<uintptr_t>(k) |
+          reinterpret_cast<uintptr_t>(v) | (num_q_heads > 0 ? reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) : 0)) &
+         15) ||
+        ((strides * size) & 15))
+        return KVX_EINVAL;
+    RopeAppendParams p{};
+    p.pool = static_cast<uint8_t *>(kv->pool);
+    p.stats = const_cast<float *>(kv->stats);
+    p.block_table = block_table;
+    p.q_start = q_start;
+    p.positions = positions;
+    p.error_flag = error_flag;
+    p.turns = table ? table->turns : nullptr;
+    p.q = q, p.k = k, p.v = v, p.q_out = q_out;
+    p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride;
+    p.batch = batch, p.total = total_tokens, p.hq = num_q_heads, p.hkv = kv->num_kv_heads;
+    p.max_pages = max_pages, p.num_pages = kv->num_pages;
+    const int e = 16 / size;
+    p.rotary = table ? table->rotary_dim : 2 * e;
+    const bool half = table && table->layout == KVX_ROPE_HALF;
+    const bool vec = rope_vector_sizes(kHeadDim, p.rotary, half, e);
+    p.half_layout = half;
+    p.items = rope_items(kHeadDim, p.rotary, half, vec ? e : 1);
+    p.amplitude = table ? table->amplitude : 1.f;
+    // 16 tokens a CTA once their pages alone fill the SMs
+    p.tokens_per_block = total_tokens >= kPageTokens * sm_count() ? kPageTokens : 1;
+    p.kv_blocks = (total_tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return io_dtype == KVX_F16 ? launch_rope_append<__half>(p, i8, half, vec, st)
+                               : launch_rope_append<float>(p, i8, half, vec, st);
+}

@@ -94,7 +94,33 @@ lib.kvx_decode_attn.restype = C.c_int
 lib.kvx_attn_to_metrics.argtypes = [_vp, _vp, _i32, _vp, _i32, _vp, _i32, C.c_uint64, _vp]
 lib.kvx_attn_to_metrics.restype = C.c_int
 lib.kvx_evict_select_composite.argtypes = [_vp, _vp, _i32, _vp, _sz, _f32, _vp, _vp, _vp]
-for _fn in ("kvx_append", "kvx_decode", "kvx_append_decode", "kvx_append_decode_signal", "kvx_stream_wait_geq",
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [("rotary_dim", C.c_int32), ("scaling", C.c_int32), ("base", C.c_double), ("factor", C.c_double),
+                ("low", C.c_double), ("high", C.c_double), ("original_context", C.c_double)]
+
+
+class RopeTableC(C.Structure):
+    _fields_ = [("turns", C.c_void_p), ("rotary_dim", C.c_int32), ("layout", C.c_int32), ("amplitude", C.c_float)]
+
+
+class RopeRows(C.Structure):
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int32), ("in_token_stride", C.c_int64),
+                ("in_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64)]
+
+
+_i64 = C.c_int64
+lib.kvx_rope_frequencies.argtypes = [C.POINTER(RopeConfig), _vp, C.POINTER(C.c_float)]
+lib.kvx_rope.argtypes = [C.POINTER(RopeTableC), _vp, _i32, _i32, _i32, C.POINTER(RopeRows), _i32, _i32, _vp]
+lib.kvx_rope_append.argtypes = [C.POINTER(KvPaged), _vp, _i32, _vp, _vp, _i32, _i32, C.POINTER(RopeTableC), _i32, _vp, _i64,
+                                _vp, _i32, _vp, _i64, _vp, _i64, _vp, _vp]
+lib.kvx_attend_chunk_workspace_bytes.restype = _sz
+lib.kvx_attend_chunk_workspace_bytes.argtypes = [_i32, _i32, _i32, _i32, _i32]
+lib.kvx_attend_chunk.argtypes = [C.POINTER(KvPaged), _vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _f32, _i32, _vp,
+                                 _sz, _vp, _vp]
+for _fn in ("kvx_rope_frequencies", "kvx_rope", "kvx_rope_append", "kvx_attend_chunk",
+            "kvx_append", "kvx_decode", "kvx_append_decode", "kvx_append_decode_signal", "kvx_stream_wait_geq",
             "kvx_decode_workspace_init", "kvx_compress_int8", "kvx_decompress_int8",
             "kvx_compress_nf4", "kvx_decompress_nf4", "kvx_fp16_wrap_encode", "kvx_fp16_wrap_decode",
             "kvx_f32_to_f16_trunc", "kvx_f16_trunc_to_f32", "kvx_lru_select",
@@ -433,3 +459,213 @@ def attn_to_metrics(page_mass, block_table, seq_lens, metrics, current_token, st
                                  block_table.shape[0], _ptr(metrics), metrics.numel() // 48, current_token,
                                  _stream(stream))
     _check("kvx_attn_to_metrics", rc)
+
+
+# ---- rotary positions, ragged append, attention of several new tokens
+
+ROPE_LAYOUT = {"half": 0, "interleaved": 1}
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "llama3": 3, "yarn": 4}
+
+
+def _require(cond, what):
+    if not cond:
+        raise ValueError(what)
+
+
+def _on_device(tensors, stream, call):
+    """call(stream) with the tensors' device current, so that a launch never
+    lands on another device than its operands; stream None: that device's
+    current one."""
+    torch = _torch()
+    dev = tensors[0].device
+    for t in tensors:
+        _require(t is None or t.device == dev and t.is_cuda, "tensors of one call lie on one CUDA device")
+    if dev.index == torch.cuda.current_device():
+        return call(_stream(stream))
+    with torch.cuda.device(dev):
+        return call(_stream(stream))
+
+
+def _vector(t, n, what):
+    """An int32 tensor [n] (n None: any length), contiguous."""
+    torch = _torch()
+    _require(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and (n is None or t.shape[0] == n),
+             f"{what}: contiguous int32 [{'n' if n is None else n}]")
+
+
+def _flag(t):
+    torch = _torch()
+    _require(t is None or t.dtype == torch.int32 and t.numel() >= 1, "error_flag: int32, one element")
+
+
+class RopeTable:
+    """Frequencies of a rotary embedding on the device (see rope_table)."""
+
+    def __init__(self, turns, rotary_dim, layout, amplitude):
+        self.turns, self.rotary_dim, self.layout, self.amplitude = turns, rotary_dim, layout, amplitude
+        self.c = RopeTableC(turns.data_ptr(), rotary_dim, ROPE_LAYOUT[layout], amplitude)
+
+
+def rope_frequencies(rotary_dim, base=10000.0, scaling="none", factor=1.0, low=1.0, high=4.0, original_context=8192.0):
+    """(turns, amplitude): host list of rotary_dim / 2 angles per position in
+    units of 2^-64 turns, and the factor on cosine and sine."""
+    cfg = RopeConfig(rotary_dim, ROPE_SCALING[scaling], base, factor, low, high, original_context)
+    turns, amplitude = (C.c_uint64 * max(rotary_dim // 2, 1))(), C.c_float()
+    _check("kvx_rope_frequencies", lib.kvx_rope_frequencies(C.byref(cfg), turns, C.byref(amplitude)))
+    return list(turns), amplitude.value
+
+
+def rope_table(rotary_dim, base=10000.0, layout="half", scaling="none", factor=1.0, low=1.0, high=4.0,
+               original_context=8192.0, device="cuda"):
+    """Frequencies base^(-2i/rotary_dim), scaled for long contexts: "linear",
+    "ntk", "llama3" (low / high: turns within original_context between which
+    factor fades in) or "yarn" (low / high likewise, commonly 1 and 32)."""
+    torch = _torch()
+    _require(layout in ROPE_LAYOUT, f"layout: one of {sorted(ROPE_LAYOUT)}")
+    _require(scaling in ROPE_SCALING, f"scaling: one of {sorted(ROPE_SCALING)}")
+    turns, amplitude = rope_frequencies(rotary_dim, base, scaling, factor, low, high, original_context)
+    signed = [t - (1 << 64) if t >> 63 else t for t in turns]
+    return RopeTable(torch.tensor(signed, dtype=torch.int64).to(device), rotary_dim, layout, amplitude)
+
+
+def _rows3(x, what, like=None):
+    _require(x.dim() == 3 and (x.shape[2] <= 1 or x.stride(2) == 1), f"{what}: [tokens][heads][dim], last dimension contiguous")
+    _require(like is None or (x.shape == like.shape and x.dtype == like.dtype), f"{what}: shape and dtype of its input")
+
+
+def _single(x, what):
+    """No two elements of an output share memory by a stride of zero."""
+    _require(all(n <= 1 or st != 0 for n, st in zip(x.shape, x.stride())), f"{what}: strides without overlap")
+
+
+def rope(q, k, positions, table, q_out=None, k_out=None, inverse=False, stream=None):
+    """Rotate q [tokens][hq][dim] and k [tokens][hk][dim] (k may be None) by
+    positions [tokens] (int32); any token and head strides.  q_out = q rotates
+    in place.  inverse=True turns back, which is the gradient of the rotation.
+    Returns (q_out, k_out)."""
+    torch = _torch()
+    _rows3(q, "q")
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _rows3(q_out, "q_out", q)
+    _single(q_out, "q_out")
+    tokens, _, dim = q.shape
+    if k is not None:
+        _rows3(k, "k")
+        _require(k.shape[0] == tokens and k.shape[2] == dim and k.dtype == q.dtype, "k: tokens, dim and dtype of q")
+        if k_out is None:
+            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        _rows3(k_out, "k_out", k)
+        _single(k_out, "k_out")
+    _vector(positions, tokens, "positions")
+    rows = (RopeRows * 2)()
+    n = 0
+    for x, o in ((q, q_out), (k, k_out)):
+        if x is not None:
+            rows[n] = RopeRows(x.data_ptr(), o.data_ptr(), x.shape[1], x.stride(0), x.stride(1), o.stride(0), o.stride(1))
+            n += 1
+    _require(q.dtype in (torch.float16, torch.float32), "q: float16 or float32")
+    rc = _on_device((q, q_out, k, k_out, positions, table.turns), stream,
+                    lambda st: lib.kvx_rope(C.byref(table.c), _ptr(positions), tokens, dim, _dtype_code(q), rows, n,
+                                            int(bool(inverse)), st))
+    _check("kvx_rope", rc)
+    return q_out, k_out
+
+
+def _packed(x, heads, what):
+    """[tokens][heads][128] with the heads of a token side by side."""
+    _require(x.dim() == 3 and x.shape[2] == HEAD_DIM and (heads is None or x.shape[1] == heads) and
+             (x.shape[0] == 0 or (x.stride(2) == 1 and (x.shape[1] <= 1 or x.stride(1) == HEAD_DIM))),
+             f"{what}: [tokens][heads][128], heads side by side")
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * HEAD_DIM
+
+
+def _ragged(block_table, q_start, positions):
+    torch = _torch()
+    _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.is_contiguous(),
+             "block_table: contiguous int32 [batch][max_pages]")
+    batch = block_table.shape[0]
+    _vector(positions, batch, "positions")
+    _vector(q_start, batch + 1, "q_start")
+    return batch
+
+
+def _pool_tensors(pool, stats):
+    """paged(pool, stats) and the tensors behind it."""
+    torch = _torch()
+    kv = paged(pool, stats)
+    _require(kv.dtype != KVX_I8 or kv.stats, "stats: an int8 pool has them")
+    if stats is not None and not isinstance(pool, KvPaged):
+        _require(stats.dtype == torch.float32 and stats.is_contiguous() and
+                 tuple(stats.shape) == (kv.num_pages, 2, kv.num_kv_heads, 4), "stats: contiguous float32 [pages][2][hkv][4]")
+    return kv, (None if isinstance(pool, KvPaged) else pool, stats)
+
+
+def rope_append(pool, block_table, q_start, positions, k, v, q=None, q_out=None, table=None, stats=None, error_flag=None,
+                stream=None):
+    """Rotate and append a ragged batch: packed rows q_start[s] ..
+    q_start[s+1]-1 of k, v ([tokens][hkv][128]) and q ([tokens][hq][128] or
+    None) belong to sequence s and start at position positions[s].  k is
+    rotated and stored with v in the pages (int8 pools: quantised, stats
+    updated); q is rotated into q_out, which is returned.  table None: no
+    rotation."""
+    torch = _torch()
+    kv, tensors = _pool_tensors(pool, stats)
+    batch = _ragged(block_table, q_start, positions)
+    tokens = k.shape[0]
+    ks, vs = _packed(k, kv.num_kv_heads, "k"), _packed(v, kv.num_kv_heads, "v")
+    _require(v.shape[0] == tokens and v.dtype == k.dtype and k.dtype in (torch.float16, torch.float32),
+             "k, v: as many tokens, both float16 or float32")
+    hq = qs = 0
+    if q is not None:
+        qs, hq = _packed(q, None, "q"), q.shape[1]
+        _require(q.shape[0] == tokens and q.dtype == k.dtype, "q: tokens and dtype of k")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _require(q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.is_contiguous(), "q_out: contiguous, shape and dtype of q")
+    else:
+        _require(q_out is None, "q_out: only with q")
+    _flag(error_flag)
+    rc = _on_device((k, v, q, q_out, block_table, q_start, positions, error_flag, None if table is None else table.turns) + tensors,
+                    stream,
+                    lambda st: lib.kvx_rope_append(
+                        C.byref(kv), _ptr(block_table), block_table.shape[1], _ptr(q_start), _ptr(positions), batch, tokens,
+                        None if table is None else C.byref(table.c), _dtype_code(k), _ptr(q), qs, _ptr(q_out), hq, _ptr(k), ks,
+                        _ptr(v), vs, _ptr(error_flag), st))
+    _check("kvx_rope_append", rc)
+    return q_out
+
+
+def attend_chunk_workspace(batch, total_tokens, num_q_heads, num_kv_heads, max_pages, device="cuda"):
+    """Scratch of attend_chunk for calls up to this size (no initialisation needed)."""
+    torch = _torch()
+    n = lib.kvx_attend_chunk_workspace_bytes(batch, total_tokens, num_q_heads, num_kv_heads, max_pages)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+
+
+def attend_chunk(pool, block_table, q_start, positions, q, stats=None, out=None, workspace=None, error_flag=None,
+                 sm_scale=0.0, causal=True, stream=None):
+    """Attention of a ragged batch of new tokens over an int8 pool that holds
+    them already: packed rows q [tokens][hq][128] as in rope_append; the query
+    at position p sees keys 0 .. p (causal=False: every key of its sequence,
+    positions[s] + its new tokens)."""
+    torch = _torch()
+    kv, tensors = _pool_tensors(pool, stats)
+    batch = _ragged(block_table, q_start, positions)
+    _require(q.dim() == 3 and q.shape[2] == HEAD_DIM and q.is_contiguous() and q.dtype in (torch.float16, torch.float32),
+             "q: contiguous float16 or float32 [tokens][hq][128]")
+    tokens, hq, _ = q.shape
+    if out is None:
+        out = torch.zeros_like(q)
+    _require(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "out: contiguous, shape and dtype of q")
+    if workspace is None:
+        workspace = attend_chunk_workspace(batch, tokens, hq, kv.num_kv_heads, block_table.shape[1], q.device)
+    _require(workspace.is_contiguous(), "workspace: contiguous")
+    _flag(error_flag)
+    rc = _on_device((q, out, block_table, q_start, positions, workspace, error_flag) + tensors, stream,
+                    lambda st: lib.kvx_attend_chunk(
+                        C.byref(kv), _ptr(block_table), block_table.shape[1], _ptr(q_start), _ptr(positions), batch, tokens, hq,
+                        _ptr(q), _ptr(out), _dtype_code(q), sm_scale, int(bool(causal)), _ptr(workspace),
+                        workspace.numel() * workspace.element_size(), _ptr(error_flag), st))
+    _check("kvx_attend_chunk", rc)
+    return out

@@ -352,6 +352,176 @@ KVX_API int kvx_migrate_frames(void *dev_base, int32_t dev_capacity, void *host_
                                size_t frame_bytes, int32_t direction, int32_t ctas,
                                int32_t *error_flag, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * Rotary positions.  Additive: the reference's runtime leaves them to its
+ * model loaders.  Pair i of a row's first rotary_dim elements turns by
+ * positions[t] * f_i, times an amplitude:
+ *     (a, b) -> amplitude * (a cos - b sin, b cos + a sin)
+ * with (a, b) = (x[i], x[i + rotary_dim/2]) in the half layout and
+ * (x[2i], x[2i+1]) in the interleaved one; later elements pass unchanged.
+ * f_i is held as a fraction of a turn per position in units of 2^-64, so
+ * position * f_i modulo one turn is an exact integer product at any int32
+ * position (negative ones too). */
+enum kvx_rope_layout { KVX_ROPE_HALF = 0, KVX_ROPE_INTERLEAVED = 1 };
+enum kvx_rope_scaling {
+    KVX_ROPE_NONE = 0,   /* f_i = base^(-2i/d) radians, d = rotary_dim */
+    KVX_ROPE_LINEAR = 1, /* f_i / factor */
+    KVX_ROPE_NTK = 2,    /* base * factor^(d/(d-2)) in place of base (d > 2) */
+    KVX_ROPE_LLAMA3 = 3, /* f/factor below `low` turns in original_context, f above `high`, mixed between */
+    KVX_ROPE_YARN = 4    /* f above `high` turns, f/factor below `low`, a ramp over i between; amplitude
+                            0.1 ln(factor) + 1 */
+};
+typedef struct kvx_rope_config {
+    int32_t rotary_dim;      /* even, 2..1024 */
+    int32_t scaling;         /* enum kvx_rope_scaling */
+    double base;             /* > 0; > 1 for KVX_ROPE_YARN */
+    double factor;           /* >= 1 (not read for KVX_ROPE_NONE) */
+    double low, high;        /* LLAMA3, YARN: turns within original_context, 0 < low < high */
+    double original_context; /* LLAMA3, YARN: > 0 */
+} kvx_rope_config;
+/* Host: turns[rotary_dim/2] (2^-64 turns per position) and the amplitude. */
+KVX_API int kvx_rope_frequencies(const kvx_rope_config *cfg, uint64_t *turns, float *amplitude);
+
+typedef struct kvx_rope_table {
+    const uint64_t *turns; /* device, [rotary_dim/2] */
+    int32_t rotary_dim;    /* even, <= head_dim */
+    int32_t layout;        /* enum kvx_rope_layout */
+    float amplitude;
+} kvx_rope_table;
+
+/* Rows of one tensor [tokens][heads][head_dim] with the last dimension
+ * contiguous; strides in elements, of either sign or zero for the input.
+ * out may be in with the same strides (in place); otherwise the two do not
+ * overlap. */
+typedef struct kvx_rope_rows {
+    const void *in;
+    void *out;
+    int32_t heads;
+    int64_t in_token_stride, in_head_stride, out_token_stride, out_head_stride;
+} kvx_rope_rows;
+
+/* Rotate num_rows (1 or 2: queries and keys) tensors of `tokens` tokens in
+ * one launch.  positions: device int32 [tokens].  dtype KVX_F16 / KVX_F32;
+ * products in fp32, one rounding to fp16.  inverse = 1 turns the other way
+ * with the same amplitude, which is the gradient of the rotation.  head_dim
+ * up to 1024. */
+KVX_API int kvx_rope(const kvx_rope_table *table, const int32_t *positions, int32_t tokens,
+                     int32_t head_dim, int32_t dtype, const kvx_rope_rows *rows, int32_t num_rows,
+                     int32_t inverse, void *stream);
+
+/* Rotate and append a ragged batch.  Tokens of all sequences lie packed:
+ * sequence s owns rows q_start[s] .. q_start[s+1]-1 (device int32
+ * [batch + 1], ascending), its first token at position positions[s] (device
+ * int32 [batch]).  Rows outside every sequence are neither read nor written.
+ * q (NULL with num_q_heads 0): [total_tokens][num_q_heads][128] is rotated
+ * into q_out (contiguous; q_out may be q when q is contiguous); k, v:
+ * [total_tokens][num_kv_heads][128]; k is rotated, then k and v are stored in
+ * the pages of the block table.  *_stride: elements between tokens (at least
+ * heads * 128); every row 16-byte aligned.  table NULL: no rotation.
+ *
+ * KVX_F16 / KVX_F32 pools (io_dtype the pool's): the bits of kvx_rope, then
+ * kvx_append.  KVX_I8 pools (io_dtype KVX_F16 or KVX_F32; kv->stats is
+ * written): the new rows of a page join its (K|V, head) block: min and max
+ * become those of the new rows' fp32 values (keys after the rotation) and,
+ * when rows before them lie in the page, of the block's statistics; scale =
+ * (max - min) / 255 (0 -> 1), zeroPoint = min, codes as kvx_compress_int8.
+ * Earlier rows keep their codes when min and max stay, else their values are
+ * quantised anew (each widening rounds them once more, by half a step).  Rows
+ * behind the last new one keep their codes.  NaN does not enter min and max.
+ *
+ * A negative position, or a page outside block table or pool, skips those
+ * rows of k and v and sets bit 1 of *error_flag (may be NULL); q is rotated
+ * all the same.  Two sequences of one call may not append to the same page. */
+KVX_API int kvx_rope_append(const kvx_paged *kv, const int32_t *block_table, int32_t max_pages,
+                            const int32_t *q_start, const int32_t *positions, int32_t batch,
+                            int32_t total_tokens, const kvx_rope_table *table, int32_t io_dtype,
+                            const void *q, int64_t q_stride, void *q_out, int32_t num_q_heads,
+                            const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                            int32_t *error_flag, void *stream);
+
+/* Attention of a ragged batch of new tokens over an int8 pool (a prompt
+ * chunk, drafted tokens to check, mixed batches); kvx_decode with several
+ * queries per sequence.  Packed rows, q_start and positions as in
+ * kvx_rope_append, whose rows are in the pages already: the query at
+ * position p sees keys 0 .. p (causal = 1) or all positions[s] + n keys of
+ * its sequence (causal = 0).  q/out: [total_tokens][num_q_heads][128],
+ * contiguous, 16-byte aligned, io_dtype KVX_F16 or KVX_F32; q-head h reads
+ * kv-head h / (num_q_heads/num_kv_heads).  sm_scale <= 0 means 1/sqrt(128).
+ * Pages outside the pool are left out (bit 1 of *error_flag), keys past the
+ * block table too (bit 2), a sequence of negative position altogether (bit
+ * 1); a query that sees no key gives a zero row.  Output rows outside every
+ * sequence keep what they hold.  Accumulation and softmax in fp32; fp16
+ * calls round the probabilities to fp16 for the second product.  workspace:
+ * kvx_attend_chunk_workspace_bytes(), 16-byte aligned, needs no
+ * initialisation; calls that share one are ordered. */
+KVX_API size_t kvx_attend_chunk_workspace_bytes(int32_t batch, int32_t total_tokens,
+                                                int32_t num_q_heads, int32_t num_kv_heads,
+                                                int32_t max_pages);
+KVX_API int kvx_attend_chunk(const kvx_paged *kv, const int32_t *block_table, int32_t max_pages,
+                             const int32_t *q_start, const int32_t *positions, int32_t batch,
+                             int32_t total_tokens, int32_t num_q_heads, const void *q, void *out,
+                             int32_t io_dtype, float sm_scale, int32_t causal, void *workspace,
+                             size_t workspace_bytes, int32_t *error_flag, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Page bookkeeping on the device: who holds which page of the pools.
+ * refcounts[p] counts the block-table entries that name page p (0: free).  A
+ * row's pages fill a prefix of its block-table entries, the others are -1;
+ * seq_lens[row] tokens of them are in use.  Pages are always taken lowest id
+ * first, so results do not depend on timing.  `layers`: host array of the
+ * num_layers pools that share the block table (same geometry and dtype;
+ * KVX_I8 pools with their stats, which move with the page).  Calls that share
+ * a table or a workspace are ordered (one stream); the workspace needs no
+ * initialisation.  A refused call changes nothing and sets a bit of
+ * *error_flag (device int32, may be NULL): bit 1 a row or page id out of
+ * range, bit 2 more tokens than a block-table row holds, bit 3 too few free
+ * pages, bit 4 a row given twice, or a child that is not empty. */
+typedef struct kvx_pages {
+    int32_t *refcounts;   /* [num_pages] */
+    int32_t *block_table; /* [num_rows][max_pages] */
+    int32_t *seq_lens;    /* [num_rows] */
+    int32_t num_pages, num_rows, max_pages;
+} kvx_pages;
+KVX_API size_t kvx_pages_workspace_bytes(int32_t num_pages, int32_t num_rows);
+
+/* Give every row the pages that its next new_tokens[row] tokens (device int32
+ * [num_rows], >= 0) need: entries below ceil((seq_lens + new_tokens) / 16)
+ * that are still -1, rows in order.  seq_lens stays. */
+KVX_API int kvx_pages_reserve(const kvx_pages *pages, const int32_t *new_tokens, void *workspace,
+                              size_t workspace_bytes, int32_t *error_flag, void *stream);
+
+/* Make row children[i] (empty, distinct) a copy of row parents[i] (device
+ * int32 [n]) for i < n: full pages are shared, a last page that is only
+ * partly used is copied into a page of the child's own in every layer, so
+ * both can append.  Pages reserved past the parent's length stay its own.  A
+ * full page's entry that names no page is -1 in the child (bit 1). */
+KVX_API int kvx_pages_fork(const kvx_pages *pages, const kvx_paged *layers, int32_t num_layers,
+                           const int32_t *parents, const int32_t *children, int32_t n,
+                           void *workspace, size_t workspace_bytes, int32_t *error_flag, void *stream);
+
+/* Drop every page of rows[0..n) (device int32): entries become -1, seq_lens
+ * 0, counts fall by one each.  A row given twice is freed once.  A row id out
+ * of range is skipped (bit 1), as is an entry whose page is out of range or
+ * has no count. */
+KVX_API int kvx_pages_free(const kvx_pages *pages, const int32_t *rows, int32_t n, int32_t *error_flag,
+                           void *stream);
+
+/* Move the held pages with the highest ids into the lowest free ones until
+ * the pages 0 .. live-1 are held and the rest free: the i-th held page with
+ * id >= live (ascending) goes to the i-th free page with id < live.  Contents
+ * move in every layer, the whole block table and refcounts follow, *num_live
+ * (device int32, may be NULL) receives live.  A block-table entry that names
+ * a free or unknown page stays (bit 1). */
+KVX_API int kvx_pages_compact(const kvx_pages *pages, const kvx_paged *layers, int32_t num_layers,
+                              void *workspace, size_t workspace_bytes, int32_t *num_live,
+                              int32_t *error_flag, void *stream);
+
+/* Copy page src[i] to page dst[i] (device int32 [n]) in every layer.  The
+ * dst are distinct and none is a src of another pair; src[i] == dst[i] does
+ * nothing.  A pair with an id out of range is skipped (bit 1). */
+KVX_API int kvx_pages_copy(const kvx_paged *layers, int32_t num_layers, const int32_t *src,
+                           const int32_t *dst, int32_t n, int32_t *error_flag, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
