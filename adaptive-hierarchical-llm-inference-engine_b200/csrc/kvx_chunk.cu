@@ -13,7 +13,7 @@
 // major.  A CTA owns a tile of rows and a range of 128-key tiles (8 pages):
 //  * loader warp: a bulk copy (TMA) per page and K|V, 2 KB of codes each, into
 //    staging slots;
-//  * 4 convert warps: codes -> fp16 into the 128-byte-swizzled K and V tiles
+//  * 4 convert warps (2 for K, 2 for V): codes -> fp16 into the 128-byte-swizzled K and V tiles
 //    (K: the K-major B operand of Q K^T; V: the MN-major B operand of P V,
 //    the same bytes), two stages each;
 //  * MMA warp: one thread issues S = Q K^T (M 128, N 128, 8 steps of K 16)
@@ -43,7 +43,12 @@ namespace {
 
 constexpr int kTileKeys = 128, kTilePages = kTileKeys / kPageTokens;
 constexpr int kBlockBytes = kPageTokens * kHeadDim;  // codes of one (page, K|V, head)
-constexpr int kConvertWarp = 8, kMmaWarp = 12, kLoadWarp = 13, kChunkThreads = 14 * 32;
+constexpr int kConvertWarp = 8, kMmaWarp = 12, kLoadWarp = 13, kChunkThreads = 16 * 32;
+// registers a thread, by warpgroup (setmaxnreg): 2 x 128 x 184 + 128 x 80 +
+// 128 x 64 = the 512 x 128 of the launch.  A softmax thread holds its 128
+// scores from the maximum to the exponentials.
+constexpr int kSoftmaxRegs = 184, kConvertRegs = 80, kIssueRegs = 64;
+static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs == 4 * 128, "the launch's registers, dealt out");
 constexpr int kTileBytes = 128 * kHeadDim * 2;  // an fp16 tile of Q, K or V: two halves of 64 dims
 constexpr int kHalfBytes = kTileBytes / 2, kSlotBytes = kTileKeys * kHeadDim;
 // shared memory: Q0, Q1 (staging slots 2, 3 when unused), K x 2, V x 2, staging x 2, the rest
@@ -128,6 +133,11 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, 
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ void umma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -136,6 +146,11 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+}
 __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
@@ -144,9 +159,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at) : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at) : "memory");
-}
 
 // 2^x on the special-function unit (2^-inf = +0)
 __device__ __forceinline__ float ex2(float x) {
@@ -154,6 +166,36 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// Two floats side by side: the packed fp32 operations of sm_100.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+template <int kRegs> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 
@@ -264,12 +306,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     if (threadIdx.x == 32) {
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bars->ld_full[i], 1);
-            mbar_init(&bars->ld_empty[i], 4);
+            mbar_init(&bars->ld_empty[i], 2);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&bars->k_full[i], 4);
+            mbar_init(&bars->k_full[i], 2);
             mbar_init(&bars->k_empty[i], 1);
-            mbar_init(&bars->v_full[i], 4);
+            mbar_init(&bars->v_full[i], 2);
             mbar_init(&bars->v_empty[i], 1);
             mbar_init(&bars->s_full[i], 1);
             mbar_init(&bars->p_full[i], 128);
@@ -301,7 +343,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     const int t0 = split * p.chunk, tiles = min(p.chunk, rt.tiles - t0);  // this CTA's key tiles
     const bool turns = kSplit || rt.rows <= 128;  // the warpgroups take turns at the key tiles
     const int items = turns ? tiles : 2 * tiles;  // item w: warpgroup w % 2, key tile w or w / 2
-    const int slots = turns && !kSplit ? 4 : 2;
+    const int slot_bits = turns && !kSplit ? 2 : 1, slot_mask = (1 << slot_bits) - 1;  // 4 or 2 staging slots
     const int32_t *table = p.block_table + (size_t)seq * p.max_pages;
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&bars->tmem)) : "memory");
@@ -313,77 +355,56 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     const uint32_t tmem = bars->tmem;  // S0, S1, O0, O1: 128 columns each
     auto slot_at = [&](int s) { return s < 2 ? kAtStage + s * kSlotBytes : kTileBytes + (s - 2) * kSlotBytes; };
 
-    if (warp == kLoadWarp) {
-        // ---- loader: lane i < 8 copies page i of the tile's K, then V codes
-        for (int i = 0; i < tiles; ++i) {
-            const int lp = (t0 + i) * kTilePages + (lane & 7);
-            const bool want = lane < 8 && lp * kPageTokens < rt.keys;
-            const int phys = want ? table[lp] : -1;
-            const bool have = phys >= 0 && phys < p.num_pages;
-            if (want && !have && p.error_flag) atomicOr(p.error_flag, 2);
-            const uint32_t known = __ballot_sync(0xffffffffu, have);
-            for (int kv = 0; kv < 2; ++kv) {
-                const int u = 2 * i + kv, s = u % slots;
-                wait_or_give_up(&bars->ld_empty[s], ((u / slots) & 1) ^ 1, bars, p.error_flag);
-                if (lane == 0) {
-                    bars->known[s] = known;
-                    mbar_arrive_expect_tx(&bars->ld_full[s], __popc(known) * kBlockBytes);
+    if (warp >= kMmaWarp) {
+        fewer_registers<kIssueRegs>();
+        if (warp == kLoadWarp) {
+            // ---- loader: lane i < 8 copies page i of the tile's K, then V codes
+            for (int i = 0; i < tiles; ++i) {
+                const int lp = (t0 + i) * kTilePages + (lane & 7);
+                const bool want = lane < 8 && lp * kPageTokens < rt.keys;
+                const int phys = want ? table[lp] : -1;
+                const bool have = phys >= 0 && phys < p.num_pages;
+                if (want && !have && p.error_flag) atomicOr(p.error_flag, 2);
+                const uint32_t known = __ballot_sync(0xffffffffu, have);
+                for (int kv = 0; kv < 2; ++kv) {
+                    const int u = 2 * i + kv, s = u & slot_mask;
+                    wait_or_give_up(&bars->ld_empty[s], (u >> slot_bits & 1) ^ 1, bars, p.error_flag);
+                    if (lane == 0) {
+                        bars->known[s] = known;
+                        mbar_arrive_expect_tx(&bars->ld_full[s], __popc(known) * kBlockBytes);
+                    }
+                    __syncwarp();
+                    if (have)
+                        bulk_g2s(sm + slot_at(s) + lane * kBlockBytes,
+                                 p.pool + (((size_t)phys * 2 + kv) * p.hkv + kvh) * kBlockBytes, kBlockBytes, &bars->ld_full[s]);
                 }
-                __syncwarp();
-                if (have)
-                    bulk_g2s(sm + slot_at(s) + lane * kBlockBytes,
-                             p.pool + (((size_t)phys * 2 + kv) * p.hkv + kvh) * kBlockBytes, kBlockBytes, &bars->ld_full[s]);
             }
-        }
-        // no copy is in flight when the CTA ends, however it ends
-        for (int u = max(0, 2 * tiles - slots); u < 2 * tiles; ++u)
-            (void)mbar_wait_bounded(&bars->ld_full[u % slots], (u / slots) & 1, nullptr);
-    } else if (warp >= kConvertWarp && warp < kMmaWarp) {
-        // ---- convert: per step, 8 lanes take row r (even) chunks 0-3 and row
-        // r + 1 chunks 4-7: reads of 128 contiguous bytes, writes to 8
-        // different 16-byte banks
-        const int tid = threadIdx.x - 32 * kConvertWarp;
-        for (int u = 0; u < 2 * tiles; ++u) {
-            const int i = u >> 1, kv = u & 1, s = u % slots, st = i & 1;
-            wait_or_give_up(&bars->ld_full[s], (u / slots) & 1, bars, p.error_flag);
-            wait_or_give_up(kv ? &bars->v_empty[st] : &bars->k_empty[st], ((i >> 1) & 1) ^ 1, bars, p.error_flag);
-            const uint32_t known = bars->known[s];
-            const uint8_t *src = sm + slot_at(s);
-            const uint32_t dst = base + (kv ? kAtV : kAtK) + st * kTileBytes;
-            const int g = tid >> 3, j = tid & 7;  // group of 8 lanes: 16 groups
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int pair = (g + 16 * (k >> 1)), swap = k & 1;  // rows 2 pair, 2 pair + 1
-                const int r = 2 * pair + ((j >> 2) ^ swap), c = j;
-                uint4 w = *reinterpret_cast<const uint4 *>(src + r * 128 + c * 16);
-                if (!(known >> (r >> 4) & 1)) w = make_uint4(0, 0, 0, 0);
-                const uint2 a = codes_to_half(w.x), b = codes_to_half(w.y), d = codes_to_half(w.z), e = codes_to_half(w.w);
-                st_shared16(dst + tile_chunk(r, 2 * c), a.x, a.y, b.x, b.y);
-                st_shared16(dst + tile_chunk(r, 2 * c + 1), d.x, d.y, e.x, e.y);
-            }
-            fence_proxy_async_smem();  // before the tensor core's reads, and the next copy into the slot
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&bars->ld_empty[s]);
-                mbar_arrive(kv ? &bars->v_full[st] : &bars->k_full[st]);
-            }
-        }
-    } else if (warp == kMmaWarp) {
-        if (lane == 0) {
+            // no copy is in flight when the CTA ends, however it ends
+            for (int u = max(0, 2 * tiles - slot_mask - 1); u < 2 * tiles; ++u)
+                (void)mbar_wait_bounded(&bars->ld_full[u & slot_mask], u >> slot_bits & 1, nullptr);
+        } else if (warp == kMmaWarp) {
+            // the whole warp walks the items (uniform addresses and
+            // descriptors stay in uniform registers), one lane issues
+            const bool issues = elect_one();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             auto scores = [&](int w) {
                 const int i = turns ? w : w >> 1, j = w & 1, st = i & 1;
                 wait_or_give_up(&bars->k_full[st], (i >> 1) & 1, bars, p.error_flag);
                 tc_fence_after();
-                const uint32_t q = base + (turns ? 0 : j * kTileBytes), k = base + kAtK + st * kTileBytes;
-                for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+                if (issues) {
+                    const uint64_t q = umma_desc(base + (turns ? 0 : j * kTileBytes), 16, 1024),
+                                   k = umma_desc(base + kAtK + st * kTileBytes, 16, 1024);
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        const uint32_t off = (ks >> 2) * kHalfBytes + (ks & 3) * 32;
-                        umma_f16_ss(tmem + j * 128, umma_desc(q + part * kTileBytes + off, 16, 1024),
-                                    umma_desc(k + off, 16, 1024), kIdescQK, part | ks);
-                    }
-                umma_commit(&bars->s_full[j]);
-                if (turns || j) umma_commit(&bars->k_empty[st]);
+                    for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks) {  // addresses in a descriptor count 16 bytes
+                            const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                            umma_f16_ss(tm + j * 128, q + (part * kTileBytes >> 4) + off, k + off, kIdescQK, part | ks);
+                        }
+                    umma_commit(&bars->s_full[j]);
+                    if (turns || j) umma_commit(&bars->k_empty[st]);
+                }
+                __syncwarp();
             };
             wait_or_give_up(&bars->q_full, 0, bars, p.error_flag);
             scores(0);
@@ -393,19 +414,60 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 wait_or_give_up(&bars->v_full[st], (i >> 1) & 1, bars, p.error_flag);
                 wait_or_give_up(&bars->p_full[j], (w >> 1) & 1, bars, p.error_flag);
                 tc_fence_after();
-                const uint32_t v = base + kAtV + st * kTileBytes;
-                for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+                if (issues) {
+                    const uint64_t v = umma_desc(base + kAtV + st * kTileBytes, kHalfBytes, 1024);
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)  // 16 keys: P over S's columns 32 (ks/2) .., half of them
-                        umma_f16_ts(tmem + 256 + j * 128, tmem + j * 128 + (ks >> 1) * 32 + (ks & 1) * 8 + part * 16,
-                                    umma_desc(v + ks * 2048, kHalfBytes, 1024), kIdescPV, (w > 1) | part | ks);
-                if (turns || j) umma_commit(&bars->v_empty[st]);
+                    for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks)  // 16 keys: P over S's columns 32 (ks/2) .., half of them
+                            umma_f16_ts(tm + 256 + j * 128, tm + j * 128 + (ks >> 1) * 32 + (ks & 1) * 8 + part * 16,
+                                        v + (ks * 2048 >> 4), kIdescPV, (w > 1) | part | ks);
+                    if (turns || j) umma_commit(&bars->v_empty[st]);
+                }
+                __syncwarp();
                 if (w + 2 < items) scores(w + 2);
             }
-            umma_commit(&bars->done);
+            if (issues) umma_commit(&bars->done);
+            __syncwarp();
         }
-        __syncwarp();
-    } else if (warp < kConvertWarp) {
+    } else if (warp >= kConvertWarp) {
+        fewer_registers<kConvertRegs>();
+        // ---- convert: two warps take the K codes, two the V codes.  8 lanes
+        // take row r (even) chunks 0-3 and row r + 1 chunks 4-7: reads of 128
+        // contiguous bytes, writes to 8 different 16-byte banks
+        const int kv = warp & 1, g = (warp & 2) * 2 + (lane >> 3), j = lane & 7;  // groups 0..7 of 8 lanes
+        for (int i = 0; i < tiles; ++i) {
+            const int u = 2 * i + kv, s = u & slot_mask, st = i & 1;
+            wait_or_give_up(&bars->ld_full[s], u >> slot_bits & 1, bars, p.error_flag);
+            const uint32_t known = bars->known[s];
+            const uint8_t *src = sm + slot_at(s);
+            const uint32_t dst = base + (kv ? kAtV : kAtK) + st * kTileBytes;
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                auto row_of = [&](int k) { return 2 * (g + 8 * (k >> 1) + 32 * part) + ((j >> 2) ^ (k & 1)); };
+                uint4 w[8];  // all loads before the first store
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const uint4 *>(src + row_of(k) * 128 + j * 16);
+                if (part == 0) wait_or_give_up(kv ? &bars->v_empty[st] : &bars->k_empty[st], ((i >> 1) & 1) ^ 1, bars, p.error_flag);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int r = row_of(k);
+                    if (!(known >> (r >> 4) & 1)) w[k] = make_uint4(0, 0, 0, 0);
+                    const uint2 a = codes_to_half(w[k].x), b = codes_to_half(w[k].y), d = codes_to_half(w[k].z),
+                                e = codes_to_half(w[k].w);
+                    st_shared16(dst + tile_chunk(r, 2 * j), a.x, a.y, b.x, b.y);
+                    st_shared16(dst + tile_chunk(r, 2 * j + 1), d.x, d.y, e.x, e.y);
+                }
+            }
+            fence_proxy_async_smem();  // before the tensor core's reads, and the next copy into the slot
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&bars->ld_empty[s]);
+                mbar_arrive(kv ? &bars->v_full[st] : &bars->k_full[st]);
+            }
+        }
+    } else {
+        more_registers<kSoftmaxRegs>();
         // ---- softmax: thread = row
         const int j = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -500,28 +562,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             wait_or_give_up(&bars->s_full[j], (w >> 1) & 1, bars, p.error_flag);
             __syncwarp();
             tc_fence_after();
+            uint32_t x[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, x[c]);
+            tmem_wait_ld();
+            if (masked) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        if (32 * c + k >= seen || !(known >> (2 * c + (k >> 4)) & 1)) x[c][k] = 0xff800000u;  // -inf
+            }
+            // a page this row sees nothing of: every score -inf, whatever its statistics
+            auto hidden = [&](int page) { return masked && (seen <= page * kPageTokens || !(known >> page & 1)); };
             float top = -CUDART_INF_F;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t x[32];
-                tmem_ld32(t_s + 32 * c, x);
-                tmem_wait_ld();
+            for (int page = 0; page < kTilePages; ++page) {
+                const float2 ks = rows[page];
+                float big = -CUDART_INF_F;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float2 ks = rows[2 * c + h];
-                    float big = -CUDART_INF_F;
-                    if (masked) {
-                        const int n = known >> (2 * c + h) & 1 ? seen - (2 * c + h) * kPageTokens : 0;
-#pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            if (k < n) big = fmaxf(big, __uint_as_float(x[16 * h + k]));
-                        if (n > 0) top = fmaxf(top, fmaf(ks.x * unscale, big, ks.y * q_sum));
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) big = fmaxf(big, __uint_as_float(x[16 * h + k]));
-                        top = fmaxf(top, fmaf(ks.x * unscale, big, ks.y * q_sum));
-                    }
-                }
+                for (int k = 0; k < 16; ++k) big = fmaxf(big, __uint_as_float(x[page >> 1][16 * (page & 1) + k]));
+                if (!hidden(page)) top = fmaxf(top, fmaf(ks.x * unscale, big, ks.y * q_sum));
             }
             if (w < 2) {
                 m = top;
@@ -532,51 +593,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 l *= f;
                 z *= f;
                 const float fo = f * shrink;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32];
-                    tmem_ld32(t_o + 32 * c, x);
+#pragma unroll 1
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t o[16];
+                    tmem_ld16(t_o + 16 * c, o);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * fo);
-                    tmem_st32(t_o + 32 * c, x);
+                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fo);
+                    tmem_st16(t_o + 16 * c, o);
                 }
             }
             const float m_use = m == -CUDART_INF_F ? 0.f : m;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                uint32_t x[32], hi[16], lo[16];
-                tmem_ld32(t_s + 32 * c, x);
-                tmem_wait_ld();
+                uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int page = 2 * c + h;
-                    const float2 ks = rows[page], vs = rows[8 + page];
-                    const float a = ks.x * unscale, b = fmaf(ks.y, q_sum, -m_use);
-                    const int n = known >> page & 1 ? seen - page * kPageTokens : 0;
-                    float sum = 0.f;
+                    float2 ks = rows[page], vs = rows[8 + page];
+                    float a = ks.x * unscale, b = fmaf(ks.y, q_sum, -m_use);
+                    if (hidden(page)) a = 1.f, b = 0.f, vs = make_float2(0.f, 0.f);
+                    const uint64_t aa = pack2(a, a), bb = pack2(b, b), ss = pack2(vs.x, vs.x);
+                    uint64_t sum = 0;
 #pragma unroll
                     for (int k = 0; k < 16; k += 2) {
-                        float p0 = ex2(fmaf(a, __uint_as_float(x[16 * h + k]), b));
-                        float p1 = ex2(fmaf(a, __uint_as_float(x[16 * h + k + 1]), b));
-                        if (masked) {
-                            p0 = k < n ? p0 : 0.f;
-                            p1 = k + 1 < n ? p1 : 0.f;
-                        }
-                        sum += p0 + p1;
-                        float w0 = p0 * vs.x, w1 = p1 * vs.x;
-                        if (masked) {  // a scale that is no number stays out too
-                            w0 = k < n ? w0 : 0.f;
-                            w1 = k + 1 < n ? w1 : 0.f;
-                        }
-                        hi[8 * h + k / 2] = pack_half(w0, w1);
+                        const float2 t = unpack2(fma2(aa, pack2(__uint_as_float(x[c][16 * h + k]), __uint_as_float(x[c][16 * h + k + 1])), bb));
+                        const uint64_t e2 = pack2(ex2(t.x), ex2(t.y));
+                        sum = add2(sum, e2);
+                        const float2 f = unpack2(mul2(e2, ss));
+                        hi[8 * h + k / 2] = pack_half(f.x, f.y);
                         if constexpr (kSplit) {
-                            const float2 f = h2_to_f2(hi[8 * h + k / 2]);
-                            lo[8 * h + k / 2] = pack_half(w0 - f.x, w1 - f.y);
+                            const float2 g = h2_to_f2(hi[8 * h + k / 2]);
+                            lo[8 * h + k / 2] = pack_half(f.x - g.x, f.y - g.y);
                         }
                     }
-                    l += sum;
-                    if (!masked || n > 0) z = fmaf(sum, vs.y, z);
+                    const float2 both = unpack2(sum);
+                    l += both.x + both.y;
+                    z = fmaf(both.x + both.y, vs.y, z);
                 }
                 tmem_st16(t_s + 32 * c, hi);
                 if constexpr (kSplit) tmem_st16(t_s + 32 * c + 16, lo);
