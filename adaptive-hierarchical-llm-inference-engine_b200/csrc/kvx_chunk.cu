@@ -13,7 +13,7 @@
 // major.  A CTA owns a tile of rows and a range of 128-key tiles (8 pages):
 //  * loader warp: a bulk copy (TMA) per page and K|V, 2 KB of codes each, into
 //    staging slots;
-//  * 4 convert warps (2 for K, 2 for V): codes -> fp16 into the 128-byte-swizzled K and V tiles
+//  * 8 convert warps (4 for K, 4 for V): codes -> fp16 into the 128-byte-swizzled K and V tiles
 //    (K: the K-major B operand of Q K^T; V: the MN-major B operand of P V,
 //    the same bytes), two stages each;
 //  * MMA warp: one thread issues S = Q K^T (M 128, N 128, 8 steps of K 16)
@@ -43,17 +43,24 @@ namespace {
 
 constexpr int kTileKeys = 128, kTilePages = kTileKeys / kPageTokens;
 constexpr int kBlockBytes = kPageTokens * kHeadDim;  // codes of one (page, K|V, head)
-constexpr int kConvertWarp = 8, kMmaWarp = 12, kLoadWarp = 13, kChunkThreads = 16 * 32;
-// registers a thread, by warpgroup (setmaxnreg): 2 x 128 x 184 + 128 x 80 +
-// 128 x 64 = the 512 x 128 of the launch.  A softmax thread holds its 128
-// scores from the maximum to the exponentials.
-constexpr int kSoftmaxRegs = 184, kConvertRegs = 80, kIssueRegs = 64;
-static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs == 4 * 128, "the launch's registers, dealt out");
+constexpr int kConvertWarp = 8, kMmaWarp = 16, kLoadWarp = 17, kStatWarp = 18, kChunkThreads = 20 * 32;
+// registers a thread, by warpgroup (setmaxnreg): 2 x 128 x 128 + 2 x 128 x 72
+// + 128 x 80 = the 640 x 96 of the launch
+constexpr int kSoftmaxRegs = 128, kConvertRegs = 72, kIssueRegs = 80;
+static_assert(2 * kSoftmaxRegs + 2 * kConvertRegs + kIssueRegs == 5 * 96, "the launch's registers, dealt out");
 constexpr int kTileBytes = 128 * kHeadDim * 2;  // an fp16 tile of Q, K or V: two halves of 64 dims
 constexpr int kHalfBytes = kTileBytes / 2, kSlotBytes = kTileKeys * kHeadDim;
+// What the softmax needs of a key tile's statistics.
+constexpr int kStatSlots = 4;
+struct TileStats {
+    float4 page[kTilePages];  // K: scale, mid (times the softmax scale, log2); V: scale 2^(7 - exponent), mid
+    int exponent;             // 2^exponent is above every V scale up to this tile
+    uint32_t known;           // bit i: page i is there
+    uint32_t pad[2];
+};
 // shared memory: Q0, Q1 (staging slots 2, 3 when unused), K x 2, V x 2, staging x 2, the rest
 constexpr int kAtK = 2 * kTileBytes, kAtV = kAtK + 2 * kTileBytes, kAtStage = kAtV + 2 * kTileBytes,
-              kAtMisc = kAtStage + 2 * kSlotBytes, kChunkSmem = 1024 + kAtMisc + 512 + 8 * 16 * 8;
+              kAtMisc = kAtStage + 2 * kSlotBytes, kChunkSmem = 1024 + kAtMisc + 512 + kStatSlots * (int)sizeof(TileStats);
 static_assert(kChunkSmem <= 227 * 1024, "chunk attention exceeds the shared memory of a CTA");
 constexpr float kLazy = 8.f;  // log2 of the growth of a row's maximum that is let pass
 
@@ -71,7 +78,7 @@ struct ChunkParams {
 };
 
 struct ChunkBars {
-    uint64_t ld_full[4], ld_empty[4], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], q_full, done;
+    uint64_t ld_full[4], ld_empty[4], stat_full[kStatSlots], stat_empty[kStatSlots], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], q_full, done;
     uint32_t tmem, gave_up;
     uint32_t known[4];  // staging slot: bit i, page i was loaded
     int seq, tile;
@@ -112,38 +119,56 @@ __device__ __forceinline__ RowTile row_tile(const ChunkParams &p, int s, int til
 
 // ---- tcgen05
 
-__device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)((lbo >> 4) & 0x3fff) << 16) |
-           ((uint64_t)((sbo >> 4) & 0x3fff) << 32) | (1ull << 46) /* sm100 descriptor */ |
-           (2ull << 61) /* 128-byte swizzle */;
-}
+// Shared-memory descriptor of a 128-byte-swizzled operand whose 8-row groups
+// lie 1024 bytes apart: the low word holds the address and the leading
+// offset (both count 16 bytes), the high word is the same for all.
+__device__ __forceinline__ uint32_t umma_desc_low(uint32_t addr, uint32_t leading) { return (addr >> 4) | (leading >> 4) << 16; }
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 /* sm100 descriptor */ | 2u << 29 /* 128-byte swizzle */;
 // D fp32, A and B fp16, M = N = 128, A K-major
 constexpr uint32_t kIdescQK = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kIdescPV = kIdescQK | (1u << 16);  // B MN-major
 
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Issued by the lane whose `issues` is set, under a predicate and not a
+// branch: the operands stay in uniform registers.
+__device__ __forceinline__ void umma_f16_ss(uint32_t issues, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "mov.b64 x, {%1, %6};\n\tmov.b64 y, {%2, %6};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(issues), "n"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f16_ts(uint32_t issues, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "mov.b64 y, {%2, %6};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(issues), "n"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ bool elect_one() {
+__device__ __forceinline__ uint32_t elect_one() {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-    return r != 0;
+    return r;
 }
-__device__ __forceinline__ void umma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+__device__ __forceinline__ void umma_commit(uint32_t issues, uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)), "r"(issues)
+        : "memory");
 }
+// The same value in every lane, known to be so.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// ... and nothing that uses these registers moves above it
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&a)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]) : : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&a)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]), "+r"(a[16]), "+r"(a[17]), "+r"(a[18]), "+r"(a[19]), "+r"(a[20]), "+r"(a[21]), "+r"(a[22]), "+r"(a[23]), "+r"(a[24]), "+r"(a[25]), "+r"(a[26]), "+r"(a[27]), "+r"(a[28]), "+r"(a[29]), "+r"(a[30]), "+r"(a[31]) : : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&a)[32], uint32_t (&b)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]), "+r"(a[16]), "+r"(a[17]), "+r"(a[18]), "+r"(a[19]), "+r"(a[20]), "+r"(a[21]), "+r"(a[22]), "+r"(a[23]), "+r"(a[24]), "+r"(a[25]), "+r"(a[26]), "+r"(a[27]), "+r"(a[28]), "+r"(a[29]), "+r"(a[30]), "+r"(a[31]), "+r"(b[0]), "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(b[4]), "+r"(b[5]), "+r"(b[6]), "+r"(b[7]), "+r"(b[8]), "+r"(b[9]), "+r"(b[10]), "+r"(b[11]), "+r"(b[12]), "+r"(b[13]), "+r"(b[14]), "+r"(b[15]), "+r"(b[16]), "+r"(b[17]), "+r"(b[18]), "+r"(b[19]), "+r"(b[20]), "+r"(b[21]), "+r"(b[22]), "+r"(b[23]), "+r"(b[24]), "+r"(b[25]), "+r"(b[26]), "+r"(b[27]), "+r"(b[28]), "+r"(b[29]), "+r"(b[30]), "+r"(b[31]) : : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
@@ -155,6 +180,9 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(at));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(at) : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at) : "memory");
@@ -208,6 +236,7 @@ __device__ __forceinline__ int exponent_above(float x) {
 // once: the CTA finishes (with wrong results and bit 0 of the error flag)
 // instead of waiting again and again.
 __device__ __forceinline__ void wait_or_give_up(uint64_t *bar, uint32_t parity, ChunkBars *b, int32_t *error_flag) {
+#pragma unroll 1
     for (uint32_t i = 0; i < kWaitPolls; ++i) {
         if (mbar_try_wait(bar, parity)) return;
         if ((i & 255) == 255 && *reinterpret_cast<volatile uint32_t *>(&b->gave_up)) return;
@@ -271,7 +300,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(chunk_smem) + 1023) & ~uintptr_t(1023));
     const uint32_t base = smem_addr(sm);
     ChunkBars *bars = reinterpret_cast<ChunkBars *>(sm + kAtMisc);
-    float2 *stat_rows = reinterpret_cast<float2 *>(sm + kAtMisc + 512);
+    TileStats *tile_stats = reinterpret_cast<TileStats *>(sm + kAtMisc + 512);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kvh = blockIdx.y, split = blockIdx.z;
 
@@ -303,23 +332,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             bars->gave_up = 0;
         }
     }
-    if (threadIdx.x == 32) {
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(&bars->ld_full[i], 1);
-            mbar_init(&bars->ld_empty[i], 2);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&bars->k_full[i], 2);
-            mbar_init(&bars->k_empty[i], 1);
-            mbar_init(&bars->v_full[i], 2);
-            mbar_init(&bars->v_empty[i], 1);
-            mbar_init(&bars->s_full[i], 1);
-            mbar_init(&bars->p_full[i], 128);
-        }
-        mbar_init(&bars->q_full, 256);
-        mbar_init(&bars->done, 1);
-        fence_barrier_init();
-    }
     __syncthreads();
     const int seq = bars->seq, tile = bars->tile;
     if (seq < 0) return;  // the grid is an upper bound
@@ -345,6 +357,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     const int items = turns ? tiles : 2 * tiles;  // item w: warpgroup w % 2, key tile w or w / 2
     const int slot_bits = turns && !kSplit ? 2 : 1, slot_mask = (1 << slot_bits) - 1;  // 4 or 2 staging slots
     const int32_t *table = p.block_table + (size_t)seq * p.max_pages;
+    if (threadIdx.x == 32) {
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&bars->ld_full[i], 1);
+            mbar_init(&bars->ld_empty[i], 4);
+        }
+        for (int i = 0; i < kStatSlots; ++i) {
+            mbar_init(&bars->stat_full[i], 1);
+            mbar_init(&bars->stat_empty[i], turns ? 4 : 8);  // the softmax warps that look at a tile
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars->k_full[i], 4);
+            mbar_init(&bars->k_empty[i], 1);
+            mbar_init(&bars->v_full[i], 4);
+            mbar_init(&bars->v_empty[i], 1);
+            mbar_init(&bars->s_full[i], 1);
+            mbar_init(&bars->p_full[i], 128);
+        }
+        mbar_init(&bars->q_full, 256);
+        mbar_init(&bars->done, 1);
+        fence_barrier_init();
+    }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&bars->tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -352,18 +385,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = bars->tmem;  // S0, S1, O0, O1: 128 columns each
+    // S0, S1, O0, O1: 128 columns each.  All 512 columns were asked for, so
+    // they begin at 0 (were they to begin elsewhere, nothing is done).
+    constexpr uint32_t tmem = 0;
+    if (bars->tmem != 0) {
+        if (threadIdx.x == 0 && p.error_flag) atomicOr(p.error_flag, 1);
+        if (warp == kMmaWarp)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(bars->tmem) : "memory");
+        return;
+    }
     auto slot_at = [&](int s) { return s < 2 ? kAtStage + s * kSlotBytes : kTileBytes + (s - 2) * kSlotBytes; };
 
     if (warp >= kMmaWarp) {
         fewer_registers<kIssueRegs>();
         if (warp == kLoadWarp) {
             // ---- loader: lane i < 8 copies page i of the tile's K, then V codes
+            auto wanted = [&](int i) { return lane < 8 && i < tiles && ((t0 + i) * kTilePages + lane) * kPageTokens < rt.keys; };
+            int next = wanted(0) ? table[t0 * kTilePages + lane] : -1;
             for (int i = 0; i < tiles; ++i) {
-                const int lp = (t0 + i) * kTilePages + (lane & 7);
-                const bool want = lane < 8 && lp * kPageTokens < rt.keys;
-                const int phys = want ? table[lp] : -1;
-                const bool have = phys >= 0 && phys < p.num_pages;
+                const bool want = wanted(i);
+                const int phys = next;
+                if (wanted(i + 1)) next = table[(t0 + i + 1) * kTilePages + lane];
+                const bool have = want && phys >= 0 && phys < p.num_pages;
                 if (want && !have && p.error_flag) atomicOr(p.error_flag, 2);
                 const uint32_t known = __ballot_sync(0xffffffffu, have);
                 for (int kv = 0; kv < 2; ++kv) {
@@ -382,89 +425,122 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             // no copy is in flight when the CTA ends, however it ends
             for (int u = max(0, 2 * tiles - slot_mask - 1); u < 2 * tiles; ++u)
                 (void)mbar_wait_bounded(&bars->ld_full[u & slot_mask], u >> slot_bits & 1, nullptr);
-        } else if (warp == kMmaWarp) {
-            // the whole warp walks the items (uniform addresses and
-            // descriptors stay in uniform registers), one lane issues
-            const bool issues = elect_one();
-            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-            auto scores = [&](int w) {
-                const int i = turns ? w : w >> 1, j = w & 1, st = i & 1;
-                wait_or_give_up(&bars->k_full[st], (i >> 1) & 1, bars, p.error_flag);
-                tc_fence_after();
-                if (issues) {
-                    const uint64_t q = umma_desc(base + (turns ? 0 : j * kTileBytes), 16, 1024),
-                                   k = umma_desc(base + kAtK + st * kTileBytes, 16, 1024);
-#pragma unroll
-                    for (int part = 0; part < (kSplit ? 2 : 1); ++part)
-#pragma unroll
-                        for (int ks = 0; ks < 8; ++ks) {  // addresses in a descriptor count 16 bytes
-                            const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
-                            umma_f16_ss(tm + j * 128, q + (part * kTileBytes >> 4) + off, k + off, kIdescQK, part | ks);
-                        }
-                    umma_commit(&bars->s_full[j]);
-                    if (turns || j) umma_commit(&bars->k_empty[st]);
-                }
-                __syncwarp();
+        } else if (warp == kStatWarp) {
+            // ---- statistics: lane i < 8 takes page i's of K, lane 8 + i of V;
+            // page ids two tiles ahead, statistics one
+            auto page_of = [&](int i) {
+                const int lp = (t0 + i) * kTilePages + (lane & 7);
+                return lane < 16 && i < tiles && lp * kPageTokens < rt.keys ? table[lp] : -1;
             };
+            auto stat_of = [&](int phys) {
+                return phys >= 0 && phys < p.num_pages
+                           ? __ldg(reinterpret_cast<const float4 *>(p.stats) + ((size_t)phys * 2 + (lane >> 3)) * p.hkv + kvh)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+            };
+            int id = page_of(0), id_next = page_of(1), E = -100;
+            float4 stat = stat_of(id);
+            for (int i = 0; i < tiles; ++i) {
+                const uint32_t known = __ballot_sync(0xffffffffu, id >= 0 && id < p.num_pages) & 0xffu;
+                const float4 cur = stat;
+                id = id_next;
+                stat = stat_of(id);
+                id_next = page_of(i + 2);
+                // scales that are no numbers do not count
+                const int e = lane >= 8 && lane < 16 && fabsf(cur.z) < CUDART_INF_F ? exponent_above(cur.z) : -100;
+                E = max(E, __reduce_max_sync(0xffffffffu, e));
+                const float mid = fmaf(128.f, cur.z, cur.w), f = lane < 8 ? p.scale_log2 : pow2i(7 - E);
+                TileStats &t = tile_stats[i & (kStatSlots - 1)];
+                wait_or_give_up(&bars->stat_empty[i & (kStatSlots - 1)], (i / kStatSlots & 1) ^ 1, bars, p.error_flag);
+                if (lane < 16)
+                    reinterpret_cast<float2 *>(&t.page[lane & 7])[lane >> 3] = make_float2(cur.z * f, lane < 8 ? mid * f : mid);
+                if (lane == 0) {
+                    t.exponent = E;
+                    t.known = known;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->stat_full[i & (kStatSlots - 1)]);
+            }
+        } else if (warp == kMmaWarp) {
+            // The whole warp walks the items and one lane issues, from uniform
+            // registers: an MMA is 64 cycles, so its issue has to be a few
+            // instructions.  The 512 tensor-memory columns begin at 0.
+            const uint32_t issues = elect_one(), at = uniform(base);
+            const bool u_turns = uniform(turns);
+            const int u_items = (int)uniform(items);
             wait_or_give_up(&bars->q_full, 0, bars, p.error_flag);
-            scores(0);
-            if (items > 1) scores(1);
-            for (int w = 0; w < items; ++w) {
-                const int i = turns ? w : w >> 1, j = w & 1, st = i & 1;
-                wait_or_give_up(&bars->v_full[st], (i >> 1) & 1, bars, p.error_flag);
-                wait_or_give_up(&bars->p_full[j], (w >> 1) & 1, bars, p.error_flag);
-                tc_fence_after();
-                if (issues) {
-                    const uint64_t v = umma_desc(base + kAtV + st * kTileBytes, kHalfBytes, 1024);
+#pragma unroll 1
+            for (int w = -2; w < u_items; ++w) {  // P V of item w, then the scores of item w + 2
+                const int j = w & 1;
+                if (w >= 0) {
+                    const int i = u_turns ? w : w >> 1, st = i & 1;
+                    wait_or_give_up(&bars->v_full[st], (i >> 1) & 1, bars, p.error_flag);
+                    wait_or_give_up(&bars->p_full[j], (w >> 1) & 1, bars, p.error_flag);
+                    tc_fence_after();
+                    const uint32_t v = umma_desc_low(at + kAtV + st * kTileBytes, kHalfBytes);
 #pragma unroll
                     for (int part = 0; part < (kSplit ? 2 : 1); ++part)
 #pragma unroll
-                        for (int ks = 0; ks < 8; ++ks)  // 16 keys: P over S's columns 32 (ks/2) .., half of them
-                            umma_f16_ts(tm + 256 + j * 128, tm + j * 128 + (ks >> 1) * 32 + (ks & 1) * 8 + part * 16,
-                                        v + (ks * 2048 >> 4), kIdescPV, (w > 1) | part | ks);
-                    if (turns || j) umma_commit(&bars->v_empty[st]);
+                        for (int ks = 0; ks < 8; ++ks)  // a page: its P over its columns of S
+                            umma_f16_ts(issues, tmem + 256 + j * 128, tmem + j * 128 + ks * 16 + part * 8, v + (ks * 2048 >> 4),
+                                        kIdescPV, (w > 1) | part | ks);
+                    if (u_turns || j) umma_commit(issues, &bars->v_empty[st]);
                 }
-                __syncwarp();
-                if (w + 2 < items) scores(w + 2);
+                if (w + 2 < u_items) {
+                    const int i = u_turns ? w + 2 : (w + 2) >> 1, st = i & 1;
+                    wait_or_give_up(&bars->k_full[st], (i >> 1) & 1, bars, p.error_flag);
+                    tc_fence_after();
+                    const uint32_t q = umma_desc_low(at + (u_turns ? 0 : j * kTileBytes), 16),
+                                   k = umma_desc_low(at + kAtK + st * kTileBytes, 16);
+#pragma unroll
+                    for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks) {
+                            const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                            umma_f16_ss(issues, tmem + j * 128, q + ((part * kTileBytes >> 4) + off), k + off, kIdescQK, part | ks);
+                        }
+                    umma_commit(issues, &bars->s_full[j]);
+                    if (u_turns || j) umma_commit(issues, &bars->k_empty[st]);
+                }
             }
-            if (issues) umma_commit(&bars->done);
+            umma_commit(issues, &bars->done);
             __syncwarp();
         }
     } else if (warp >= kConvertWarp) {
         fewer_registers<kConvertRegs>();
-        // ---- convert: two warps take the K codes, two the V codes.  8 lanes
-        // take row r (even) chunks 0-3 and row r + 1 chunks 4-7: reads of 128
-        // contiguous bytes, writes to 8 different 16-byte banks
-        const int kv = warp & 1, g = (warp & 2) * 2 + (lane >> 3), j = lane & 7;  // groups 0..7 of 8 lanes
+        // ---- convert: a warpgroup for K, one for V.  8 lanes take row r (even)
+        // chunks 0-3 and row r + 1 chunks 4-7: reads of 128 contiguous bytes,
+        // writes to 8 different 16-byte banks.  The slot is free as soon as its
+        // codes are in registers: its next copy runs under the conversion.
+        const int kv = warp >> 2 & 1, g = (warp & 3) * 4 + (lane >> 3), j = lane & 7;  // groups 0..15 of 8 lanes
+        auto row_of = [&](int k) { return 2 * (g + 16 * (k >> 1)) + ((j >> 2) ^ (k & 1)); };
         for (int i = 0; i < tiles; ++i) {
             const int u = 2 * i + kv, s = u & slot_mask, st = i & 1;
             wait_or_give_up(&bars->ld_full[s], u >> slot_bits & 1, bars, p.error_flag);
             const uint32_t known = bars->known[s];
             const uint8_t *src = sm + slot_at(s);
+            uint4 w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const uint4 *>(src + row_of(k) * 128 + j * 16);
+            if (known != 0xffu) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (!(known >> (row_of(k) >> 4) & 1)) w[k] = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();  // these reads before the slot's next copy
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->ld_empty[s]);
+            wait_or_give_up(kv ? &bars->v_empty[st] : &bars->k_empty[st], ((i >> 1) & 1) ^ 1, bars, p.error_flag);
             const uint32_t dst = base + (kv ? kAtV : kAtK) + st * kTileBytes;
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
-                auto row_of = [&](int k) { return 2 * (g + 8 * (k >> 1) + 32 * part) + ((j >> 2) ^ (k & 1)); };
-                uint4 w[8];  // all loads before the first store
-#pragma unroll
-                for (int k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const uint4 *>(src + row_of(k) * 128 + j * 16);
-                if (part == 0) wait_or_give_up(kv ? &bars->v_empty[st] : &bars->k_empty[st], ((i >> 1) & 1) ^ 1, bars, p.error_flag);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int r = row_of(k);
-                    if (!(known >> (r >> 4) & 1)) w[k] = make_uint4(0, 0, 0, 0);
-                    const uint2 a = codes_to_half(w[k].x), b = codes_to_half(w[k].y), d = codes_to_half(w[k].z),
-                                e = codes_to_half(w[k].w);
-                    st_shared16(dst + tile_chunk(r, 2 * j), a.x, a.y, b.x, b.y);
-                    st_shared16(dst + tile_chunk(r, 2 * j + 1), d.x, d.y, e.x, e.y);
-                }
+            for (int k = 0; k < 8; ++k) {
+                const int r = row_of(k);
+                const uint2 a = codes_to_half(w[k].x), b = codes_to_half(w[k].y), d = codes_to_half(w[k].z), e = codes_to_half(w[k].w);
+                st_shared16(dst + tile_chunk(r, 2 * j), a.x, a.y, b.x, b.y);
+                st_shared16(dst + tile_chunk(r, 2 * j + 1), d.x, d.y, e.x, e.y);
             }
-            fence_proxy_async_smem();  // before the tensor core's reads, and the next copy into the slot
+            fence_proxy_async_smem();  // before the tensor core's reads
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&bars->ld_empty[s]);
-                mbar_arrive(kv ? &bars->v_full[st] : &bars->k_full[st]);
-            }
+            if (lane == 0) mbar_arrive(kv ? &bars->v_full[st] : &bars->k_full[st]);
         }
     } else {
         more_registers<kSoftmaxRegs>();
@@ -520,124 +596,130 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             mbar_arrive(&bars->q_full);
         }
         const int limit = valid ? row_keys(p, rt, row0 + my_row) : 0x7fffffff;  // a row that is none needs no mask
-        // the statistics of a tile: lane i < 8 page i's of K, lane 8 + i of V;
-        // page ids two items ahead, statistics one
         const int step = turns ? 2 : 1;
-        auto page_of = [&](int i) {
-            const int lp = (t0 + i) * kTilePages + (lane & 7);
-            return lane < 16 && i < tiles && lp * kPageTokens < rt.keys ? table[lp] : -1;
+        // O by f (rare, so in little code)
+        auto scale_o = [&](float f) {
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                uint32_t o[16];
+                tmem_ld16(t_o + 16 * c, o);
+                tmem_wait_ld(o);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                tmem_st16(t_o + 16 * c, o);
+            }
         };
-        auto stat_of = [&](int phys) {
-            return phys >= 0 && phys < p.num_pages
-                       ? __ldg(reinterpret_cast<const float4 *>(p.stats) + ((size_t)phys * 2 + (lane >> 3)) * p.hkv + kvh)
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
-        };
-        int i = turns ? j : 0;
-        int id = page_of(i), id_next = page_of(i + step);
-        float4 stat = stat_of(id);
-        float2 *rows = stat_rows + warp * 16;
         float m = -CUDART_INF_F, l = 0.f, z = 0.f;  // maximum (log2), sum, sum of p mid
         int E = -100;
+        int i = turns ? j : 0;
         for (int w = j; w < items; w += 2, i += step) {
-            const uint32_t known = __ballot_sync(0xffffffffu, id >= 0 && id < p.num_pages) & 0xffu;
-            const float4 cur = stat;
-            id = id_next;
-            stat = stat_of(id);
-            id_next = page_of(i + 2 * step);
-            // 2^E above the tile's V scales (those that are numbers)
-            int e = lane >= 8 && lane < 16 && fabsf(cur.z) < CUDART_INF_F ? exponent_above(cur.z) : -100;
-            e = max(E, __reduce_max_sync(0xffffffffu, e));
-            const float shrink = E - e < -126 ? 0.f : pow2i(E - e);  // what O loses to a larger E
-            const bool larger = e > E;
-            E = e;
-            if (lane < 16) {
-                const float mid = fmaf(128.f, cur.z, cur.w);
-                rows[lane] = lane < 8 ? make_float2(cur.z * p.scale_log2, mid * p.scale_log2) : make_float2(cur.z * pow2i(7 - E), mid);
-            }
-            __syncwarp();
-            const int key0 = (t0 + i) * kTileKeys;
-            const bool masked = __any_sync(0xffffffffu, limit - key0 < kTileKeys) || known != 0xffu;
-            const int seen = limit - key0;
-
+            const TileStats &ts = tile_stats[i & (kStatSlots - 1)];
+            wait_or_give_up(&bars->stat_full[i & (kStatSlots - 1)], i / kStatSlots & 1, bars, p.error_flag);
+            const uint32_t known = ts.known;
+            const int e = ts.exponent, seen = limit - (t0 + i) * kTileKeys;  // the tile's keys that the row sees
+            const bool masked = __any_sync(0xffffffffu, seen < kTileKeys) || known != 0xffu;
+            // a page this row sees nothing of: scores of -inf, whatever its statistics
+            auto hidden = [&](int page) { return seen <= page * kPageTokens || !(known >> page & 1); };
             wait_or_give_up(&bars->s_full[j], (w >> 1) & 1, bars, p.error_flag);
             __syncwarp();
             tc_fence_after();
-            uint32_t x[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, x[c]);
-            tmem_wait_ld();
-            if (masked) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if (32 * c + k >= seen || !(known >> (2 * c + (k >> 4)) & 1)) x[c][k] = 0xff800000u;  // -inf
-            }
-            // a page this row sees nothing of: every score -inf, whatever its statistics
-            auto hidden = [&](int page) { return masked && (seen <= page * kPageTokens || !(known >> page & 1)); };
-            float top = -CUDART_INF_F;
-#pragma unroll
-            for (int page = 0; page < kTilePages; ++page) {
-                const float2 ks = rows[page];
-                float big = -CUDART_INF_F;
-#pragma unroll
-                for (int k = 0; k < 16; ++k) big = fmaxf(big, __uint_as_float(x[page >> 1][16 * (page & 1) + k]));
-                if (!hidden(page)) top = fmaxf(top, fmaf(ks.x * unscale, big, ks.y * q_sum));
-            }
-            if (w < 2) {
-                m = top;
-            } else if (__any_sync(0xffffffffu, top > m + kLazy) || larger) {
-                const float mn = fmaxf(m, top);
-                const float f = mn == -CUDART_INF_F ? 1.f : ex2(m - mn);
-                m = mn;
-                l *= f;
-                z *= f;
-                const float fo = f * shrink;
+            if (masked) {  // few tiles: their scores are masked where they are
 #pragma unroll 1
-                for (int c = 0; c < 8; ++c) {
-                    uint32_t o[16];
-                    tmem_ld16(t_o + 16 * c, o);
-                    tmem_wait_ld();
+                for (int page = 0; page < kTilePages; ++page) {
+                    uint32_t v[16];
+                    tmem_ld16(t_s + 16 * page, v);
+                    tmem_wait_ld(v);
+                    const int n = known >> page & 1 ? seen - page * kPageTokens : 0;
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fo);
-                    tmem_st16(t_o + 16 * c, o);
+                    for (int k = 0; k < 16; ++k)
+                        if (k >= n) v[k] = 0xff800000u;  // -inf
+                    tmem_st16(t_s + 16 * page, v);
+                }
+                tmem_wait_st();
+            }
+            // Two loops of two chunks of 32 keys each: the code of all warps
+            // together has to stay in the instruction cache.
+            float top = -CUDART_INF_F;
+#pragma unroll 1
+            for (int c = 0; c < 4; c += 2) {
+                uint32_t x[2][32];
+                tmem_ld32(t_s + 32 * c, x[0]);
+                tmem_ld32(t_s + 32 * c + 32, x[1]);
+                tmem_wait_ld(x[0], x[1]);
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const int page = 2 * c + h;
+                    uint32_t(&v)[32] = x[h >> 1];
+                    float2 ks = *reinterpret_cast<const float2 *>(&ts.page[page]);
+                    ks.x *= unscale, ks.y *= q_sum;
+                    if (masked && hidden(page)) ks = make_float2(1.f, 0.f);
+                    float a = __uint_as_float(v[16 * (h & 1)]), b = __uint_as_float(v[16 * (h & 1) + 1]);
+#pragma unroll
+                    for (int k = 2; k < 14; k += 4) {  // three-input maxima
+                        a = fmaxf(fmaxf(a, __uint_as_float(v[16 * (h & 1) + k])), __uint_as_float(v[16 * (h & 1) + k + 1]));
+                        b = fmaxf(fmaxf(b, __uint_as_float(v[16 * (h & 1) + k + 2])), __uint_as_float(v[16 * (h & 1) + k + 3]));
+                    }
+                    a = fmaxf(fmaxf(a, __uint_as_float(v[16 * (h & 1) + 14])), __uint_as_float(v[16 * (h & 1) + 15]));
+                    top = fmaxf(top, fmaf(ks.x, fmaxf(a, b), ks.y));
                 }
             }
+            // the maximum in use may lag by kLazy; O follows where it catches
+            // up, and where a larger V scale came
+            const bool lags = __any_sync(0xffffffffu, top > m + kLazy);
+            if (lags || e > E) {
+                float f = 1.f;
+                if (lags) {
+                    const float mn = fmaxf(m, top);
+                    if (mn != -CUDART_INF_F) f = ex2(m - mn);
+                    m = mn;
+                    l *= f;
+                    z *= f;
+                }
+                if (w >= 2) scale_o(E - e < -126 ? 0.f : f * pow2i(E - e));
+                E = e;
+            }
             const float m_use = m == -CUDART_INF_F ? 0.f : m;
+#pragma unroll 1
+            for (int c = 0; c < 4; c += 2) {
+                uint32_t x[2][32];
+                tmem_ld32(t_s + 32 * c, x[0]);
+                tmem_ld32(t_s + 32 * c + 32, x[1]);
+                tmem_wait_ld(x[0], x[1]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < 4; ++h) {
                     const int page = 2 * c + h;
-                    float2 ks = rows[page], vs = rows[8 + page];
-                    float a = ks.x * unscale, b = fmaf(ks.y, q_sum, -m_use);
-                    if (hidden(page)) a = 1.f, b = 0.f, vs = make_float2(0.f, 0.f);
-                    const uint64_t aa = pack2(a, a), bb = pack2(b, b), ss = pack2(vs.x, vs.x);
+                    uint32_t(&v)[32] = x[h >> 1];
+                    float4 st = ts.page[page];
+                    st.x *= unscale;
+                    st.y = fmaf(st.y, q_sum, -m_use);
+                    if (masked && hidden(page)) st = make_float4(1.f, 0.f, 0.f, 0.f);
+                    const uint64_t aa = pack2(st.x, st.x), bb = pack2(st.y, st.y), ss = pack2(st.z, st.z);
                     uint64_t sum = 0;
+                    uint32_t hi[8], lo[8];
 #pragma unroll
                     for (int k = 0; k < 16; k += 2) {
-                        const float2 t = unpack2(fma2(aa, pack2(__uint_as_float(x[c][16 * h + k]), __uint_as_float(x[c][16 * h + k + 1])), bb));
+                        const float2 t = unpack2(fma2(aa, pack2(__uint_as_float(v[16 * (h & 1) + k]), __uint_as_float(v[16 * (h & 1) + k + 1])), bb));
                         const uint64_t e2 = pack2(ex2(t.x), ex2(t.y));
                         sum = add2(sum, e2);
                         const float2 f = unpack2(mul2(e2, ss));
-                        hi[8 * h + k / 2] = pack_half(f.x, f.y);
+                        hi[k / 2] = pack_half(f.x, f.y);
                         if constexpr (kSplit) {
-                            const float2 g = h2_to_f2(hi[8 * h + k / 2]);
-                            lo[8 * h + k / 2] = pack_half(f.x - g.x, f.y - g.y);
+                            const float2 g = h2_to_f2(hi[k / 2]);
+                            lo[k / 2] = pack_half(f.x - g.x, f.y - g.y);
                         }
                     }
                     const float2 both = unpack2(sum);
                     l += both.x + both.y;
-                    z = fmaf(both.x + both.y, vs.y, z);
+                    z = fmaf(both.x + both.y, st.w, z);
+                    tmem_st8(t_s + 16 * page, hi);  // over the page's own scores
+                    if constexpr (kSplit) tmem_st8(t_s + 16 * page + 8, lo);
                 }
-                tmem_st16(t_s + 32 * c, hi);
-                if constexpr (kSplit) tmem_st16(t_s + 32 * c + 16, lo);
             }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&bars->p_full[j]);
-            __syncwarp();  // rows is free for the next tile
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->stat_empty[i & (kStatSlots - 1)]);
         }
 
         // ---- O
@@ -656,7 +738,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                     if (!worked) break;
                     uint32_t x[32];
                     tmem_ld32(t_o + 32 * c, x);
-                    tmem_wait_ld();
+                    tmem_wait_ld(x);
 #pragma unroll
                     for (int k = 0; k < 32; ++k)
                         shared_o[(32 * c + k) * 128 + r] = fmaf(__uint_as_float(x[k]), back, z);
@@ -686,7 +768,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             for (int c = 0; c < 4; ++c) {
                 uint32_t x[32];
                 tmem_ld32(t_o + 32 * c, x);  // by whole warps: rows that are none are loaded, not stored
-                tmem_wait_ld();
+                tmem_wait_ld(x);
 #pragma unroll
                 for (int k = 0; k < 32; k += 4) {
                     float f[4];
