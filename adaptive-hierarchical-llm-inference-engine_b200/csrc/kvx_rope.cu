@@ -12,6 +12,7 @@
 #include <cmath>
 
 #include "kvx_common.cuh"
+#include "kvx_decode_params.cuh"  // grid_dependents_launch, grid_dependency_wait
 #include "kvx_rope.cuh"
 
 namespace kvx {
@@ -104,7 +105,6 @@ struct RopeAppendParams {
     void *q_out;
     int64_t q_stride, k_stride, v_stride;
     int batch, total, hq, hkv, max_pages, num_pages, rotary, items;
-    int half_layout;
     float amplitude;
     int kv_blocks, tokens_per_block;  // int8: CTAs that write pages, and the tokens each looks at
 };
@@ -177,52 +177,75 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_
 constexpr float kTieLimit = 0.5f - 4.0e-5f;  // as in kvx_quant.cu: nearer to a half-integer, divide exactly
 constexpr float kTwo23 = 8388608.0f;
 
-// code + 128 of x: clamp(round((x - mn) / scale), 0, 255), NaN -> 0.  The
-// product with the reciprocal decides except next to a half-integer (or
-// where scale or its reciprocal is not finite), where the division does.
-__device__ __forceinline__ uint32_t level(float x, float mn, float scale, float rcp) {
-    const float t = __fmul_rn(__fsub_rn(x, mn), rcp);
-    const float s = __fadd_rn(t, kTwo23);
-    if (fabsf(__fsub_rn(t, __fsub_rn(s, kTwo23))) <= kTieLimit && t >= -0.5f && t <= 255.5f)
-        return __float_as_uint(s) & 0xffu;
+// code + 128 of x: clamp(round((x - mn) / scale), 0, 255), NaN -> 0.
+__device__ __noinline__ uint32_t level_exact(float x, float mn, float scale) {
     const float r = roundf(__fdiv_rn(__fsub_rn(x, mn), scale));
     return r >= 255.f && r < 2147483648.f ? 255u : (r > 0.f && r < 255.f ? (uint32_t)r : 0u);
 }
 
+// Four codes.  The product with the reciprocal decides; next to a
+// half-integer, and where anything is not finite (a NaN wins the maximum),
+// the division does.
 __device__ __forceinline__ uint32_t code4(const float *x, float mn, float scale, float rcp) {
-    uint32_t w = 0;
+    uint32_t u[4];
+    float worst = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w |= level(x[k], mn, scale, rcp) << (8 * k);
-    return w ^ 0x80808080u;
+    for (int k = 0; k < 4; ++k) {
+        const float t = __fmul_rn(__fsub_rn(x[k], mn), rcp), s = __fadd_rn(t, kTwo23);
+        const float off = fabsf(__fsub_rn(t, __fsub_rn(s, kTwo23)));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(worst) : "f"(off));
+        u[k] = __float_as_uint(s);
+    }
+    if (!(worst <= kTieLimit)) {
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t exact = level_exact(k < 2 ? (k ? x[1] : x[0]) : (k == 2 ? x[2] : x[3]), mn, scale);
+            if (k == 0) u[0] = exact;
+            if (k == 1) u[1] = exact;
+            if (k == 2) u[2] = exact;
+            if (k == 3) u[3] = exact;
+        }
+    }
+    return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410) ^ 0x80808080u;
 }
 
-template <typename T> __device__ __forceinline__ void load4(const T *p, float *f);
-template <> __device__ __forceinline__ void load4<float>(const float *p, float *f) {
-    const float4 v = *reinterpret_cast<const float4 *>(p);
-    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
-}
-template <> __device__ __forceinline__ void load4<__half>(const __half *p, float *f) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    const float2 a = h2_to_f2(v.x), b = h2_to_f2(v.y);
-    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
-}
+// Four elements as they lie in memory.
+template <typename T> struct Raw4;
+template <> struct Raw4<float> {
+    float4 v;
+    __device__ __forceinline__ void load(const float *p) { v = *reinterpret_cast<const float4 *>(p); }
+    __device__ __forceinline__ void unpack(float *f) const { f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w; }
+};
+template <> struct Raw4<__half> {
+    uint2 v;
+    __device__ __forceinline__ void load(const __half *p) { v = *reinterpret_cast<const uint2 *>(p); }
+    __device__ __forceinline__ void unpack(float *f) const {
+        const float2 a = h2_to_f2(v.x), b = h2_to_f2(v.y);
+        f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+    }
+};
 
 // One warp: the new rows (n from slot `slot0`) of one (page, K|V, head)
-// block.  Lane: elements 4 lane .. 4 lane + 3 of every row, held in registers
-// between the range and the codes.  cs: (cos, sin) of row i's pairs at
-// cs + i * rotary/2, null for V and without a table.
-template <typename T>
+// block.  Lane: elements 4 lane .. 4 lane + 3 of every row, in registers from
+// the range to the codes (read, unpacked and turned twice instead, the kernel
+// issued 2.5 times the instructions, and it is bound by them).  cs: (cos,
+// sin) of row i's pairs at cs + i * rotary/2, null for V and without a table.
+// kVec: partners in the half layout lie a multiple of 4 away.
+template <typename T, bool kHalf, bool kVec>
 __device__ __forceinline__ void append_block_i8(const T *src, int64_t stride, uint8_t *codes, float *stats, int slot0,
-                                                int n, const float2 *cs, int rotary, bool half_layout) {
+                                                int n, const float2 *cs, int rotary) {
     const int lane = threadIdx.x & 31, d = 4 * lane, half = rotary / 2;
     const float4 old = *reinterpret_cast<const float4 *>(stats);
     float x[kPageTokens][4];
-    float mn = INFINITY, mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kPageTokens; ++i)
-        if (i < n) load4<T>(src + i * stride + d, x[i]);
+        if (i < n) {
+            Raw4<T> raw;
+            raw.load(src + i * stride + d);
+            raw.unpack(x[i]);
+        }
     if (cs && d < rotary) {
-        if (!half_layout) {
+        if constexpr (!kHalf) {
 #pragma unroll
             for (int i = 0; i < kPageTokens; ++i)
                 if (i < n) {
@@ -230,29 +253,40 @@ __device__ __forceinline__ void append_block_i8(const T *src, int64_t stride, ui
                     rope_pair(x[i][0], x[i][1], c[0]);
                     if (d + 2 < rotary) rope_pair(x[i][2], x[i][3], c[1]);
                 }
+        } else if constexpr (kVec) {  // rope_pair's half of the pair: a where d < half, else b
+            const int far = d < half ? half : -half, at = d < half ? d : d - half;
+            const float sign = d < half ? -1.f : 1.f;
+#pragma unroll
+            for (int i = 0; i < kPageTokens; ++i)
+                if (i < n) {
+                    Raw4<T> raw;
+                    float y[4];
+                    raw.load(src + i * stride + d + far);
+                    raw.unpack(y);
+                    const float4 c0 = *reinterpret_cast<const float4 *>(cs + i * half + at),
+                                 c1 = *reinterpret_cast<const float4 *>(cs + i * half + at + 2);
+                    x[i][0] = fmaf(x[i][0], c0.x, __fmul_rn(y[0], sign * c0.y));
+                    x[i][1] = fmaf(x[i][1], c0.z, __fmul_rn(y[1], sign * c0.w));
+                    x[i][2] = fmaf(x[i][2], c1.x, __fmul_rn(y[2], sign * c1.y));
+                    x[i][3] = fmaf(x[i][3], c1.z, __fmul_rn(y[3], sign * c1.w));
+                }
         } else {
 #pragma unroll
             for (int i = 0; i < kPageTokens; ++i)
                 if (i < n) {
                     const T *row = src + i * stride;
-                    float y[4];
-                    if (half % 4 == 0) {
-                        load4<T>(row + (d < half ? d + half : d - half), y);
-                    } else {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            y[k] = d + k < rotary ? io_traits<T>::load(row + (d + k < half ? d + k + half : d + k - half)) : 0.f;
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (d + k < half)
-                            rope_pair(x[i][k], y[k], cs[i * half + d + k]);
-                        else if (d + k < rotary)
-                            rope_pair(y[k], x[i][k], cs[i * half + d + k - half]);
-                    }
+                    for (int k = 0; k < 4; ++k)
+                        if (d + k < rotary) {
+                            const bool first = d + k < half;
+                            const float y = io_traits<T>::load(row + (first ? d + k + half : d + k - half));
+                            const float2 c = cs[i * half + (first ? d + k : d + k - half)];
+                            x[i][k] = fmaf(x[i][k], c.x, __fmul_rn(y, first ? -c.y : c.y));
+                        }
                 }
         }
     }
+    float mn = INFINITY, mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kPageTokens; ++i)
         if (i < n)
@@ -291,22 +325,35 @@ __device__ __forceinline__ void append_block_i8(const T *src, int64_t stride, ui
     if (lane == 0) *reinterpret_cast<float4 *>(stats) = make_float4(mn, mx, scale, mn);
 }
 
-// CTAs 0 .. kv_blocks-1 write pages, the others rotate the q rows of one
-// token each.  A page is written by whoever holds its first new token (the
+// CTAs 0 .. kv_blocks-1 write pages (even ones K, odd ones V blocks), the
+// others rotate the q rows of one token each.  A page is written by whoever holds its first new token (the
 // sequence's first, or one at a page start) among its tokens_per_block packed
 // rows: one token a CTA while tokens are few (a decode step, where every
 // token leads), 16 when they fill the GPU anyway.
+//
+// A warp with more than kDirectRows rows brings them to shared memory first,
+// a bulk copy (TMA) a row, all in flight together; fewer are read in place,
+// which is one round trip sooner.
+constexpr int kDirectRows = 2;
+template <typename T> constexpr int kStageBytes = kRopeThreads / 32 * kPageTokens * kHeadDim * (int)sizeof(T);
+
 template <typename T, bool kHalf, bool kVec>
-__global__ void __launch_bounds__(kRopeThreads) rope_append_i8_kernel(const __grid_constant__ RopeAppendParams p) {
-    __shared__ float2 cs[kPageTokens * kHeadDim / 2];
+__global__ void __launch_bounds__(kRopeThreads, 2) rope_append_i8_kernel(const __grid_constant__ RopeAppendParams p) {
+    extern __shared__ __align__(128) uint8_t stage[];
+    __shared__ __align__(16) float2 cs[kPageTokens * kHeadDim / 2];
+    __shared__ uint64_t bars[kRopeThreads / 32];
     __shared__ int slot, found;
     __shared__ int2 lead[kPageTokens];  // (sequence, packed row)
+    grid_dependents_launch();
     if (blockIdx.x >= p.kv_blocks) {
         rope_append_rows<T, kHalf, kVec>(p, blockIdx.x - p.kv_blocks, false, cs, &slot);
         return;
     }
-    const int r0 = blockIdx.x * p.tokens_per_block, r1 = min(r0 + p.tokens_per_block, p.total);
+    const bool is_v = blockIdx.x & 1;
+    const int r0 = (blockIdx.x >> 1) * p.tokens_per_block, r1 = min(r0 + p.tokens_per_block, p.total);
     if (threadIdx.x == 0) found = 0;
+    if (threadIdx.x < kRopeThreads / 32) mbar_init(&bars[threadIdx.x], 1);
+    fence_barrier_init();
     __syncthreads();
     for (int s = threadIdx.x; s < p.batch; s += blockDim.x) {
         const int a = p.q_start[s], b = min(p.q_start[s + 1], p.total);
@@ -327,7 +374,9 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_i8_kernel(const __gr
         }
     }
     __syncthreads();
-    const int n_lead = min(found, kPageTokens), warp = threadIdx.x >> 5, half = p.rotary / 2;
+    const int n_lead = min(found, kPageTokens), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = p.rotary / 2;
+    T *rows = reinterpret_cast<T *>(stage) + warp * kPageTokens * kHeadDim;
+    uint32_t phase = 0;
     for (int i = 0; i < n_lead; ++i) {
         const int s = lead[i].x, t = lead[i].y;
         const int a = p.q_start[s], b = min(p.q_start[s + 1], p.total);
@@ -338,22 +387,52 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_i8_kernel(const __gr
             if (p.error_flag && threadIdx.x == 0) atomicOr(p.error_flag, 2);
             continue;
         }
-        if (p.turns) {
+        const int64_t stride = is_v ? p.v_stride : p.k_stride;
+        const T *row0 = static_cast<const T *>(is_v ? p.v : p.k) + t * stride;
+        const bool staged = n > kDirectRows;
+        auto fetch = [&](int h) {  // head h's rows, a lane each
+            if (lane == 0) mbar_arrive_expect_tx(&bars[warp], n * kHeadDim * (int)sizeof(T));
+            __syncwarp();
+            if (lane < n)
+                bulk_g2s(rows + lane * kHeadDim, row0 + lane * stride + h * kHeadDim, kHeadDim * (int)sizeof(T), &bars[warp]);
+        };
+        if (staged && warp < p.hkv) fetch(warp);  // under the work on the cosines
+        if (p.turns && !is_v) {
             __syncthreads();  // the previous page's rows are rotated
             for (int j = threadIdx.x; j < n * half; j += blockDim.x)
                 cs[j] = rope_turn(p.turns[j % half], pos + j / half, p.amplitude);
             __syncthreads();
         }
-        for (int task = warp; task < 2 * p.hkv; task += kRopeThreads / 32) {
-            const bool is_v = task >= p.hkv;
-            const int h = is_v ? task - p.hkv : task;
-            const int64_t stride = is_v ? p.v_stride : p.k_stride;
-            const T *src = static_cast<const T *>(is_v ? p.v : p.k) + t * stride + h * kHeadDim;
-            const size_t block = (size_t)phys * 2 * p.hkv + task;
-            append_block_i8<T>(src, stride, p.pool + block * kPageTokens * kHeadDim, p.stats + block * 4, slot0, n,
-                               !is_v && p.turns ? cs : nullptr, p.rotary, p.half_layout);
+        for (int h = warp; h < p.hkv; h += kRopeThreads / 32) {
+            const size_t block = (size_t)phys * 2 * p.hkv + (is_v ? p.hkv : 0) + h;
+            uint8_t *codes = p.pool + block * kPageTokens * kHeadDim;
+            float *stats = p.stats + block * 4;
+            const float2 *turn = !is_v && p.turns ? cs : nullptr;
+            if (staged) {
+                if (!mbar_wait_bounded(&bars[warp], phase, p.error_flag)) {
+                    (void)mbar_wait_bounded(&bars[warp], phase, nullptr);
+                    return;
+                }
+                phase ^= 1;
+                append_block_i8<T, kHalf, kVec>(rows, kHeadDim, codes, stats, slot0, n, turn, p.rotary);
+                fence_proxy_async_smem();  // these reads before the next copies
+                __syncwarp();
+                if (h + kRopeThreads / 32 < p.hkv) fetch(h + kRopeThreads / 32);
+            } else {
+                append_block_i8<T, kHalf, kVec>(row0 + h * kHeadDim, stride, codes, stats, slot0, n, turn, p.rotary);
+            }
         }
     }
+}
+
+// The q rows of many tokens, beside the CTAs that write their pages: placed
+// while those run (nothing here depends on them), done when they are done.
+template <typename T, bool kHalf, bool kVec>
+__global__ void __launch_bounds__(kRopeThreads) rope_append_q_kernel(const __grid_constant__ RopeAppendParams p) {
+    __shared__ float2 cs[kHeadDim / 2];
+    __shared__ int slot;
+    rope_append_rows<T, kHalf, kVec>(p, blockIdx.x, false, cs, &slot);
+    grid_dependency_wait();
 }
 
 template <typename T>
@@ -369,7 +448,31 @@ int launch_rope_append(const RopeAppendParams &p, bool i8, bool half, bool vec, 
     if (i8) {
         auto kern = half ? (vec ? rope_append_i8_kernel<T, true, true> : rope_append_i8_kernel<T, true, false>)
                          : (vec ? rope_append_i8_kernel<T, false, true> : rope_append_i8_kernel<T, false, false>);
-        kern<<<(unsigned)p.kv_blocks + (p.hq ? (unsigned)p.total : 0u), kRopeThreads, 0, st>>>(p);
+        // rows to stage: only where a page gets more than kDirectRows of them
+        const int smem = p.total > kDirectRows ? kStageBytes<T> : 0;
+        static std::atomic<bool> attr_done[4][kMaxDevices];
+        if (smem && ensure_smem_attr(attr_done[2 * half + vec], kern, smem) != KVX_OK) return KVX_ECUDA;
+        // Many tokens: the CTAs that rotate q get a launch of their own, whose
+        // few registers let 8 of them on an SM (with the other role's 128
+        // registers it is 2, too few to keep the memory busy).
+        const bool apart = p.hq > 0 && p.tokens_per_block > 1;
+        kern<<<(unsigned)p.kv_blocks + (p.hq && !apart ? (unsigned)p.total : 0u), kRopeThreads, smem, st>>>(p);
+        if (!apart || launch_status() != KVX_OK) return launch_status();
+        auto q_kern = half ? (vec ? rope_append_q_kernel<T, true, true> : rope_append_q_kernel<T, true, false>)
+                           : (vec ? rope_append_q_kernel<T, false, true> : rope_append_q_kernel<T, false, false>);
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)p.total);
+        cfg.blockDim = dim3(kRopeThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, q_kern, p) != cudaSuccess) {
+            cudaGetLastError();
+            return KVX_ECUDA;
+        }
     } else {
         auto kern = half ? (vec ? rope_append_kernel<T, true, true> : rope_append_kernel<T, true, false>)
                          : (vec ? rope_append_kernel<T, false, true> : rope_append_kernel<T, false, false>);
@@ -523,12 +626,11 @@ extern "C" KVX_API int kvx_rope_append(const kvx_paged *kv, const int32_t *block
     p.rotary = table ? table->rotary_dim : 2 * e;
     const bool half = table && table->layout == KVX_ROPE_HALF;
     const bool vec = rope_vector_sizes(kHeadDim, p.rotary, half, e);
-    p.half_layout = half;
     p.items = rope_items(kHeadDim, p.rotary, half, vec ? e : 1);
     p.amplitude = table ? table->amplitude : 1.f;
     // 16 tokens a CTA once their pages alone fill the SMs
     p.tokens_per_block = total_tokens >= kPageTokens * sm_count() ? kPageTokens : 1;
-    p.kv_blocks = (total_tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+    p.kv_blocks = (total_tokens + p.tokens_per_block - 1) / p.tokens_per_block * 2;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return io_dtype == KVX_F16 ? launch_rope_append<__half>(p, i8, half, vec, st)
                                : launch_rope_append<float>(p, i8, half, vec, st);

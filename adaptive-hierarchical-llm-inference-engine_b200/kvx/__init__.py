@@ -467,35 +467,68 @@ ROPE_LAYOUT = {"half": 0, "interleaved": 1}
 ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "llama3": 3, "yarn": 4}
 
 
+# These calls are made once per layer and step, so their checks are plain
+# comparisons and the message is only made when one fails.
+
 def _require(cond, what):
     if not cond:
         raise ValueError(what)
 
 
-def _on_device(tensors, stream, call):
-    """call(stream) with the tensors' device current, so that a launch never
+_rt = None  # (float16, float32, int32, current raw stream of a device, current device)
+
+
+def _runtime():
+    global _rt
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    _rt = (torch.float16, torch.float32, torch.int32, raw, torch.cuda.current_device)
+    return _rt
+
+
+def _launch(dev, stream, fn, *args):
+    """fn(*args, stream) with device `dev` current, so that a launch never
     lands on another device than its operands; stream None: that device's
     current one."""
-    torch = _torch()
-    dev = tensors[0].device
-    for t in tensors:
-        _require(t is None or t.device == dev and t.is_cuda, "tensors of one call lie on one CUDA device")
-    if dev.index == torch.cuda.current_device():
-        return call(_stream(stream))
-    with torch.cuda.device(dev):
-        return call(_stream(stream))
+    rt = _rt or _runtime()
+    if dev == rt[4]():
+        return fn(*args, rt[3](dev) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream)
+    with _torch().cuda.device(dev):
+        return fn(*args, rt[3](dev) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream)
+
+
+def _one_device(first, *others):
+    """The CUDA device that all of these tensors (or None) lie on."""
+    dev = first.get_device()
+    if dev < 0:
+        raise ValueError("tensors of one call lie on one CUDA device")
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("tensors of one call lie on one CUDA device")
+    return dev
 
 
 def _vector(t, n, what):
     """An int32 tensor [n] (n None: any length), contiguous."""
-    torch = _torch()
-    _require(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and (n is None or t.shape[0] == n),
-             f"{what}: contiguous int32 [{'n' if n is None else n}]")
+    if t.dtype != (_rt or _runtime())[2] or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+        raise ValueError(what + ": contiguous int32" + ("" if n is None else f" [{n}]"))
 
 
 def _flag(t):
-    torch = _torch()
-    _require(t is None or t.dtype == torch.int32 and t.numel() >= 1, "error_flag: int32, one element")
+    if t is None:
+        return None
+    if t.dtype != (_rt or _runtime())[2] or t.numel() < 1:
+        raise ValueError("error_flag: int32, one element")
+    return t.data_ptr()
+
+
+def _io_code(x, what):
+    rt = _rt or _runtime()
+    if x.dtype == rt[0]:
+        return KVX_F16
+    if x.dtype == rt[1]:
+        return KVX_F32
+    raise ValueError(what + ": float16 or float32")
 
 
 class RopeTable:
@@ -528,14 +561,17 @@ def rope_table(rotary_dim, base=10000.0, layout="half", scaling="none", factor=1
     return RopeTable(torch.tensor(signed, dtype=torch.int64).to(device), rotary_dim, layout, amplitude)
 
 
-def _rows3(x, what, like=None):
-    _require(x.dim() == 3 and (x.shape[2] <= 1 or x.stride(2) == 1), f"{what}: [tokens][heads][dim], last dimension contiguous")
-    _require(like is None or (x.shape == like.shape and x.dtype == like.dtype), f"{what}: shape and dtype of its input")
-
-
-def _single(x, what):
-    """No two elements of an output share memory by a stride of zero."""
-    _require(all(n <= 1 or st != 0 for n, st in zip(x.shape, x.stride())), f"{what}: strides without overlap")
+def _rope_rows(x, out, what):
+    """The RopeRows of a tensor [tokens][heads][dim] and its output."""
+    sx, so = x.stride(), out.stride()
+    shape = x.shape
+    if len(shape) != 3 or (shape[2] > 1 and (sx[2] != 1 or so[2] != 1)):
+        raise ValueError(what + ": [tokens][heads][dim], last dimension contiguous")
+    if out.shape != shape or out.dtype != x.dtype:
+        raise ValueError(what + "_out: shape and dtype of its input")
+    if (so[0] == 0 and shape[0] > 1) or (so[1] == 0 and shape[1] > 1):
+        raise ValueError(what + "_out: strides without overlap")
+    return RopeRows(x.data_ptr(), out.data_ptr(), shape[1], sx[0], sx[1], so[0], so[1])
 
 
 def rope(q, k, positions, table, q_out=None, k_out=None, inverse=False, stream=None):
@@ -543,62 +579,58 @@ def rope(q, k, positions, table, q_out=None, k_out=None, inverse=False, stream=N
     positions [tokens] (int32); any token and head strides.  q_out = q rotates
     in place.  inverse=True turns back, which is the gradient of the rotation.
     Returns (q_out, k_out)."""
-    torch = _torch()
-    _rows3(q, "q")
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _rows3(q_out, "q_out", q)
-    _single(q_out, "q_out")
-    tokens, _, dim = q.shape
-    if k is not None:
-        _rows3(k, "k")
-        _require(k.shape[0] == tokens and k.shape[2] == dim and k.dtype == q.dtype, "k: tokens, dim and dtype of q")
-        if k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        _rows3(k_out, "k_out", k)
-        _single(k_out, "k_out")
-    _vector(positions, tokens, "positions")
+        q_out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
     rows = (RopeRows * 2)()
-    n = 0
-    for x, o in ((q, q_out), (k, k_out)):
-        if x is not None:
-            rows[n] = RopeRows(x.data_ptr(), o.data_ptr(), x.shape[1], x.stride(0), x.stride(1), o.stride(0), o.stride(1))
-            n += 1
-    _require(q.dtype in (torch.float16, torch.float32), "q: float16 or float32")
-    rc = _on_device((q, q_out, k, k_out, positions, table.turns), stream,
-                    lambda st: lib.kvx_rope(C.byref(table.c), _ptr(positions), tokens, dim, _dtype_code(q), rows, n,
-                                            int(bool(inverse)), st))
-    _check("kvx_rope", rc)
+    rows[0] = _rope_rows(q, q_out, "q")
+    tokens, _, dim = q.shape
+    n = 1
+    if k is not None:
+        if k_out is None:
+            k_out = _torch().empty(k.shape, dtype=k.dtype, device=k.device)
+        rows[1] = _rope_rows(k, k_out, "k")
+        n = 2
+        if k.shape[0] != tokens or k.shape[2] != dim or k.dtype != q.dtype:
+            raise ValueError("k: tokens, dim and dtype of q")
+    _vector(positions, tokens, "positions")
+    code = _io_code(q, "q")
+    dev = _one_device(q, q_out, k, k_out, positions, table.turns)
+    rc = _launch(dev, stream, lib.kvx_rope, C.byref(table.c), positions.data_ptr(), tokens, dim, code, rows, n, 1 if inverse else 0)
+    if rc:
+        raise KvxError("kvx_rope", rc)
     return q_out, k_out
 
 
 def _packed(x, heads, what):
-    """[tokens][heads][128] with the heads of a token side by side."""
-    _require(x.dim() == 3 and x.shape[2] == HEAD_DIM and (heads is None or x.shape[1] == heads) and
-             (x.shape[0] == 0 or (x.stride(2) == 1 and (x.shape[1] <= 1 or x.stride(1) == HEAD_DIM))),
-             f"{what}: [tokens][heads][128], heads side by side")
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * HEAD_DIM
+    """Token stride of [tokens][heads][128] with the heads of a token side by side."""
+    shape, st = x.shape, x.stride()
+    if len(shape) != 3 or shape[2] != HEAD_DIM or (heads is not None and shape[1] != heads) or (
+            shape[0] and (st[2] != 1 or (shape[1] > 1 and st[1] != HEAD_DIM))):
+        raise ValueError(what + ": [tokens][heads][128], heads side by side")
+    return st[0] if shape[0] > 1 else shape[1] * HEAD_DIM
 
 
 def _ragged(block_table, q_start, positions):
-    torch = _torch()
-    _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.is_contiguous(),
-             "block_table: contiguous int32 [batch][max_pages]")
-    batch = block_table.shape[0]
+    if block_table.dtype != (_rt or _runtime())[2] or block_table.dim() != 2 or not block_table.is_contiguous():
+        raise ValueError("block_table: contiguous int32 [batch][max_pages]")
+    batch, max_pages = block_table.shape
     _vector(positions, batch, "positions")
     _vector(q_start, batch + 1, "q_start")
-    return batch
+    return batch, max_pages
 
 
-def _pool_tensors(pool, stats):
-    """paged(pool, stats) and the tensors behind it."""
-    torch = _torch()
+def _pool(pool, stats):
+    """paged(pool, stats), with the shapes of both checked, and the pool as a
+    tensor (None for a KvPaged view)."""
+    if isinstance(pool, KvPaged):
+        return pool, None
     kv = paged(pool, stats)
-    _require(kv.dtype != KVX_I8 or kv.stats, "stats: an int8 pool has them")
-    if stats is not None and not isinstance(pool, KvPaged):
-        _require(stats.dtype == torch.float32 and stats.is_contiguous() and
-                 tuple(stats.shape) == (kv.num_pages, 2, kv.num_kv_heads, 4), "stats: contiguous float32 [pages][2][hkv][4]")
-    return kv, (None if isinstance(pool, KvPaged) else pool, stats)
+    if kv.dtype == KVX_I8 and stats is None:
+        raise ValueError("stats: an int8 pool has them")
+    if stats is not None and (stats.dtype != (_rt or _runtime())[1] or not stats.is_contiguous() or
+                              tuple(stats.shape) != (kv.num_pages, 2, kv.num_kv_heads, 4)):
+        raise ValueError("stats: contiguous float32 [pages][2][hkv][4]")
+    return kv, pool
 
 
 def rope_append(pool, block_table, q_start, positions, k, v, q=None, q_out=None, table=None, stats=None, error_flag=None,
@@ -609,38 +641,40 @@ def rope_append(pool, block_table, q_start, positions, k, v, q=None, q_out=None,
     rotated and stored with v in the pages (int8 pools: quantised, stats
     updated); q is rotated into q_out, which is returned.  table None: no
     rotation."""
-    torch = _torch()
-    kv, tensors = _pool_tensors(pool, stats)
-    batch = _ragged(block_table, q_start, positions)
+    kv, tensor = _pool(pool, stats)
+    batch, max_pages = _ragged(block_table, q_start, positions)
     tokens = k.shape[0]
     ks, vs = _packed(k, kv.num_kv_heads, "k"), _packed(v, kv.num_kv_heads, "v")
-    _require(v.shape[0] == tokens and v.dtype == k.dtype and k.dtype in (torch.float16, torch.float32),
-             "k, v: as many tokens, both float16 or float32")
+    code = _io_code(k, "k")
+    if v.shape[0] != tokens or v.dtype != k.dtype:
+        raise ValueError("v: tokens and dtype of k")
     hq = qs = 0
+    q_ptr = out_ptr = None
     if q is not None:
         qs, hq = _packed(q, None, "q"), q.shape[1]
-        _require(q.shape[0] == tokens and q.dtype == k.dtype, "q: tokens and dtype of k")
+        if q.shape[0] != tokens or q.dtype != k.dtype:
+            raise ValueError("q: tokens and dtype of k")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _require(q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.is_contiguous(), "q_out: contiguous, shape and dtype of q")
-    else:
-        _require(q_out is None, "q_out: only with q")
-    _flag(error_flag)
-    rc = _on_device((k, v, q, q_out, block_table, q_start, positions, error_flag, None if table is None else table.turns) + tensors,
-                    stream,
-                    lambda st: lib.kvx_rope_append(
-                        C.byref(kv), _ptr(block_table), block_table.shape[1], _ptr(q_start), _ptr(positions), batch, tokens,
-                        None if table is None else C.byref(table.c), _dtype_code(k), _ptr(q), qs, _ptr(q_out), hq, _ptr(k), ks,
-                        _ptr(v), vs, _ptr(error_flag), st))
-    _check("kvx_rope_append", rc)
+            q_out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+        if q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
+            raise ValueError("q_out: contiguous, shape and dtype of q")
+        q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        raise ValueError("q_out: only with q")
+    dev = _one_device(k, v, q, q_out, block_table, q_start, positions, error_flag, tensor, stats,
+                      None if table is None else table.turns)
+    rc = _launch(dev, stream, lib.kvx_rope_append, C.byref(kv), block_table.data_ptr(), max_pages, q_start.data_ptr(),
+                 positions.data_ptr(), batch, tokens, None if table is None else C.byref(table.c), code, q_ptr, qs, out_ptr, hq,
+                 k.data_ptr(), ks, v.data_ptr(), vs, _flag(error_flag))
+    if rc:
+        raise KvxError("kvx_rope_append", rc)
     return q_out
 
 
 def attend_chunk_workspace(batch, total_tokens, num_q_heads, num_kv_heads, max_pages, device="cuda"):
     """Scratch of attend_chunk for calls up to this size (no initialisation needed)."""
-    torch = _torch()
     n = lib.kvx_attend_chunk_workspace_bytes(batch, total_tokens, num_q_heads, num_kv_heads, max_pages)
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+    return _torch().empty(max(n, 16), dtype=_torch().uint8, device=device)
 
 
 def attend_chunk(pool, block_table, q_start, positions, q, stats=None, out=None, workspace=None, error_flag=None,
@@ -649,23 +683,24 @@ def attend_chunk(pool, block_table, q_start, positions, q, stats=None, out=None,
     them already: packed rows q [tokens][hq][128] as in rope_append; the query
     at position p sees keys 0 .. p (causal=False: every key of its sequence,
     positions[s] + its new tokens)."""
-    torch = _torch()
-    kv, tensors = _pool_tensors(pool, stats)
-    batch = _ragged(block_table, q_start, positions)
-    _require(q.dim() == 3 and q.shape[2] == HEAD_DIM and q.is_contiguous() and q.dtype in (torch.float16, torch.float32),
-             "q: contiguous float16 or float32 [tokens][hq][128]")
+    kv, tensor = _pool(pool, stats)
+    batch, max_pages = _ragged(block_table, q_start, positions)
+    code = _io_code(q, "q")
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM or not q.is_contiguous():
+        raise ValueError("q: contiguous [tokens][hq][128]")
     tokens, hq, _ = q.shape
     if out is None:
-        out = torch.zeros_like(q)
-    _require(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "out: contiguous, shape and dtype of q")
+        out = _torch().zeros_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out: contiguous, shape and dtype of q")
     if workspace is None:
-        workspace = attend_chunk_workspace(batch, tokens, hq, kv.num_kv_heads, block_table.shape[1], q.device)
-    _require(workspace.is_contiguous(), "workspace: contiguous")
-    _flag(error_flag)
-    rc = _on_device((q, out, block_table, q_start, positions, workspace, error_flag) + tensors, stream,
-                    lambda st: lib.kvx_attend_chunk(
-                        C.byref(kv), _ptr(block_table), block_table.shape[1], _ptr(q_start), _ptr(positions), batch, tokens, hq,
-                        _ptr(q), _ptr(out), _dtype_code(q), sm_scale, int(bool(causal)), _ptr(workspace),
-                        workspace.numel() * workspace.element_size(), _ptr(error_flag), st))
-    _check("kvx_attend_chunk", rc)
+        workspace = attend_chunk_workspace(batch, tokens, hq, kv.num_kv_heads, max_pages, q.device)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace: contiguous")
+    dev = _one_device(q, out, block_table, q_start, positions, workspace, error_flag, tensor, stats)
+    rc = _launch(dev, stream, lib.kvx_attend_chunk, C.byref(kv), block_table.data_ptr(), max_pages, q_start.data_ptr(),
+                 positions.data_ptr(), batch, tokens, hq, q.data_ptr(), out.data_ptr(), code, sm_scale, 1 if causal else 0,
+                 workspace.data_ptr(), workspace.nbytes, _flag(error_flag))
+    if rc:
+        raise KvxError("kvx_attend_chunk", rc)
     return out

@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import ctypes as C
 
-from . import KvPaged, _check, _flag, _on_device, _pool_tensors, _ptr, _require, _torch, _vector, lib
+from . import KvPaged, KvxError, _flag, _launch, _one_device, _pool, _require, _torch, _vector, lib
 
 _vp, _i32, _sz = C.c_void_p, C.c_int32, C.c_size_t
 
@@ -50,13 +50,12 @@ class Pages:
         _require(stats is None or len(stats) == len(pools), "stats: one per pool")
         self.refcounts, self.block_table, self.seq_lens = refcounts, block_table, seq_lens
         self.pools, self.stats = list(pools), None if stats is None else list(stats)
-        described = [_pool_tensors(p, None if stats is None else stats[i]) for i, p in enumerate(self.pools)]
+        described = [_pool(p, None if stats is None else stats[i]) for i, p in enumerate(self.pools)]
         _require(all(kv.num_pages == refcounts.shape[0] for kv, _ in described), "refcounts: one per page of the pools")
-        self._tensors = [refcounts, block_table, seq_lens] + [t for _, ts in described for t in ts if t is not None]
-        _require(all(t.is_cuda and t.device == refcounts.device for t in self._tensors), "tensors lie on one CUDA device")
+        self._device = _one_device(refcounts, block_table, seq_lens, *(t for _, t in described), *(self.stats or ()))
         self._layers = (KvPaged * max(len(described), 1))(*(kv for kv, _ in described))
-        self._pages = PagesC(refcounts.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), refcounts.shape[0],
-                             block_table.shape[0], block_table.shape[1])
+        self._pages = C.byref(PagesC(refcounts.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), refcounts.shape[0],
+                                     block_table.shape[0], block_table.shape[1]))
         self._bytes = lib.kvx_pages_workspace_bytes(refcounts.shape[0], block_table.shape[0])
         self._workspace = torch.empty(max(self._bytes, 16), dtype=torch.uint8, device=refcounts.device)
 
@@ -68,41 +67,46 @@ class Pages:
                    torch.full((num_rows, max_pages), -1, dtype=torch.int32, device=device),
                    torch.zeros(num_rows, dtype=torch.int32, device=device), pools, stats)
 
-    def _run(self, name, tensors, error_flag, stream, call):
-        _flag(error_flag)
-        _check(name, _on_device((self.refcounts, *tensors, error_flag), stream, call))
+    def _run(self, fn, name, stream, tensors, *args):
+        for t in tensors:
+            if t is not None and t.get_device() != self._device:
+                raise ValueError("tensors of one call lie on one CUDA device")
+        rc = _launch(self._device, stream, fn, *args)
+        if rc:
+            raise KvxError(name, rc)
 
     def reserve(self, new_tokens, error_flag=None, stream=None):
         """Pages for the next new_tokens[row] tokens of every row."""
         _vector(new_tokens, self.block_table.shape[0], "new_tokens")
-        self._run("kvx_pages_reserve", (new_tokens,), error_flag, stream, lambda st: lib.kvx_pages_reserve(
-            C.byref(self._pages), _ptr(new_tokens), _ptr(self._workspace), self._bytes, _ptr(error_flag), st))
+        self._run(lib.kvx_pages_reserve, "kvx_pages_reserve", stream, (new_tokens, error_flag), self._pages, new_tokens.data_ptr(),
+                  self._workspace.data_ptr(), self._bytes, _flag(error_flag))
 
     def fork(self, parents, children, error_flag=None, stream=None):
         """Row children[i] (empty) becomes a copy of row parents[i]."""
         _vector(parents, None, "parents")
-        _vector(children, parents.shape[0], "children")
-        self._run("kvx_pages_fork", (parents, children), error_flag, stream, lambda st: lib.kvx_pages_fork(
-            C.byref(self._pages), self._layers, len(self.pools), _ptr(parents), _ptr(children), parents.shape[0],
-            _ptr(self._workspace), self._bytes, _ptr(error_flag), st))
+        n = parents.shape[0]
+        _vector(children, n, "children")
+        self._run(lib.kvx_pages_fork, "kvx_pages_fork", stream, (parents, children, error_flag), self._pages, self._layers,
+                  len(self.pools), parents.data_ptr(), children.data_ptr(), n, self._workspace.data_ptr(), self._bytes,
+                  _flag(error_flag))
 
     def free(self, rows, error_flag=None, stream=None):
         """Drop the pages of these rows."""
         _vector(rows, None, "rows")
-        self._run("kvx_pages_free", (rows,), error_flag, stream, lambda st: lib.kvx_pages_free(
-            C.byref(self._pages), _ptr(rows), rows.shape[0], _ptr(error_flag), st))
+        self._run(lib.kvx_pages_free, "kvx_pages_free", stream, (rows, error_flag), self._pages, rows.data_ptr(), rows.shape[0],
+                  _flag(error_flag))
 
     def compact(self, num_live=None, error_flag=None, stream=None):
         """Move the held pages to the front; num_live (int32 [1]) gets their number."""
         if num_live is not None:
             _vector(num_live, 1, "num_live")
-        self._run("kvx_pages_compact", (num_live,), error_flag, stream, lambda st: lib.kvx_pages_compact(
-            C.byref(self._pages), self._layers, len(self.pools), _ptr(self._workspace), self._bytes, _ptr(num_live),
-            _ptr(error_flag), st))
+        self._run(lib.kvx_pages_compact, "kvx_pages_compact", stream, (num_live, error_flag), self._pages, self._layers,
+                  len(self.pools), self._workspace.data_ptr(), self._bytes, None if num_live is None else num_live.data_ptr(),
+                  _flag(error_flag))
 
     def copy(self, src, dst, error_flag=None, stream=None):
         """Page src[i] to page dst[i] in every layer."""
         _vector(src, None, "src")
         _vector(dst, src.shape[0], "dst")
-        self._run("kvx_pages_copy", (src, dst), error_flag, stream, lambda st: lib.kvx_pages_copy(
-            self._layers, len(self.pools), _ptr(src), _ptr(dst), src.shape[0], _ptr(error_flag), st))
+        self._run(lib.kvx_pages_copy, "kvx_pages_copy", stream, (src, dst, error_flag), self._layers, len(self.pools), src.data_ptr(),
+                  dst.data_ptr(), src.shape[0], _flag(error_flag))
