@@ -27,6 +27,9 @@
 // rows they own 128 rows each and share every key tile; up to 128 rows they
 // take turns at the key tiles of the same rows and are merged at the end.
 //
+// Sequences of at most 16 rows (a decode step, a few drafted tokens) would use
+// an eighth of those tiles: attend_rows_kernel takes them, on mma.sync.
+//
 // fp16 calls: P' = p s 2^(7 - E) with 2^E above the largest V scale so far: at
 // most 2^15 and normal in fp16 down to p s = 2^-21 of that scale, so a block
 // of small scale keeps its precision.  fp32 calls: q (scaled to 2^13) and P'
@@ -72,8 +75,13 @@ struct ChunkParams {
     void *out;
     float *part_o;     // [split][total * hq][128]
     float2 *part_ml;   // [split][total * hq]
+    float *few_o;      // attend_rows_kernel: [CTA][2][16][128]
+    float2 *few_ml;    // [CTA][2][16]
     int32_t *error_flag;
-    int batch, total, hq, hkv, group, max_pages, num_pages, causal, chunk;  // chunk: key tiles of a split
+    int batch, total, hq, hkv, group, max_pages, num_pages, causal;
+    int chunk;             // attend_chunk_kernel: key tiles of a split
+    int few_ctas;          // attend_rows_kernel: CTAs
+    int few_rows;          // sequences of at most so many rows are attend_rows_kernel's (0: none)
     float scale_log2;
 };
 
@@ -104,7 +112,7 @@ __device__ __forceinline__ int row_keys(const ChunkParams &p, const RowTile &t, 
     return (int)min(k, (long long)p.max_pages * kPageTokens);
 }
 
-__device__ __forceinline__ RowTile row_tile(const ChunkParams &p, int s, int tile, int tile_rows) {
+__device__ __forceinline__ RowTile row_tile(const ChunkParams &p, int s, int tile, int tile_rows, int chunk) {
     RowTile t;
     t.begin = p.q_start[s];
     t.n = sequence_tokens(p, s);
@@ -113,7 +121,7 @@ __device__ __forceinline__ RowTile row_tile(const ChunkParams &p, int s, int til
     t.rows = min(tile_rows, all - tile * tile_rows);
     t.keys = row_keys(p, t, tile * tile_rows + t.rows - 1);
     t.tiles = (t.keys + kTileKeys - 1) / kTileKeys;
-    t.splits = max(1, (t.tiles + p.chunk - 1) / p.chunk);
+    t.splits = max(1, (t.tiles + chunk - 1) / chunk);
     return t;
 }
 
@@ -284,6 +292,17 @@ template <> __device__ __forceinline__ void load_q8<float>(const float *row, int
     f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
 }
 
+template <typename T> __device__ __forceinline__ void load_q4(const T *p, float *f);
+template <> __device__ __forceinline__ void load_q4<__half>(const __half *p, float *f) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    const float2 a = h2_to_f2(w.x), b = h2_to_f2(w.y);
+    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+}
+template <> __device__ __forceinline__ void load_q4<float>(const float *p, float *f) {
+    const float4 v = *reinterpret_cast<const float4 *>(p);
+    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+}
+
 template <typename T> __device__ __forceinline__ void store_out4(T *o, float a, float b, float c, float d);
 template <> __device__ __forceinline__ void store_out4<float>(float *o, float a, float b, float c, float d) {
     *reinterpret_cast<float4 *>(o) = make_float4(a, b, c, d);
@@ -311,7 +330,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         int before = 0, seq = -1, tile = 0;
         for (int s0 = 0; s0 < p.batch && seq < 0; s0 += 32) {
             const int s = s0 + lane;
-            const int mine = s < p.batch ? (sequence_tokens(p, s) * p.group + kTileRows - 1) / kTileRows : 0;
+            const int rows = s < p.batch ? sequence_tokens(p, s) * p.group : 0;
+            const int mine = rows > p.few_rows ? (rows + kTileRows - 1) / kTileRows : 0;
             int x = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -335,7 +355,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     __syncthreads();
     const int seq = bars->seq, tile = bars->tile;
     if (seq < 0) return;  // the grid is an upper bound
-    const RowTile rt = row_tile(p, seq, tile, kTileRows);
+    const RowTile rt = row_tile(p, seq, tile, kTileRows, p.chunk);
     if (split >= rt.splits) return;
     const int row0 = tile * kTileRows;
     if (threadIdx.x == 0 && split == 0 && p.error_flag) {
@@ -798,37 +818,487 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     }
 }
 
+// ---- at most 16 rows
+
+constexpr int kFewWarps = 4, kFewRows = 16;
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+// The product alone (a zero accumulator).
+__device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// 16 bytes, memory to shared memory, in this thread's next group
+__device__ __forceinline__ void copy16(uint32_t to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
+// One page of one head: 16 rows of K, 16 of V, their statistics.  16-byte
+// chunk c of row r lies at few_chunk(r, c), so that neither reader (K: the
+// same chunk of rows r and r + 1; V: rows r, r + 4, r + 8, r + 12) meets
+// itself in a bank.
+constexpr int kFewStages = 3;
+struct FewPage {
+    uint8_t k[kBlockBytes], v[kBlockBytes];
+    float4 ks, vs;
+};
+__device__ __forceinline__ int few_chunk(int row, int chunk) {
+    return row * kHeadDim + 16 * (chunk ^ (((row >> 2) << 1) ^ ((row & 1) << 2)));
+}
+template <bool kSplit> struct FewShared {
+    union {
+        FewPage page[kFewStages];
+        float o[kFewRows][kHeadDim + 4];  // once the warp has no more pages
+    } of[kFewWarps];
+    uint4 q_frag[kSplit ? 2 : 1][8][32];
+    int row_at[kFewRows], row_limit[kFewRows];
+    float row_sum[kFewRows], row_unscale[kFewRows], m[kFewWarps][kFewRows], l[kFewWarps][kFewRows];
+};
+
+// The key tiles of the sequences of at most 16 rows, one (sequence, kv-head)
+// after the other, are dealt out to the CTAs in equal ranges, whatever the
+// lengths (which the host does not know).
+struct FewWork {
+    int tiles;  // of all
+    int ctas;   // that have a range (at least kFewTiles tiles each, where there are so many)
+};
+constexpr int kFewTiles = 2;
+
+__device__ __forceinline__ int few_tiles(const ChunkParams &p, int s) {  // of one kv-head; one even where nothing is seen
+    const int rows = sequence_tokens(p, s) * p.group;
+    return rows > 0 && rows <= p.few_rows ? max(1, row_tile(p, s, 0, kFewRows, 1).tiles) : 0;
+}
+__device__ __forceinline__ int few_used(const ChunkParams &p, int tiles) { return max(1, min(p.few_ctas, tiles / kFewTiles)); }
+// By a whole warp: the work, and the tiles before sequence `seq`.
+__device__ __forceinline__ FewWork few_work(const ChunkParams &p, int seq, int *before) {
+    int all = 0, first = 0;
+    for (int s = threadIdx.x & 31; s < p.batch; s += 32) {
+        const int t = few_tiles(p, s) * p.hkv;
+        all += t;
+        if (s < seq) first += t;
+    }
+    *before = __reduce_add_sync(0xffffffffu, first);
+    FewWork w;
+    w.tiles = __reduce_add_sync(0xffffffffu, all);
+    w.ctas = few_used(p, w.tiles);
+    return w;
+}
+__device__ __forceinline__ int few_begin(const FewWork &w, int cta) { return (int)((long long)w.tiles * cta / w.ctas); }
+__device__ __forceinline__ int few_owner(const FewWork &w, int tile) { return (int)((((long long)tile + 1) * w.ctas - 1) / w.tiles); }
+
+// Sequences of at most 16 rows: bound by the codes' bytes.  A CTA's 4 warps
+// take the pages of its range in turn.  The codes go from memory to the operands of mma.sync (m16n8k16) in registers:
+// the order of the dims within Q K^T, and of the keys and dims within P V, is
+// free as long as both operands agree, so with g = lane / 4, q = lane % 4
+//  * K: a lane reads dims 16 q .. + 15 and 64 + 16 q .. + 15 of key
+//    4 (g / 2) + g % 2 (+ 2 for the second n-tile); word s of those 32 bytes
+//    is its B fragment of k-step s.  Its scores are then keys 4 q .. 4 q + 3;
+//  * V: a lane reads dims 16 g .. + 15 of keys 4 q .. 4 q + 3, transposes them
+//    4 x 4 bytes at a time, and has its B fragments of the 16 n-tiles: n-tile
+//    t holds dims 16 n + t, so the lane ends with dims 32 q .. 32 q + 31 of O.
+// A page is one k-step of P V and has one V scale, so the scale is applied to
+// its product in fp32.  Where a range
+// ends inside a (sequence, kv-head) the rows' partial results go to the
+// workspace; a CTA has two such ends at most.
+template <typename T, bool kSplit>
+__global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_kernel(const __grid_constant__ ChunkParams p) {
+    extern __shared__ __align__(16) uint8_t few_smem[];
+    FewShared<kSplit> &sh = *reinterpret_cast<FewShared<kSplit> *>(few_smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3, cta = blockIdx.x;
+    grid_dependents_launch();
+    // this CTA's tiles, and the sequence that the first belongs to
+    int w0 = 0, w1 = 0, seq = 0, before = 0;  // before: tiles of earlier sequences
+    {
+        const int t = lane < p.batch ? few_tiles(p, lane) * p.hkv : 0;  // the first 32 sequences, looked at once
+        int all = t;
+        for (int i = 32 + lane; i < p.batch; i += 32) all += few_tiles(p, i) * p.hkv;
+        FewWork work_of;
+        work_of.tiles = __reduce_add_sync(0xffffffffu, all);
+        work_of.ctas = few_used(p, work_of.tiles);
+        if (cta < work_of.ctas) {
+            w0 = few_begin(work_of, cta);
+            w1 = few_begin(work_of, cta + 1);
+            for (int s0 = 0;; s0 += 32) {
+                const int mine = s0 == 0 ? t : (s0 + lane < p.batch ? few_tiles(p, s0 + lane) * p.hkv : 0);
+                int x = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, x, o);
+                    if (lane >= o) x += y;
+                }
+                const uint32_t hit = __ballot_sync(0xffffffffu, w0 < before + x);
+                if (hit || s0 + 32 >= p.batch) {
+                    const int at = hit ? __ffs(hit) - 1 : 0;
+                    seq = s0 + at;
+                    before += __shfl_sync(0xffffffffu, x - mine, at);
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, x, 31);
+            }
+        }
+    }
+#pragma unroll 1
+    for (int w = w0; w < w1;) {
+        RowTile rt = row_tile(p, seq, 0, kFewRows, 1);
+        const int n_rows = rt.n * p.group, seq_tiles = n_rows > 0 && n_rows <= p.few_rows ? max(1, rt.tiles) : 0;
+        if (w >= before + seq_tiles * p.hkv) {
+            before += seq_tiles * p.hkv;
+            ++seq;
+            continue;
+        }
+        const int kvh = (w - before) / seq_tiles, tile0 = (w - before) % seq_tiles;
+        const int piece = min(seq_tiles - tile0, w1 - w);  // tiles of it in this range
+        const bool whole = piece == seq_tiles, first_piece = w == w0;
+        w += piece;
+        if (threadIdx.x == 0 && tile0 == 0 && p.error_flag) {
+            if (rt.pos < 0) atomicOr(p.error_flag, 2);
+            if ((long long)rt.pos + rt.n > (long long)p.max_pages * kPageTokens) atomicOr(p.error_flag, 4);
+        }
+        const int page0 = tile0 * kTilePages, page1 = min(page0 + piece * kTilePages, (rt.keys + kPageTokens - 1) / kPageTokens);
+        const int32_t *table = p.block_table + (size_t)seq * p.max_pages;
+        auto page_of = [&](int lp) { return lp < page1 ? table[lp] : -1; };
+        const int key_a = 4 * (g >> 1) + (g & 1);  // key of this lane's column of Q K^T (+ 2 for the second n-tile)
+        // this warp's pages page0 + warp, + 4, ...: contents three ahead, ids of 32 at once
+        const int first = page0 + warp, count = first < page1 ? (page1 - first + kFewWarps - 1) / kFewWarps : 0;
+        FewPage *page = sh.of[warp].page;
+        int ids = page_of(first + lane * kFewWarps);
+        uint32_t here = 0;  // bit i % 32: page i has an id that is one
+        auto fetch = [&](int i, int stage) {
+            if (i < count) {
+                if (i && !(i & 31)) ids = page_of(first + (i + lane) * kFewWarps);
+                const int phys = __shfl_sync(0xffffffffu, ids, i & 31);
+                const bool known = phys >= 0 && phys < p.num_pages;
+                here = (here & ~(1u << (i & 31))) | (uint32_t)known << (i & 31);
+                if (known) {
+                    const size_t kb = (size_t)phys * 2 * p.hkv + kvh;
+                    const int row = lane >> 3, chunk = lane & 7;
+                    const uint8_t *k = p.pool + kb * kBlockBytes + 16 * lane, *v = k + (size_t)p.hkv * kBlockBytes;
+                    const uint32_t to = smem_addr(&page[stage]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) copy16(to + few_chunk(row + 4 * j, chunk), k + 512 * j);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) copy16(to + kBlockBytes + few_chunk(row + 4 * j, chunk), v + 512 * j);
+                    if (lane < 2) copy16(to + 2 * kBlockBytes + 16 * lane, reinterpret_cast<const float4 *>(p.stats) + kb + lane * p.hkv);
+                }
+            }
+            copy_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < kFewStages; ++i) fetch(i, i);
+
+        // where each row of q and out lies, and up to which key it sees
+        if (threadIdx.x < kFewRows) {
+            const int row = min((int)threadIdx.x, n_rows - 1);  // rows that are none see what the last one sees
+            sh.row_at[threadIdx.x] = (rt.begin + row / p.group) * p.hq + kvh * p.group + row % p.group;
+            sh.row_limit[threadIdx.x] = row_keys(p, rt, row);
+        }
+        __syncthreads();
+        // q: row sums and (fp32) scales by warps, then the A fragments
+        const T *q = static_cast<const T *>(p.q);
+        for (int row = warp; row < n_rows; row += kFewWarps) {
+            float f[4], big = 0.f;
+            load_q4<T>(q + (size_t)sh.row_at[row] * kHeadDim + 4 * lane, f);
+            float sum = f[0] + f[1] + f[2] + f[3];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if constexpr (kSplit) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) big = fmaxf(big, fabsf(f[k]));
+#pragma unroll
+                for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            }
+            if (lane == 0) {
+                sh.row_sum[row] = sum;
+                sh.row_unscale[row] = kSplit && big > 0.f && big < CUDART_INF_F ? pow2i(exponent_above(big) - 13) : 1.f;
+            }
+        }
+        if constexpr (kSplit) __syncthreads();
+#pragma unroll
+        for (int s0 = 0; s0 < 8; s0 += kFewWarps) {
+            const int s = s0 + warp, d = (s >> 2) * 64 + 16 * q4 + 4 * (s & 3);  // this lane's four dims of k-step s
+            uint32_t hi[2][2], lo[2][2];                                         // [row g, g + 8][dims d, d + 2]
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = g + 8 * r;
+                float f[4] = {0.f, 0.f, 0.f, 0.f};
+                if (row < n_rows) {
+                    load_q4<T>(q + (size_t)sh.row_at[row] * kHeadDim + d, f);
+                    if constexpr (kSplit) {
+                        const float up = 1.f / sh.row_unscale[row];  // a power of two
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) f[k] *= up;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    hi[r][k] = pack_half(f[2 * k], f[2 * k + 1]);
+                    if constexpr (kSplit) {
+                        const float2 h = h2_to_f2(hi[r][k]);
+                        lo[r][k] = pack_half(f[2 * k] - h.x, f[2 * k + 1] - h.y);
+                    }
+                }
+            }
+            sh.q_frag[0][s][lane] = make_uint4(hi[0][0], hi[1][0], hi[0][1], hi[1][1]);
+            if constexpr (kSplit) sh.q_frag[1][s][lane] = make_uint4(lo[0][0], lo[1][0], lo[0][1], lo[1][1]);
+        }
+        __syncthreads();
+
+        uint64_t o[16][2];  // n-tile t: two dims of row g, of row g + 8
+#pragma unroll
+        for (int t = 0; t < 16; ++t) o[t][0] = o[t][1] = 0;
+        // rows g and g + 8
+        int limit[2];
+        float m[2], l[2], z[2], q_sum[2], unscale[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = g + 8 * r;
+            limit[r] = sh.row_limit[row];
+            m[r] = -CUDART_INF_F;
+            l[r] = z[r] = 0.f;
+            q_sum[r] = row < n_rows ? sh.row_sum[row] : 0.f;
+            unscale[r] = row < n_rows ? sh.row_unscale[row] : 1.f;
+        }
+        const int least = sh.row_limit[0];  // the first row sees the fewest keys
+
+        int stage = 0;
+#pragma unroll 1
+        for (int i = 0; i < count; ++i) {
+            copy_wait<kFewStages - 1>();
+            __syncwarp();
+            const FewPage &f = page[stage];
+            if (!(here >> (i & 31) & 1)) {
+                if (p.error_flag && lane == 0) atomicOr(p.error_flag, 2);
+                fetch(i + kFewStages, stage);
+                stage = stage == kFewStages - 1 ? 0 : stage + 1;
+                continue;
+            }
+            const float2 ks = make_float2(f.ks.z, f.ks.w), vs = make_float2(f.vs.z, f.vs.w);  // {scale, zero point}
+            uint4 kw[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) kw[j][h] = *reinterpret_cast<const uint4 *>(f.k + few_chunk(key_a + 2 * j, q4 + 4 * h));
+            float c[2][4], c2[2][4];  // even and odd steps: two chains each
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const uint4 a = sh.q_frag[0][s][lane];
+                uint4 al;
+                if constexpr (kSplit) al = sh.q_frag[1][s][lane];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint4 &w = kw[j][s >> 2];
+                    const uint2 b = codes_to_half((s & 3) == 0 ? w.x : (s & 3) == 1 ? w.y : (s & 3) == 2 ? w.z : w.w);
+                    float(&d)[4] = s & 1 ? c2[j] : c[j];
+                    if (s < 2)
+                        mma_f16_zero(d, a, b.x, b.y);
+                    else
+                        mma_f16(d, a, b.x, b.y);
+                    if constexpr (kSplit) mma_f16(d, al, b.x, b.y);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[j][e] += c2[j][e];
+            // scores (log2): keys key0 + 4 q + 2 j + e of rows g (c[j][e]) and g + 8 (c[j][2 + e])
+            const int key0 = (first + i * kFewWarps) * kPageTokens;
+            const bool masked = least < key0 + kPageTokens;
+            const float k_mid = fmaf(128.f, ks.x, ks.y) * p.scale_log2, v_mid = fmaf(128.f, vs.x, vs.y);
+            float scale[2], top[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float a = ks.x * p.scale_log2 * unscale[r], b = k_mid * q_sum[r];
+                top[r] = -CUDART_INF_F;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float &x = c[j][2 * r + e];
+                        x = fmaf(a, x, b);
+                        if (masked && key0 + 4 * q4 + 2 * j + e >= limit[r]) x = -CUDART_INF_F;
+                        top[r] = fmaxf(top[r], x);
+                    }
+                // a row that sees nothing of the page takes nothing from it, whatever its statistics
+                scale[r] = masked && limit[r] <= key0 ? 0.f : vs.x;
+            }
+            if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                    const float mn = fmaxf(m[r], top[r]), f_ = mn == -CUDART_INF_F ? 1.f : ex2(m[r] - mn);
+                    m[r] = mn;
+                    l[r] *= f_;
+                    z[r] *= f_;
+                    const uint64_t ff = pack2(f_, f_);
+#pragma unroll
+                    for (int t = 0; t < 16; ++t) o[t][r] = mul2(o[t][r], ff);
+                }
+            }
+            const uint64_t ss0 = pack2(scale[0], scale[0]), ss1 = pack2(scale[1], scale[1]);
+            uint4 ph, pl;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float m_use = m[r] == -CUDART_INF_F ? 0.f : m[r];
+                float e4[4], sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {  // keys 4 q + k
+                    e4[k] = ex2(c[k >> 1][2 * r + (k & 1)] - m_use);
+                    sum += e4[k];
+                }
+                l[r] += sum;
+                if (!masked || limit[r] > key0) z[r] = fmaf(sum, v_mid, z[r]);
+                const uint32_t a = pack_half(e4[0], e4[1]), b = pack_half(e4[2], e4[3]);
+                (r ? ph.y : ph.x) = a;
+                (r ? ph.w : ph.z) = b;
+                if constexpr (kSplit) {
+                    const float2 x = h2_to_f2(a), y = h2_to_f2(b);
+                    (r ? pl.y : pl.x) = pack_half(e4[0] - x.x, e4[1] - x.y);
+                    (r ? pl.w : pl.z) = pack_half(e4[2] - y.x, e4[3] - y.y);
+                }
+            }
+            uint4 vw[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) vw[j] = *reinterpret_cast<const uint4 *>(f.v + few_chunk(4 * q4 + j, g));
+            __syncwarp();  // the warp is done with the stage
+            fetch(i + kFewStages, stage);
+            stage = stage == kFewStages - 1 ? 0 : stage + 1;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t r4[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r4[j] = w == 0 ? vw[j].x : w == 1 ? vw[j].y : w == 2 ? vw[j].z : vw[j].w;
+                const uint32_t a = __byte_perm(r4[0], r4[1], 0x5140), b = __byte_perm(r4[2], r4[3], 0x5140);
+                const uint32_t d = __byte_perm(r4[0], r4[1], 0x7362), e = __byte_perm(r4[2], r4[3], 0x7362);
+                const uint32_t col[4] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(d, e, 0x5410),
+                                         __byte_perm(d, e, 0x7632)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint2 v = codes_to_half(col[i]);
+                    float t[4];
+                    mma_f16_zero(t, ph, v.x, v.y);
+                    if constexpr (kSplit) mma_f16(t, pl, v.x, v.y);
+                    o[4 * w + i][0] = fma2(ss0, pack2(t[0], t[1]), o[4 * w + i][0]);
+                    o[4 * w + i][1] = fma2(ss1, pack2(t[2], t[3]), o[4 * w + i][1]);
+                }
+            }
+        }
+        copy_wait<0>();
+        __syncwarp();
+
+        // ---- the quad's sums, then the warps
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (int off = 1; off < 4; off <<= 1) {
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], off);
+                z[r] += __shfl_xor_sync(0xffffffffu, z[r], off);
+            }
+            const int row = g + 8 * r;
+            if (q4 == 0) {
+                sh.m[warp][row] = m[r];
+                sh.l[warp][row] = l[r];
+            }
+#pragma unroll
+            for (int t = 0; t < 16; t += 4) {
+                float2 x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = unpack2(o[t + k][r]);
+                float *to = &sh.of[warp].o[row][32 * q4 + t];
+                *reinterpret_cast<float4 *>(to) = make_float4(x[0].x + z[r], x[1].x + z[r], x[2].x + z[r], x[3].x + z[r]);
+                *reinterpret_cast<float4 *>(to + 16) = make_float4(x[0].y + z[r], x[1].y + z[r], x[2].y + z[r], x[3].y + z[r]);
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n_rows * (kHeadDim / 4); i += kFewWarps * 32) {
+            const int row = i / (kHeadDim / 4), d = 4 * (i % (kHeadDim / 4));
+            float M = sh.m[0][row];
+#pragma unroll
+            for (int w = 1; w < kFewWarps; ++w) M = fmaxf(M, sh.m[w][row]);
+            float L = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kFewWarps; ++w) {
+                const float f = sh.m[w][row] == -CUDART_INF_F && sh.l[w][row] == 0.f ? 0.f : ex2(sh.m[w][row] - M);
+                const float4 v = *reinterpret_cast<const float4 *>(&sh.of[w].o[row][d]);
+                L = fmaf(f, sh.l[w][row], L);
+                acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+            }
+            if (whole) {
+                const float inv = L == 0.f ? 0.f : 1.f / L;
+                store_out4<T>(static_cast<T *>(p.out) + (size_t)sh.row_at[row] * kHeadDim + d, acc.x * inv, acc.y * inv, acc.z * inv,
+                               acc.w * inv);
+            } else {
+                const size_t at = ((size_t)2 * cta + !first_piece) * kFewRows + row;
+                *reinterpret_cast<float4 *>(p.few_o + at * kHeadDim + d) = acc;
+                if (d == 0) p.few_ml[at] = make_float2(M, L);
+            }
+        }
+        __syncthreads();  // shared memory is free for the next piece
+    }
+    grid_dependency_wait();  // the other kernel's rows are done when this grid is
+}
+
 // out[row] of the rows whose keys were split: one warp per row, 4 dims a lane.
 template <typename T>
 __global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_constant__ ChunkParams p, int tile_rows) {
-    grid_dependency_wait();
     const size_t row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, t = (int)(row / p.hq), h = (int)(row % p.hq);
-    if (t >= p.total) return;
     int s = -1;
-    for (int s0 = 0; s0 < p.batch && s < 0; s0 += 32) {
+    for (int s0 = 0; s0 < p.batch && s < 0 && t < p.total; s0 += 32) {
         const int i = s0 + lane;
         const uint32_t hit = __ballot_sync(0xffffffffu, i < p.batch && p.q_start[i] >= 0 && p.q_start[i] <= t && t < p.q_start[i + 1]);
         if (hit) s = s0 + __ffs(hit) - 1;
     }
-    if (s < 0) return;
-    const int tile = ((t - p.q_start[s]) * p.group + h % p.group) / tile_rows;
-    const int splits = row_tile(p, s, tile, tile_rows).splits;
+    bool few = false, late = false;  // late: the first part lies in its CTA's second place
+    int splits = 1;
+    size_t at = row, step = (size_t)p.total * p.hq;
+    if (s >= 0) {
+        const int r = (t - p.q_start[s]) * p.group + h % p.group;  // among the rows of its (sequence, kv-head)
+        few = sequence_tokens(p, s) * p.group <= p.few_rows;
+        if (few) {
+            int before;
+            const FewWork work_of = few_work(p, s, &before);
+            const int tiles = few_tiles(p, s);
+            before += h / p.group * tiles;
+            const int first = few_owner(work_of, before);
+            splits = few_owner(work_of, before + tiles - 1) - first + 1;
+            late = few_begin(work_of, first) < before;
+            at = (size_t)first * 2 * kFewRows + r;
+            step = 2 * kFewRows;
+        } else {
+            splits = row_tile(p, s, r / tile_rows, tile_rows, p.chunk).splits;
+        }
+    }
+    grid_dependency_wait();  // until here only the call's own arguments are read; every thread waits, so this grid ends last
     if (splits == 1) return;
-    const size_t step = (size_t)p.total * p.hq;
+    const float2 *part_ml = few ? p.few_ml : p.part_ml;
+    const float *part_o = few ? p.few_o : p.part_o;
+    auto part = [&](int c) { return at + c * step + (c == 0 && late ? kFewRows : 0); };
     float M = -CUDART_INF_F;
-    for (int c = lane; c < splits; c += 32) M = fmaxf(M, p.part_ml[c * step + row].x);
+    for (int c = lane; c < splits; c += 32) M = fmaxf(M, part_ml[part(c)].x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     float L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int c = 0; c < splits; ++c) {
-        const float2 ml = p.part_ml[c * step + row];
-        const float4 v = reinterpret_cast<const float4 *>(p.part_o + (c * step + row) * kHeadDim)[lane];
-        const float w = ml.x == -CUDART_INF_F ? 0.f : ex2(ml.x - M);
-        L += w * ml.y;
-        acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
+        const float2 ml = part_ml[part(c)];
+        const float4 v = reinterpret_cast<const float4 *>(part_o + part(c) * kHeadDim)[lane];
+        const float w = ml.x == -CUDART_INF_F && ml.y == 0.f ? 0.f : ex2(ml.x - M);
+        L = fmaf(w, ml.y, L);
+        acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     store_out4<T>(static_cast<T *>(p.out) + row * kHeadDim + 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
@@ -838,45 +1308,81 @@ constexpr int kMinChunk = 4;  // key tiles: below, a CTA's start and end outweig
 
 int key_tiles(int max_pages) { return (max_pages + kTilePages - 1) / kTilePages; }
 
-// Key tiles of a split: one split while the row tiles (an upper bound of them)
-// fill the SMs, else as many as give every SM about two CTAs.
-long long most_splits(int batch, long long rows, int hkv, int max_pages, int tile_rows) {
-    const long long ctas = (rows / tile_rows + batch) * hkv;
-    return std::min<long long>(std::max<long long>(1, 2LL * sm_count() / ctas), std::max(1, key_tiles(max_pages) / kMinChunk));
+// Splits of the keys: one while `ctas` (an upper bound of the CTAs that have
+// rows) fill `slots`, else as many as fill them.
+long long most_splits(long long ctas, long long slots, int max_pages) {
+    return std::min<long long>(std::max<long long>(1, slots / ctas), std::max(1, key_tiles(max_pages) / kMinChunk));
 }
+long long chunk_slots() { return 2LL * sm_count(); }  // about two CTAs an SM (one is resident)
+// CTAs of attend_rows_kernel: what is resident, by shared memory (fp32) and registers
+int few_ctas(bool fp32) { return (fp32 ? 3 : 4) * sm_count(); }
 
-template <typename T, bool kSplit>
-int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
-    constexpr int tile_rows = kSplit ? 128 : 256;
-    auto kern = attend_chunk_kernel<T, kSplit>;
-    static std::atomic<bool> attr_done[kMaxDevices];
-    if (ensure_smem_attr(attr_done, kern, kChunkSmem) != KVX_OK) return KVX_ECUDA;
-    const long long rows = (long long)p.total * p.group;
-    const int tiles = key_tiles(p.max_pages);
-    const long long most = most_splits(p.batch, rows, p.hkv, p.max_pages, tile_rows);
-    p.chunk = (int)((tiles + most - 1) / most);
-    const int splits = (tiles + p.chunk - 1) / p.chunk;
-    const size_t all = (size_t)p.total * p.hq;
-    p.part_o = static_cast<float *>(workspace);
-    p.part_ml = reinterpret_cast<float2 *>(p.part_o + (size_t)splits * all * kHeadDim);
-    const dim3 grid((unsigned)(rows / tile_rows + p.batch), (unsigned)p.hkv, (unsigned)splits);
-    kern<<<grid, kChunkThreads, kChunkSmem, st>>>(p);
-    int rc = launch_status();
-    if (rc != KVX_OK || splits == 1) return rc;
+// A launch that may start while the one before it in the stream runs.
+template <typename... Args>
+int launch_beside(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t st, const Args &...args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((all + 7) / 8));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, attend_combine_kernel<T>, p, tile_rows) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) {
         cudaGetLastError();
         return KVX_ECUDA;
     }
     return launch_status();
+}
+
+// attend_chunk_kernel, attend_rows_kernel beside it, and the combine when keys
+// are split.  Only the device knows the sequences' lengths, so both kernels
+// are launched unless the sizes rule one out: every row in sequences of at
+// most 16 (few enough rows in all), or a single longer sequence.
+template <typename T, bool kSplit>
+int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
+    constexpr int tile_rows = kSplit ? 128 : 256;
+    auto kern = attend_chunk_kernel<T, kSplit>;
+    static std::atomic<bool> attr_done[kMaxDevices];
+    if (ensure_smem_attr(attr_done, kern, kChunkSmem) != KVX_OK) return KVX_ECUDA;
+    auto few_kern = attend_rows_kernel<T, kSplit>;
+    constexpr int few_smem = sizeof(FewShared<kSplit>);
+    static std::atomic<bool> few_attr_done[kMaxDevices];
+    if (ensure_smem_attr(few_attr_done, few_kern, few_smem) != KVX_OK) return KVX_ECUDA;
+    const long long rows = (long long)p.total * p.group;
+    const bool chunk = rows > kFewRows, few = p.batch > 1 || rows <= kFewRows;
+    p.few_rows = few ? kFewRows : 0;
+    const int tiles = key_tiles(p.max_pages);
+    // row tiles: a sequence of more than 16 rows has one tile beside its whole ones
+    const long long grid_x = rows / tile_rows + (few ? std::min<long long>(p.batch, rows / (kFewRows + 1)) : p.batch);
+    const long long most = chunk ? most_splits(grid_x * p.hkv, chunk_slots(), p.max_pages) : 1;
+    p.chunk = (int)((tiles + most - 1) / most);
+    const int splits = (tiles + p.chunk - 1) / p.chunk;
+    const size_t all = (size_t)p.total * p.hq, few_all = (size_t)few_ctas(kSplit) * 2 * kFewRows;
+    p.few_ctas = few_ctas(kSplit);
+    p.few_o = static_cast<float *>(workspace);
+    p.few_ml = reinterpret_cast<float2 *>(p.few_o + few_all * kHeadDim);
+    p.part_o = p.few_o + (few ? few_all * (kHeadDim + 2) : 0);
+    p.part_ml = reinterpret_cast<float2 *>(p.part_o + (size_t)splits * all * kHeadDim);
+    int rc = KVX_OK;
+    if (chunk) {
+        const dim3 grid((unsigned)grid_x, (unsigned)p.hkv, (unsigned)splits);
+        kern<<<grid, kChunkThreads, kChunkSmem, st>>>(p);
+        rc = launch_status();
+    }
+    if (few && rc == KVX_OK) {
+        const dim3 grid((unsigned)p.few_ctas);
+        if (chunk) {
+            rc = launch_beside(few_kern, grid, kFewWarps * 32, few_smem, st, p);
+        } else {
+            few_kern<<<grid, kFewWarps * 32, few_smem, st>>>(p);
+            rc = launch_status();
+        }
+    }
+    if (rc != KVX_OK || (splits == 1 && !few)) return rc;
+    return launch_beside(attend_combine_kernel<T>, dim3((unsigned)((all + 7) / 8)), 256, 0, st, p, tile_rows);
 }
 
 }  // namespace
@@ -884,17 +1390,18 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
 
 using namespace kvx;
 
-// For every call of at most this many sequences, tokens and pages: with
-// ctas >= hkv * (rows / tile_rows + 1), splits * rows * hkv < 2 SMs * tile_rows.
+// For every call of at most this many sequences, tokens and pages: splits *
+// row tiles * kv-heads stays below the slots, so the rows of the partial
+// results below slots * tile_rows; never more splits than one CTA would get.
 extern "C" KVX_API size_t kvx_attend_chunk_workspace_bytes(int32_t batch, int32_t total_tokens, int32_t num_q_heads,
                                                            int32_t num_kv_heads, int32_t max_pages) {
     if (batch <= 0 || total_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
         max_pages <= 0)
         return 0;
-    const long long splits = most_splits(1, 1, num_kv_heads, max_pages, 128);
-    if (splits == 1) return 16;
-    const long long rows = std::min(splits * total_tokens * num_q_heads, 2LL * sm_count() * 256);
-    return (size_t)std::max(rows, 1LL) * (kHeadDim + 2) * sizeof(float) / 16 * 16 + 16;
+    const long long splits = most_splits(num_kv_heads, chunk_slots(), max_pages);
+    long long rows = 2LL * few_ctas(false) * kFewRows;
+    if (splits > 1) rows += std::min(splits * total_tokens * num_q_heads, chunk_slots() * 256);
+    return (size_t)rows * (kHeadDim + 2) * sizeof(float) + 16;
 }
 
 extern "C" KVX_API int kvx_attend_chunk(const kvx_paged *kv, const int32_t *block_table, int32_t max_pages,
@@ -909,8 +1416,9 @@ extern "C" KVX_API int kvx_attend_chunk(const kvx_paged *kv, const int32_t *bloc
     if (io_dtype != KVX_F16 && io_dtype != KVX_F32) return KVX_EINVAL;
     if (kv->dtype != KVX_I8 || kv->head_dim != kHeadDim || kv->page_tokens != kPageTokens) return KVX_EUNSUPPORTED;
     if (kv->num_kv_heads > 65535 || max_pages > (0x7fffffff - kTileKeys) / kPageTokens ||
-        (long long)total_tokens * num_q_heads > 0x3fffffff)
-        return KVX_EUNSUPPORTED;  // grid, key and row counts fit an int
+        (long long)total_tokens * num_q_heads > 0x3fffffff ||
+        (long long)batch * kv->num_kv_heads * key_tiles(max_pages) > 0x7fffffff)
+        return KVX_EUNSUPPORTED;  // grid, key, row and tile counts fit an int
     if (!kv->stats) return KVX_EINVAL;
     if (batch == 0 || total_tokens == 0) return KVX_OK;
     if (!q || !out) return KVX_EINVAL;
