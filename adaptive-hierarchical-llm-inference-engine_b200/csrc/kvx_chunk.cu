@@ -866,36 +866,46 @@ template <bool kSplit> struct FewShared {
     float row_sum[kFewRows], row_unscale[kFewRows], m[kFewWarps][kFewRows], l[kFewWarps][kFewRows];
 };
 
-// The key tiles of the sequences of at most 16 rows, one (sequence, kv-head)
-// after the other, are dealt out to the CTAs in equal ranges, whatever the
-// lengths (which the host does not know).
+// The work of the sequences of at most 16 rows, one (sequence, kv-head) pair
+// after the other, is dealt out to the CTAs in equal ranges, whatever the
+// lengths (which the host does not know).  It is counted in units of 4 pages,
+// one for each warp of a CTA.  A pair is kFewStart empty units, then its
+// own: what the start and end of a pair cost a CTA, so that one whose range
+// holds two ends has less to read.
+constexpr int kFewUnit = kFewWarps * kPageTokens, kFewStart = 4;
 struct FewWork {
-    int tiles;  // of all
-    int ctas;   // that have a range (at least kFewTiles tiles each, where there are so many)
+    int units;  // of all
+    int ctas;   // that have a range (longer than kFewStart, where there are so many)
 };
-constexpr int kFewTiles = 2;
 
-__device__ __forceinline__ int few_tiles(const ChunkParams &p, int s) {  // of one kv-head; one even where nothing is seen
+__device__ __forceinline__ int few_units(int keys) { return max(1, (keys + kFewUnit - 1) / kFewUnit); }  // one even where nothing is seen
+__device__ __forceinline__ int few_pair(const ChunkParams &p, int s) {  // units of a pair of the sequence, empty ones included
     const int rows = sequence_tokens(p, s) * p.group;
-    return rows > 0 && rows <= p.few_rows ? max(1, row_tile(p, s, 0, kFewRows, 1).tiles) : 0;
+    return rows > 0 && rows <= p.few_rows ? kFewStart + few_units(row_tile(p, s, 0, kFewRows, 1).keys) : 0;
 }
-__device__ __forceinline__ int few_used(const ChunkParams &p, int tiles) { return max(1, min(p.few_ctas, tiles / kFewTiles)); }
-// By a whole warp: the work, and the tiles before sequence `seq`.
+__device__ __forceinline__ int few_used(const ChunkParams &p, int units) { return max(1, min(p.few_ctas, units / (kFewStart + 1))); }
+// By a whole warp: the work, and the units before sequence `seq`.
 __device__ __forceinline__ FewWork few_work(const ChunkParams &p, int seq, int *before) {
     int all = 0, first = 0;
     for (int s = threadIdx.x & 31; s < p.batch; s += 32) {
-        const int t = few_tiles(p, s) * p.hkv;
+        const int t = few_pair(p, s) * p.hkv;
         all += t;
         if (s < seq) first += t;
     }
     *before = __reduce_add_sync(0xffffffffu, first);
     FewWork w;
-    w.tiles = __reduce_add_sync(0xffffffffu, all);
-    w.ctas = few_used(p, w.tiles);
+    w.units = __reduce_add_sync(0xffffffffu, all);
+    w.ctas = few_used(p, w.units);
     return w;
 }
-__device__ __forceinline__ int few_begin(const FewWork &w, int cta) { return (int)((long long)w.tiles * cta / w.ctas); }
-__device__ __forceinline__ int few_owner(const FewWork &w, int tile) { return (int)((((long long)tile + 1) * w.ctas - 1) / w.tiles); }
+// Ranges of units / ctas units, the first units % ctas of them one longer.
+__device__ __forceinline__ int few_begin(const FewWork &w, int cta) {
+    return cta * (w.units / w.ctas) + min(cta, w.units % w.ctas);
+}
+__device__ __forceinline__ int few_owner(const FewWork &w, int unit) {
+    const int each = w.units / w.ctas, longer = w.units % w.ctas;
+    return unit < longer * (each + 1) ? unit / (each + 1) : (unit - longer) / each;
+}
 
 // Sequences of at most 16 rows: bound by the codes' bytes.  A CTA's 4 warps
 // take the pages of its range in turn.  The codes go from memory to the operands of mma.sync (m16n8k16) in registers:
@@ -917,20 +927,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
     FewShared<kSplit> &sh = *reinterpret_cast<FewShared<kSplit> *>(few_smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3, cta = blockIdx.x;
     grid_dependents_launch();
-    // this CTA's tiles, and the sequence that the first belongs to
-    int w0 = 0, w1 = 0, seq = 0, before = 0;  // before: tiles of earlier sequences
+    // this CTA's units, and the sequence that the first belongs to
+    int w0 = 0, w1 = 0, seq = 0, before = 0;  // before: units of earlier sequences
     {
-        const int t = lane < p.batch ? few_tiles(p, lane) * p.hkv : 0;  // the first 32 sequences, looked at once
+        const int t = lane < p.batch ? few_pair(p, lane) * p.hkv : 0;  // the first 32 sequences, looked at once
         int all = t;
-        for (int i = 32 + lane; i < p.batch; i += 32) all += few_tiles(p, i) * p.hkv;
+        for (int i = 32 + lane; i < p.batch; i += 32) all += few_pair(p, i) * p.hkv;
         FewWork work_of;
-        work_of.tiles = __reduce_add_sync(0xffffffffu, all);
-        work_of.ctas = few_used(p, work_of.tiles);
+        work_of.units = __reduce_add_sync(0xffffffffu, all);
+        work_of.ctas = few_used(p, work_of.units);
         if (cta < work_of.ctas) {
             w0 = few_begin(work_of, cta);
             w1 = few_begin(work_of, cta + 1);
             for (int s0 = 0;; s0 += 32) {
-                const int mine = s0 == 0 ? t : (s0 + lane < p.batch ? few_tiles(p, s0 + lane) * p.hkv : 0);
+                const int mine = s0 == 0 ? t : (s0 + lane < p.batch ? few_pair(p, s0 + lane) * p.hkv : 0);
                 int x = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -948,24 +958,28 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
             }
         }
     }
+    bool later = false;  // not this CTA's first pair
 #pragma unroll 1
     for (int w = w0; w < w1;) {
         RowTile rt = row_tile(p, seq, 0, kFewRows, 1);
-        const int n_rows = rt.n * p.group, seq_tiles = n_rows > 0 && n_rows <= p.few_rows ? max(1, rt.tiles) : 0;
-        if (w >= before + seq_tiles * p.hkv) {
-            before += seq_tiles * p.hkv;
+        const int n_rows = rt.n * p.group, units = n_rows > 0 && n_rows <= p.few_rows ? few_units(rt.keys) : 0;
+        const int pair = units ? kFewStart + units : 0;
+        if (w >= before + pair * p.hkv) {
+            before += pair * p.hkv;
             ++seq;
             continue;
         }
-        const int kvh = (w - before) / seq_tiles, tile0 = (w - before) % seq_tiles;
-        const int piece = min(seq_tiles - tile0, w1 - w);  // tiles of it in this range
-        const bool whole = piece == seq_tiles, first_piece = w == w0;
-        w += piece;
-        if (threadIdx.x == 0 && tile0 == 0 && p.error_flag) {
+        const int kvh = (w - before) / pair, at = (w - before) % pair, unit0 = max(at - kFewStart, 0);
+        const int piece = min(pair - at, w1 - w) - max(kFewStart - at, 0);  // units of its own in this range
+        w += min(pair - at, w1 - w);
+        if (piece <= 0) continue;  // the range ends before them
+        const bool whole = piece == units, second = later;
+        later = true;
+        if (threadIdx.x == 0 && unit0 == 0 && p.error_flag) {
             if (rt.pos < 0) atomicOr(p.error_flag, 2);
             if ((long long)rt.pos + rt.n > (long long)p.max_pages * kPageTokens) atomicOr(p.error_flag, 4);
         }
-        const int page0 = tile0 * kTilePages, page1 = min(page0 + piece * kTilePages, (rt.keys + kPageTokens - 1) / kPageTokens);
+        const int page0 = unit0 * kFewWarps, page1 = min(page0 + piece * kFewWarps, (rt.keys + kPageTokens - 1) / kPageTokens);
         const int32_t *table = p.block_table + (size_t)seq * p.max_pages;
         auto page_of = [&](int lp) { return lp < page1 ? table[lp] : -1; };
         const int key_a = 4 * (g >> 1) + (g & 1);  // key of this lane's column of Q K^T (+ 2 for the second n-tile)
@@ -974,6 +988,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
         FewPage *page = sh.of[warp].page;
         int ids = page_of(first + lane * kFewWarps);
         uint32_t here = 0;  // bit i % 32: page i has an id that is one
+        // q is asked for before the pages, and used once they are under way
+        auto row_at = [&](int row) { return (rt.begin + row / p.group) * p.hq + kvh * p.group + row % p.group; };
+        float q_raw[kFewRows / kFewWarps][4] = {};
+#pragma unroll
+        for (int j = 0; j < kFewRows / kFewWarps; ++j) {
+            const int row = warp + kFewWarps * j;
+            if (row < n_rows) load_q4<T>(static_cast<const T *>(p.q) + (size_t)row_at(row) * kHeadDim + 4 * lane, q_raw[j]);
+        }
         auto fetch = [&](int i, int stage) {
             if (i < count) {
                 if (i && !(i & 31)) ids = page_of(first + (i + lane) * kFewWarps);
@@ -997,60 +1019,45 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
 #pragma unroll
         for (int i = 0; i < kFewStages; ++i) fetch(i, i);
 
-        // where each row of q and out lies, and up to which key it sees
-        if (threadIdx.x < kFewRows) {
-            const int row = min((int)threadIdx.x, n_rows - 1);  // rows that are none see what the last one sees
-            sh.row_at[threadIdx.x] = (rt.begin + row / p.group) * p.hq + kvh * p.group + row % p.group;
-            sh.row_limit[threadIdx.x] = row_keys(p, rt, row);
-        }
-        __syncthreads();
-        // q: row sums and (fp32) scales by warps, then the A fragments
-        const T *q = static_cast<const T *>(p.q);
-        for (int row = warp; row < n_rows; row += kFewWarps) {
-            float f[4], big = 0.f;
-            load_q4<T>(q + (size_t)sh.row_at[row] * kHeadDim + 4 * lane, f);
-            float sum = f[0] + f[1] + f[2] + f[3];
+        // q: a warp's rows, 4 dims a lane, to the A fragments: the dims of a lane
+        // are those of one lane of one k-step
 #pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if constexpr (kSplit) {
+        for (int j = 0; j < kFewRows / kFewWarps; ++j) {
+            const int row = warp + kFewWarps * j;
+            float up = 1.f, *f = q_raw[j];
+            if (row < n_rows) {
+                float sum = f[0] + f[1] + f[2] + f[3];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) big = fmaxf(big, fabsf(f[k]));
+                for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                float unscale = 1.f;
+                if constexpr (kSplit) {
+                    float big = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
 #pragma unroll
-                for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                    for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                    if (big > 0.f && big < CUDART_INF_F) unscale = pow2i(exponent_above(big) - 13);
+                    up = 1.f / unscale;  // a power of two
+                }
+                if (lane == 0) {
+                    sh.row_sum[row] = sum;
+                    sh.row_unscale[row] = unscale;
+                }
             }
             if (lane == 0) {
-                sh.row_sum[row] = sum;
-                sh.row_unscale[row] = kSplit && big > 0.f && big < CUDART_INF_F ? pow2i(exponent_above(big) - 13) : 1.f;
+                const int r = min(row, n_rows - 1);  // rows that are none see what the last one sees
+                sh.row_at[row] = row_at(r);
+                sh.row_limit[row] = row_keys(p, rt, r);
             }
-        }
-        if constexpr (kSplit) __syncthreads();
+            const int step = (lane >> 4) * 4 + (lane & 3), to = (row & 7) * 4 + ((lane >> 2) & 3), half = row >> 3;
 #pragma unroll
-        for (int s0 = 0; s0 < 8; s0 += kFewWarps) {
-            const int s = s0 + warp, d = (s >> 2) * 64 + 16 * q4 + 4 * (s & 3);  // this lane's four dims of k-step s
-            uint32_t hi[2][2], lo[2][2];                                         // [row g, g + 8][dims d, d + 2]
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int row = g + 8 * r;
-                float f[4] = {0.f, 0.f, 0.f, 0.f};
-                if (row < n_rows) {
-                    load_q4<T>(q + (size_t)sh.row_at[row] * kHeadDim + d, f);
-                    if constexpr (kSplit) {
-                        const float up = 1.f / sh.row_unscale[row];  // a power of two
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) f[k] *= up;
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    hi[r][k] = pack_half(f[2 * k], f[2 * k + 1]);
-                    if constexpr (kSplit) {
-                        const float2 h = h2_to_f2(hi[r][k]);
-                        lo[r][k] = pack_half(f[2 * k] - h.x, f[2 * k + 1] - h.y);
-                    }
+            for (int k = 0; k < 2; ++k) {
+                const float x = f[2 * k] * up, y = f[2 * k + 1] * up;
+                const uint32_t hi = pack_half(x, y);
+                reinterpret_cast<uint32_t *>(&sh.q_frag[0][step][to])[2 * k + half] = hi;
+                if constexpr (kSplit) {
+                    const float2 h = h2_to_f2(hi);
+                    reinterpret_cast<uint32_t *>(&sh.q_frag[1][step][to])[2 * k + half] = pack_half(x - h.x, y - h.y);
                 }
             }
-            sh.q_frag[0][s][lane] = make_uint4(hi[0][0], hi[1][0], hi[0][1], hi[1][1]);
-            if constexpr (kSplit) sh.q_frag[1][s][lane] = make_uint4(lo[0][0], lo[1][0], lo[0][1], lo[1][1]);
         }
         __syncthreads();
 
@@ -1240,7 +1247,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
                 store_out4<T>(static_cast<T *>(p.out) + (size_t)sh.row_at[row] * kHeadDim + d, acc.x * inv, acc.y * inv, acc.z * inv,
                                acc.w * inv);
             } else {
-                const size_t at = ((size_t)2 * cta + !first_piece) * kFewRows + row;
+                const size_t at = ((size_t)2 * cta + second) * kFewRows + row;
                 *reinterpret_cast<float4 *>(p.few_o + at * kHeadDim + d) = acc;
                 if (d == 0) p.few_ml[at] = make_float2(M, L);
             }
@@ -1251,34 +1258,44 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
 }
 
 // out[row] of the rows whose keys were split: one warp per row, 4 dims a lane.
+// The first few_ctas CTAs take 8 of the up to 16 rows of a pair that was
+// attend_rows_kernel's, the others 8 of all rows.
 template <typename T>
-__global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_constant__ ChunkParams p, int tile_rows) {
-    const size_t row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, t = (int)(row / p.hq), h = (int)(row % p.hq);
-    int s = -1;
-    for (int s0 = 0; s0 < p.batch && s < 0 && t < p.total; s0 += 32) {
-        const int i = s0 + lane;
-        const uint32_t hit = __ballot_sync(0xffffffffu, i < p.batch && p.q_start[i] >= 0 && p.q_start[i] <= t && t < p.q_start[i + 1]);
-        if (hit) s = s0 + __ffs(hit) - 1;
-    }
-    bool few = false, late = false;  // late: the first part lies in its CTA's second place
+__global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_constant__ ChunkParams p, int tile_rows, int few_ctas) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool few = (int)blockIdx.x < few_ctas;
+    bool late = false;  // the first part lies in its CTA's second place
     int splits = 1;
-    size_t at = row, step = (size_t)p.total * p.hq;
-    if (s >= 0) {
-        const int r = (t - p.q_start[s]) * p.group + h % p.group;  // among the rows of its (sequence, kv-head)
-        few = sequence_tokens(p, s) * p.group <= p.few_rows;
-        if (few) {
-            int before;
-            const FewWork work_of = few_work(p, s, &before);
-            const int tiles = few_tiles(p, s);
-            before += h / p.group * tiles;
-            const int first = few_owner(work_of, before);
-            splits = few_owner(work_of, before + tiles - 1) - first + 1;
+    size_t row = 0, at = 0, step = 0;  // row of out; first part; between the parts
+    if (few) {
+        const int pair = blockIdx.x >> 1, r = (blockIdx.x & 1) * 8 + warp, s = pair / p.hkv, kvh = pair % p.hkv;
+        const int rows = sequence_tokens(p, s) * p.group;
+        int before;
+        const FewWork work_of = few_work(p, s, &before);
+        if (r < rows && rows <= p.few_rows) {
+            const int units = few_pair(p, s);
+            before += kvh * units;
+            const int first = few_owner(work_of, before + kFewStart);
+            splits = few_owner(work_of, before + units - 1) - first + 1;
             late = few_begin(work_of, first) < before;
             at = (size_t)first * 2 * kFewRows + r;
             step = 2 * kFewRows;
-        } else {
+            row = (size_t)(p.q_start[s] + r / p.group) * p.hq + kvh * p.group + r % p.group;
+        }
+    } else {
+        row = (size_t)(blockIdx.x - few_ctas) * 8 + warp;
+        const int t = (int)(row / p.hq), h = (int)(row % p.hq);
+        int s = -1;
+        for (int s0 = 0; s0 < p.batch && s < 0 && t < p.total; s0 += 32) {
+            const int i = s0 + lane;
+            const uint32_t hit = __ballot_sync(0xffffffffu, i < p.batch && p.q_start[i] >= 0 && p.q_start[i] <= t && t < p.q_start[i + 1]);
+            if (hit) s = s0 + __ffs(hit) - 1;
+        }
+        if (s >= 0 && sequence_tokens(p, s) * p.group > p.few_rows) {
+            const int r = (t - p.q_start[s]) * p.group + h % p.group;  // among the rows of its pair
             splits = row_tile(p, s, r / tile_rows, tile_rows, p.chunk).splits;
+            at = row;
+            step = (size_t)p.total * p.hq;
         }
     }
     grid_dependency_wait();  // until here only the call's own arguments are read; every thread waits, so this grid ends last
@@ -1292,7 +1309,7 @@ __global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_consta
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     float L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
     for (int c = 0; c < splits; ++c) {
         const float2 ml = part_ml[part(c)];
         const float4 v = reinterpret_cast<const float4 *>(part_o + part(c) * kHeadDim)[lane];
@@ -1382,7 +1399,9 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
         }
     }
     if (rc != KVX_OK || (splits == 1 && !few)) return rc;
-    return launch_beside(attend_combine_kernel<T>, dim3((unsigned)((all + 7) / 8)), 256, 0, st, p, tile_rows);
+    const int few_grid = few ? p.batch * p.hkv * (kFewRows / 8) : 0;
+    const unsigned grid = few_grid + (splits > 1 ? (unsigned)((all + 7) / 8) : 0);
+    return launch_beside(attend_combine_kernel<T>, dim3(grid), 256, 0, st, p, tile_rows, few_grid);
 }
 
 }  // namespace
@@ -1417,8 +1436,8 @@ extern "C" KVX_API int kvx_attend_chunk(const kvx_paged *kv, const int32_t *bloc
     if (kv->dtype != KVX_I8 || kv->head_dim != kHeadDim || kv->page_tokens != kPageTokens) return KVX_EUNSUPPORTED;
     if (kv->num_kv_heads > 65535 || max_pages > (0x7fffffff - kTileKeys) / kPageTokens ||
         (long long)total_tokens * num_q_heads > 0x3fffffff ||
-        (long long)batch * kv->num_kv_heads * key_tiles(max_pages) > 0x7fffffff)
-        return KVX_EUNSUPPORTED;  // grid, key, row and tile counts fit an int
+        (long long)batch * kv->num_kv_heads * (max_pages / kFewWarps + kFewStart + 1) > 0x7fffffff)
+        return KVX_EUNSUPPORTED;  // grid, key, row and unit counts fit an int
     if (!kv->stats) return KVX_EINVAL;
     if (batch == 0 || total_tokens == 0) return KVX_OK;
     if (!q || !out) return KVX_EINVAL;
