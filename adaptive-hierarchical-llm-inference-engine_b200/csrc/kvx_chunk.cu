@@ -80,7 +80,7 @@ struct ChunkParams {
     int32_t *error_flag;
     int batch, total, hq, hkv, group, max_pages, num_pages, causal;
     int chunk;             // attend_chunk_kernel: key tiles of a split
-    int few_ctas;          // attend_rows_kernel: CTAs
+    int few_ctas, few_keys;  // attend_rows_kernel: CTAs; log2 of a unit's keys
     int few_rows;          // sequences of at most so many rows are attend_rows_kernel's (0: none)
     float scale_log2;
 };
@@ -820,7 +820,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
 
 // ---- at most 16 rows
 
-constexpr int kFewWarps = 4, kFewRows = 16;
+constexpr int kFewRows = 16;
+// Warps of a CTA and CTAs on an SM: as many warps as the registers hold.
+template <bool kSplit> constexpr int kFewWarps = kSplit ? 4 : 8;
+template <bool kSplit> constexpr int kFewCtas = kSplit ? 3 : 2;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -860,28 +863,30 @@ template <bool kSplit> struct FewShared {
     union {
         FewPage page[kFewStages];
         float o[kFewRows][kHeadDim + 4];  // once the warp has no more pages
-    } of[kFewWarps];
+    } of[kFewWarps<kSplit>];
     uint4 q_frag[kSplit ? 2 : 1][8][32];
     int row_at[kFewRows], row_limit[kFewRows];
-    float row_sum[kFewRows], row_unscale[kFewRows], m[kFewWarps][kFewRows], l[kFewWarps][kFewRows];
+    float row_sum[kFewRows], row_unscale[kFewRows], m[kFewWarps<kSplit>][kFewRows], l[kFewWarps<kSplit>][kFewRows];
 };
 
 // The work of the sequences of at most 16 rows, one (sequence, kv-head) pair
 // after the other, is dealt out to the CTAs in equal ranges, whatever the
-// lengths (which the host does not know).  It is counted in units of 4 pages,
-// one for each warp of a CTA.  A pair is kFewStart empty units, then its
+// lengths (which the host does not know).  It is counted in units of a page
+// for each warp of a CTA (p.few_keys keys).  A pair is kFewStart empty units, then its
 // own: what the start and end of a pair cost a CTA, so that one whose range
 // holds two ends has less to read.
-constexpr int kFewUnit = kFewWarps * kPageTokens, kFewStart = 4;
+constexpr int kFewStart = 4;
 struct FewWork {
     int units;  // of all
     int ctas;   // that have a range (longer than kFewStart, where there are so many)
 };
 
-__device__ __forceinline__ int few_units(int keys) { return max(1, (keys + kFewUnit - 1) / kFewUnit); }  // one even where nothing is seen
+__device__ __forceinline__ int few_units(const ChunkParams &p, int keys) {  // one even where nothing is seen
+    return max(1, (keys + (1 << p.few_keys) - 1) >> p.few_keys);
+}
 __device__ __forceinline__ int few_pair(const ChunkParams &p, int s) {  // units of a pair of the sequence, empty ones included
     const int rows = sequence_tokens(p, s) * p.group;
-    return rows > 0 && rows <= p.few_rows ? kFewStart + few_units(row_tile(p, s, 0, kFewRows, 1).keys) : 0;
+    return rows > 0 && rows <= p.few_rows ? kFewStart + few_units(p, row_tile(p, s, 0, kFewRows, 1).keys) : 0;
 }
 __device__ __forceinline__ int few_used(const ChunkParams &p, int units) { return max(1, min(p.few_ctas, units / (kFewStart + 1))); }
 // By a whole warp: the work, and the units before sequence `seq`.
@@ -922,7 +927,8 @@ __device__ __forceinline__ int few_owner(const FewWork &w, int unit) {
 // ends inside a (sequence, kv-head) the rows' partial results go to the
 // workspace; a CTA has two such ends at most.
 template <typename T, bool kSplit>
-__global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_kernel(const __grid_constant__ ChunkParams p) {
+__global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) attend_rows_kernel(const __grid_constant__ ChunkParams p) {
+    constexpr int kWarps = kFewWarps<kSplit>;
     extern __shared__ __align__(16) uint8_t few_smem[];
     FewShared<kSplit> &sh = *reinterpret_cast<FewShared<kSplit> *>(few_smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3, cta = blockIdx.x;
@@ -962,7 +968,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
 #pragma unroll 1
     for (int w = w0; w < w1;) {
         RowTile rt = row_tile(p, seq, 0, kFewRows, 1);
-        const int n_rows = rt.n * p.group, units = n_rows > 0 && n_rows <= p.few_rows ? few_units(rt.keys) : 0;
+        const int n_rows = rt.n * p.group, units = n_rows > 0 && n_rows <= p.few_rows ? few_units(p, rt.keys) : 0;
         const int pair = units ? kFewStart + units : 0;
         if (w >= before + pair * p.hkv) {
             before += pair * p.hkv;
@@ -979,26 +985,26 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
             if (rt.pos < 0) atomicOr(p.error_flag, 2);
             if ((long long)rt.pos + rt.n > (long long)p.max_pages * kPageTokens) atomicOr(p.error_flag, 4);
         }
-        const int page0 = unit0 * kFewWarps, page1 = min(page0 + piece * kFewWarps, (rt.keys + kPageTokens - 1) / kPageTokens);
+        const int page0 = unit0 * kWarps, page1 = min(page0 + piece * kWarps, (rt.keys + kPageTokens - 1) / kPageTokens);
         const int32_t *table = p.block_table + (size_t)seq * p.max_pages;
         auto page_of = [&](int lp) { return lp < page1 ? table[lp] : -1; };
         const int key_a = 4 * (g >> 1) + (g & 1);  // key of this lane's column of Q K^T (+ 2 for the second n-tile)
         // this warp's pages page0 + warp, + 4, ...: contents three ahead, ids of 32 at once
-        const int first = page0 + warp, count = first < page1 ? (page1 - first + kFewWarps - 1) / kFewWarps : 0;
+        const int first = page0 + warp, count = first < page1 ? (page1 - first + kWarps - 1) / kWarps : 0;
         FewPage *page = sh.of[warp].page;
-        int ids = page_of(first + lane * kFewWarps);
+        int ids = page_of(first + lane * kWarps);
         uint32_t here = 0;  // bit i % 32: page i has an id that is one
         // q is asked for before the pages, and used once they are under way
         auto row_at = [&](int row) { return (rt.begin + row / p.group) * p.hq + kvh * p.group + row % p.group; };
-        float q_raw[kFewRows / kFewWarps][4] = {};
+        float q_raw[kFewRows / kWarps][4] = {};
 #pragma unroll
-        for (int j = 0; j < kFewRows / kFewWarps; ++j) {
-            const int row = warp + kFewWarps * j;
+        for (int j = 0; j < kFewRows / kWarps; ++j) {
+            const int row = warp + kWarps * j;
             if (row < n_rows) load_q4<T>(static_cast<const T *>(p.q) + (size_t)row_at(row) * kHeadDim + 4 * lane, q_raw[j]);
         }
         auto fetch = [&](int i, int stage) {
             if (i < count) {
-                if (i && !(i & 31)) ids = page_of(first + (i + lane) * kFewWarps);
+                if (i && !(i & 31)) ids = page_of(first + (i + lane) * kWarps);
                 const int phys = __shfl_sync(0xffffffffu, ids, i & 31);
                 const bool known = phys >= 0 && phys < p.num_pages;
                 here = (here & ~(1u << (i & 31))) | (uint32_t)known << (i & 31);
@@ -1022,8 +1028,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
         // q: a warp's rows, 4 dims a lane, to the A fragments: the dims of a lane
         // are those of one lane of one k-step
 #pragma unroll
-        for (int j = 0; j < kFewRows / kFewWarps; ++j) {
-            const int row = warp + kFewWarps * j;
+        for (int j = 0; j < kFewRows / kWarps; ++j) {
+            const int row = warp + kWarps * j;
             float up = 1.f, *f = q_raw[j];
             if (row < n_rows) {
                 float sum = f[0] + f[1] + f[2] + f[3];
@@ -1119,7 +1125,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[j][e] += c2[j][e];
             // scores (log2): keys key0 + 4 q + 2 j + e of rows g (c[j][e]) and g + 8 (c[j][2 + e])
-            const int key0 = (first + i * kFewWarps) * kPageTokens;
+            const int key0 = (first + i * kWarps) * kPageTokens;
             const bool masked = least < key0 + kPageTokens;
             const float k_mid = fmaf(128.f, ks.x, ks.y) * p.scale_log2, v_mid = fmaf(128.f, vs.x, vs.y);
             float scale[2], top[2];
@@ -1228,15 +1234,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, kSplit ? 3 : 4) attend_rows_ke
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < n_rows * (kHeadDim / 4); i += kFewWarps * 32) {
+        for (int i = threadIdx.x; i < n_rows * (kHeadDim / 4); i += kWarps * 32) {
             const int row = i / (kHeadDim / 4), d = 4 * (i % (kHeadDim / 4));
             float M = sh.m[0][row];
 #pragma unroll
-            for (int w = 1; w < kFewWarps; ++w) M = fmaxf(M, sh.m[w][row]);
+            for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sh.m[w][row]);
             float L = 0.f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kFewWarps; ++w) {
+            for (int w = 0; w < kWarps; ++w) {
                 const float f = sh.m[w][row] == -CUDART_INF_F && sh.l[w][row] == 0.f ? 0.f : ex2(sh.m[w][row] - M);
                 const float4 v = *reinterpret_cast<const float4 *>(&sh.of[w].o[row][d]);
                 L = fmaf(f, sh.l[w][row], L);
@@ -1331,8 +1337,7 @@ long long most_splits(long long ctas, long long slots, int max_pages) {
     return std::min<long long>(std::max<long long>(1, slots / ctas), std::max(1, key_tiles(max_pages) / kMinChunk));
 }
 long long chunk_slots() { return 2LL * sm_count(); }  // about two CTAs an SM (one is resident)
-// CTAs of attend_rows_kernel: what is resident, by shared memory (fp32) and registers
-int few_ctas(bool fp32) { return (fp32 ? 3 : 4) * sm_count(); }
+int few_ctas(bool fp32) { return (fp32 ? kFewCtas<true> : kFewCtas<false>) * sm_count(); }
 
 // A launch that may start while the one before it in the stream runs.
 template <typename... Args>
@@ -1379,6 +1384,8 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     const int splits = (tiles + p.chunk - 1) / p.chunk;
     const size_t all = (size_t)p.total * p.hq, few_all = (size_t)few_ctas(kSplit) * 2 * kFewRows;
     p.few_ctas = few_ctas(kSplit);
+    p.few_keys = kFewWarps<kSplit> == 8 ? 7 : 6;
+    static_assert(kFewWarps<kSplit> == 8 || kFewWarps<kSplit> == 4);
     p.few_o = static_cast<float *>(workspace);
     p.few_ml = reinterpret_cast<float2 *>(p.few_o + few_all * kHeadDim);
     p.part_o = p.few_o + (few ? few_all * (kHeadDim + 2) : 0);
@@ -1392,9 +1399,9 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     if (few && rc == KVX_OK) {
         const dim3 grid((unsigned)p.few_ctas);
         if (chunk) {
-            rc = launch_beside(few_kern, grid, kFewWarps * 32, few_smem, st, p);
+            rc = launch_beside(few_kern, grid, kFewWarps<kSplit> * 32, few_smem, st, p);
         } else {
-            few_kern<<<grid, kFewWarps * 32, few_smem, st>>>(p);
+            few_kern<<<grid, kFewWarps<kSplit> * 32, few_smem, st>>>(p);
             rc = launch_status();
         }
     }
@@ -1418,7 +1425,7 @@ extern "C" KVX_API size_t kvx_attend_chunk_workspace_bytes(int32_t batch, int32_
         max_pages <= 0)
         return 0;
     const long long splits = most_splits(num_kv_heads, chunk_slots(), max_pages);
-    long long rows = 2LL * few_ctas(false) * kFewRows;
+    long long rows = 2LL * few_ctas(true) * kFewRows;
     if (splits > 1) rows += std::min(splits * total_tokens * num_q_heads, chunk_slots() * 256);
     return (size_t)rows * (kHeadDim + 2) * sizeof(float) + 16;
 }
@@ -1436,7 +1443,7 @@ extern "C" KVX_API int kvx_attend_chunk(const kvx_paged *kv, const int32_t *bloc
     if (kv->dtype != KVX_I8 || kv->head_dim != kHeadDim || kv->page_tokens != kPageTokens) return KVX_EUNSUPPORTED;
     if (kv->num_kv_heads > 65535 || max_pages > (0x7fffffff - kTileKeys) / kPageTokens ||
         (long long)total_tokens * num_q_heads > 0x3fffffff ||
-        (long long)batch * kv->num_kv_heads * (max_pages / kFewWarps + kFewStart + 1) > 0x7fffffff)
+        (long long)batch * kv->num_kv_heads * (max_pages / kFewWarps<true> + kFewStart + 1) > 0x7fffffff)
         return KVX_EUNSUPPORTED;  // grid, key, row and unit counts fit an int
     if (!kv->stats) return KVX_EINVAL;
     if (batch == 0 || total_tokens == 0) return KVX_OK;
