@@ -851,7 +851,7 @@ template <int kLeft> __device__ __forceinline__ void copy_wait() { asm volatile(
 // chunk c of row r lies at few_chunk(r, c), so that neither reader (K: the
 // same chunk of rows r and r + 1; V: rows r, r + 4, r + 8, r + 12) meets
 // itself in a bank.
-constexpr int kFewStages = 3;
+constexpr int kFewStages = 2;
 struct FewPage {
     uint8_t k[kBlockBytes], v[kBlockBytes];
     float4 ks, vs;
@@ -922,8 +922,7 @@ __device__ __forceinline__ int few_owner(const FewWork &w, int unit) {
 //  * V: a lane reads dims 16 g .. + 15 of keys 4 q .. 4 q + 3, transposes them
 //    4 x 4 bytes at a time, and has its B fragments of the 16 n-tiles: n-tile
 //    t holds dims 16 n + t, so the lane ends with dims 32 q .. 32 q + 31 of O.
-// A page is one k-step of P V and has one V scale, so the scale is applied to
-// its product in fp32.  Where a range
+// A page is one k-step of P V and has one V scale, which P takes.  Where a range
 // ends inside a (sequence, kv-head) the rows' partial results go to the
 // workspace; a CTA has two such ends at most.
 template <typename T, bool kSplit>
@@ -1067,9 +1066,12 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
         }
         __syncthreads();
 
-        uint64_t o[16][2];  // n-tile t: two dims of row g, of row g + 8
+        float o[16][4];  // n-tile t: two dims of row g, of row g + 8; times 2^-v_exp
 #pragma unroll
-        for (int t = 0; t < 16; ++t) o[t][0] = o[t][1] = 0;
+        for (int t = 0; t < 16; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[t][k] = 0.f;
+        int v_exp = -100, v_top = -100;
         // rows g and g + 8
         int limit[2];
         float m[2], l[2], z[2], q_sum[2], unscale[2];
@@ -1128,7 +1130,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
             const int key0 = (first + i * kWarps) * kPageTokens;
             const bool masked = least < key0 + kPageTokens;
             const float k_mid = fmaf(128.f, ks.x, ks.y) * p.scale_log2, v_mid = fmaf(128.f, vs.x, vs.y);
-            float scale[2], top[2];
+            float top[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const float a = ks.x * p.scale_log2 * unscale[r], b = k_mid * q_sum[r];
@@ -1142,10 +1144,17 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
                         if (masked && key0 + 4 * q4 + 2 * j + e >= limit[r]) x = -CUDART_INF_F;
                         top[r] = fmaxf(top[r], x);
                     }
-                // a row that sees nothing of the page takes nothing from it, whatever its statistics
-                scale[r] = masked && limit[r] <= key0 ? 0.f : vs.x;
             }
-            if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
+            // P V takes p times the page's scale: as fp16 that keeps its 11 bits
+            // while the scale is near 2^v_exp.  v_exp goes down no further than
+            // 60 below the largest so far, so that the sums stay finite.
+            const float v_abs = fabsf(vs.x);
+            const int e_v = v_abs > 0.f && v_abs < CUDART_INF_F ? max(min(exponent_above(v_abs), 126), v_top - 60) : v_exp;
+            const bool far = e_v > v_exp || e_v < v_exp - 4;
+            if (__any_sync(0xffffffffu, far || top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
+                const float to = v_exp - e_v < -126 ? 0.f : far ? pow2i(v_exp - e_v) : 1.f;
+                if (far) v_exp = e_v;
+                v_top = max(v_top, v_exp);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
@@ -1154,12 +1163,15 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
                     m[r] = mn;
                     l[r] *= f_;
                     z[r] *= f_;
-                    const uint64_t ff = pack2(f_, f_);
+                    const float f_o = f_ * to;
 #pragma unroll
-                    for (int t = 0; t < 16; ++t) o[t][r] = mul2(o[t][r], ff);
+                    for (int t = 0; t < 16; ++t) {
+                        o[t][2 * r] *= f_o;
+                        o[t][2 * r + 1] *= f_o;
+                    }
                 }
             }
-            const uint64_t ss0 = pack2(scale[0], scale[0]), ss1 = pack2(scale[1], scale[1]);
+            const float v_scale = vs.x * pow2i(-v_exp);
             uint4 ph, pl;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -1171,7 +1183,11 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
                     sum += e4[k];
                 }
                 l[r] += sum;
-                if (!masked || limit[r] > key0) z[r] = fmaf(sum, v_mid, z[r]);
+                // a row that sees nothing of the page takes nothing from it, whatever its statistics
+                const bool sees = !masked || limit[r] > key0;
+                if (sees) z[r] = fmaf(sum, v_mid, z[r]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e4[k] = sees ? e4[k] * v_scale : 0.f;
                 const uint32_t a = pack_half(e4[0], e4[1]), b = pack_half(e4[2], e4[3]);
                 (r ? ph.y : ph.x) = a;
                 (r ? ph.w : ph.z) = b;
@@ -1199,11 +1215,8 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint2 v = codes_to_half(col[i]);
-                    float t[4];
-                    mma_f16_zero(t, ph, v.x, v.y);
-                    if constexpr (kSplit) mma_f16(t, pl, v.x, v.y);
-                    o[4 * w + i][0] = fma2(ss0, pack2(t[0], t[1]), o[4 * w + i][0]);
-                    o[4 * w + i][1] = fma2(ss1, pack2(t[2], t[3]), o[4 * w + i][1]);
+                    mma_f16(o[4 * w + i], ph, v.x, v.y);
+                    if constexpr (kSplit) mma_f16(o[4 * w + i], pl, v.x, v.y);
                 }
             }
         }
@@ -1211,6 +1224,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
         __syncwarp();
 
         // ---- the quad's sums, then the warps
+        const float v_unit = pow2i(v_exp);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
 #pragma unroll
@@ -1225,12 +1239,12 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
             }
 #pragma unroll
             for (int t = 0; t < 16; t += 4) {
-                float2 x[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = unpack2(o[t + k][r]);
                 float *to = &sh.of[warp].o[row][32 * q4 + t];
-                *reinterpret_cast<float4 *>(to) = make_float4(x[0].x + z[r], x[1].x + z[r], x[2].x + z[r], x[3].x + z[r]);
-                *reinterpret_cast<float4 *>(to + 16) = make_float4(x[0].y + z[r], x[1].y + z[r], x[2].y + z[r], x[3].y + z[r]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<float4 *>(to + 16 * h) =
+                        make_float4(fmaf(o[t][2 * r + h], v_unit, z[r]), fmaf(o[t + 1][2 * r + h], v_unit, z[r]),
+                                    fmaf(o[t + 2][2 * r + h], v_unit, z[r]), fmaf(o[t + 3][2 * r + h], v_unit, z[r]));
             }
         }
         __syncthreads();
