@@ -61,9 +61,10 @@ struct TileStats {
     uint32_t known;           // bit i: page i is there
     uint32_t pad[2];
 };
+constexpr int kBarBytes = 288;
 // shared memory: Q0, Q1 (staging slots 2, 3 when unused), K x 2, V x 2, staging x 2, the rest
 constexpr int kAtK = 2 * kTileBytes, kAtV = kAtK + 2 * kTileBytes, kAtStage = kAtV + 2 * kTileBytes,
-              kAtMisc = kAtStage + 2 * kSlotBytes, kChunkSmem = 1024 + kAtMisc + 512 + kStatSlots * (int)sizeof(TileStats);
+              kAtMisc = kAtStage + 2 * kSlotBytes, kChunkSmem = 1024 + kAtMisc + kBarBytes + kStatSlots * (int)sizeof(TileStats) + 256 * 4;
 static_assert(kChunkSmem <= 227 * 1024, "chunk attention exceeds the shared memory of a CTA");
 constexpr float kLazy = 8.f;  // log2 of the growth of a row's maximum that is let pass
 
@@ -80,6 +81,7 @@ struct ChunkParams {
     int32_t *error_flag;
     int batch, total, hq, hkv, group, max_pages, num_pages, causal;
     int chunk;             // attend_chunk_kernel: key tiles of a split
+    int tile_rows;           // attend_chunk_kernel: rows of a CTA
     int few_ctas, few_keys;  // attend_rows_kernel: CTAs; log2 of a unit's keys
     int few_rows;          // sequences of at most so many rows are attend_rows_kernel's (0: none)
     float scale_log2;
@@ -91,7 +93,7 @@ struct ChunkBars {
     uint32_t known[4];  // staging slot: bit i, page i was loaded
     int seq, tile;
 };
-static_assert(sizeof(ChunkBars) <= 512, "");
+static_assert(sizeof(ChunkBars) <= kBarBytes);
 
 // Rows of one (sequence, row tile): what the kernel and the combine agree on.
 struct RowTile {
@@ -280,18 +282,6 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// The row's 16-byte chunk of 8 dims: as fp16, or fp16 high and low parts.
-template <typename T> __device__ __forceinline__ void load_q8(const T *row, int c, float *f);
-template <> __device__ __forceinline__ void load_q8<__half>(const __half *row, int c, float *f) {
-    const uint4 w = reinterpret_cast<const uint4 *>(row)[c];
-    const float2 a = h2_to_f2(w.x), b = h2_to_f2(w.y), d = h2_to_f2(w.z), e = h2_to_f2(w.w);
-    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y, f[4] = d.x, f[5] = d.y, f[6] = e.x, f[7] = e.y;
-}
-template <> __device__ __forceinline__ void load_q8<float>(const float *row, int c, float *f) {
-    const float4 a = reinterpret_cast<const float4 *>(row)[2 * c], b = reinterpret_cast<const float4 *>(row)[2 * c + 1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-}
-
 template <typename T> __device__ __forceinline__ void load_q4(const T *p, float *f);
 template <> __device__ __forceinline__ void load_q4<__half>(const __half *p, float *f) {
     const uint2 w = *reinterpret_cast<const uint2 *>(p);
@@ -314,24 +304,25 @@ template <> __device__ __forceinline__ void store_out4<__half>(__half *o, float 
 // kSplit (fp32 calls): q and P' as high + low parts.
 template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __grid_constant__ ChunkParams p) {
-    constexpr int kTileRows = kSplit ? 128 : 256;
+    const int tile_rows = p.tile_rows;
     extern __shared__ __align__(1024) uint8_t chunk_smem[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(chunk_smem) + 1023) & ~uintptr_t(1023));
     const uint32_t base = smem_addr(sm);
     ChunkBars *bars = reinterpret_cast<ChunkBars *>(sm + kAtMisc);
-    TileStats *tile_stats = reinterpret_cast<TileStats *>(sm + kAtMisc + 512);
+    TileStats *tile_stats = reinterpret_cast<TileStats *>(sm + kAtMisc + kBarBytes);
+    float *row_sum = reinterpret_cast<float *>(tile_stats + kStatSlots), *row_unscale = row_sum + 128;  // [256]; fp32 calls: [128] each
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kvh = blockIdx.y, split = blockIdx.z;
+    const int kvh = blockIdx.x % p.hkv, split = blockIdx.y;
 
     grid_dependents_launch();  // the combine may place its CTAs; it waits for this grid
     // ---- which rows: the last tiles first (causal: they have the most keys)
     if (warp == 0) {
-        const int want = gridDim.x - 1 - blockIdx.x;
+        const int want = (gridDim.x - 1 - blockIdx.x) / p.hkv;
         int before = 0, seq = -1, tile = 0;
         for (int s0 = 0; s0 < p.batch && seq < 0; s0 += 32) {
             const int s = s0 + lane;
             const int rows = s < p.batch ? sequence_tokens(p, s) * p.group : 0;
-            const int mine = rows > p.few_rows ? (rows + kTileRows - 1) / kTileRows : 0;
+            const int mine = rows > p.few_rows ? (rows + tile_rows - 1) / tile_rows : 0;
             int x = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -355,9 +346,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     __syncthreads();
     const int seq = bars->seq, tile = bars->tile;
     if (seq < 0) return;  // the grid is an upper bound
-    const RowTile rt = row_tile(p, seq, tile, kTileRows, p.chunk);
+    const RowTile rt = row_tile(p, seq, tile, tile_rows, p.chunk);
     if (split >= rt.splits) return;
-    const int row0 = tile * kTileRows;
+    const int row0 = tile * tile_rows;
     if (threadIdx.x == 0 && split == 0 && p.error_flag) {
         if (rt.pos < 0) atomicOr(p.error_flag, 2);
         if ((long long)rt.pos + rt.n > (long long)p.max_pages * kPageTokens) atomicOr(p.error_flag, 4);
@@ -570,51 +561,77 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         const uint32_t t_s = tmem + j * 128 + lanes, t_o = tmem + 256 + j * 128 + lanes;
         const int my_row = turns ? r : j * 128 + r;
         const bool valid = my_row < rt.rows;
-        float q_sum = 0.f, unscale = 1.f;
+        // Q: 16 loads of 512 contiguous bytes a warp, all in flight at once
+        // (fp16: 2 rows each, fp32: 1); rows that are none are zero
         {
-            const T *row = static_cast<const T *>(p.q) + (valid ? row_index(my_row) : 0) * kHeadDim;
-            const bool writes = !turns || j == 0;
-            const uint32_t dst = base + (turns ? 0 : j * kTileBytes);
-            float up = 1.f;
-            if constexpr (kSplit) {
-                float big = 0.f;
-#pragma unroll 4
-                for (int c = 0; c < 16; ++c) {
-                    float f[8];
-                    if (valid) {
-                        load_q8<T>(row, c, f);
+            const int rows_all = turns ? 128 : 256;
+            constexpr int kUnits = 16, kPerUnit = kSplit ? 1 : 2;
+            uint4 x[kUnits];
+            const int first = warp * kUnits * kPerUnit, mine = first + (lane & (kUnits * kPerUnit - 1));
+            const int at = mine < rt.rows ? (int)row_index(mine) : 0;  // total * hq fits an int
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) big = fmaxf(big, fabsf(f[k]));
-                    }
-                }
-                if (big > 0.f && big < CUDART_INF_F) {
-                    const int e = exponent_above(big);
-                    up = pow2i(13 - e);
-                    unscale = pow2i(e - 13);
-                }
+            for (int u = 0; u < kUnits; ++u) {
+                const int i = u * kPerUnit + (kSplit ? 0 : lane >> 4), row_at = __shfl_sync(0xffffffffu, at, i);
+                x[u] = make_uint4(0, 0, 0, 0);
+                if (first + i < rt.rows)
+                    x[u] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (size_t)row_at * kHeadDim +
+                                                            (kSplit ? 4 * lane : 8 * (lane & 15)));
             }
-#pragma unroll 4
-            for (int c = 0; c < 16; ++c) {
-                float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (valid) load_q8<T>(row, c, f);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) q_sum += f[k];
-                if (writes) {
-                    uint32_t hi[4], lo[4];
+            for (int u = 0; u < kUnits; ++u) {
+                const int row = (warp * kUnits + u) * kPerUnit + (kSplit ? 0 : lane >> 4);
+                const uint32_t dst = base + (row >> 7) * kTileBytes;
+                if constexpr (!kSplit) {
+                    if (row < rows_all) st_shared16(dst + tile_chunk(row & 127, lane & 15), x[u].x, x[u].y, x[u].z, x[u].w);
+                } else {  // 2^13 above the row's values, as high and low parts
+                    const float f[4] = {__uint_as_float(x[u].x), __uint_as_float(x[u].y), __uint_as_float(x[u].z), __uint_as_float(x[u].w)};
+                    uint32_t big = 0, hi[2], lo[2];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
+                    for (int k = 0; k < 4; ++k) big = max(big, __float_as_uint(fabsf(f[k])));
+                    big = __reduce_max_sync(0xffffffffu, big);
+                    const int e = big > 0 && big < 0x7f800000u ? exponent_above(__uint_as_float(big)) : 13;
+                    const float up = pow2i(13 - e);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
                         const float a = f[2 * k] * up, b = f[2 * k + 1] * up;
                         hi[k] = pack_half(a, b);
                         const float2 h = h2_to_f2(hi[k]);
                         lo[k] = pack_half(a - h.x, b - h.y);
                     }
-                    st_shared16(dst + tile_chunk(r, c), hi[0], hi[1], hi[2], hi[3]);
-                    if (kSplit) st_shared16(dst + kTileBytes + tile_chunk(r, c), lo[0], lo[1], lo[2], lo[3]);
+                    const uint32_t at = dst + tile_chunk(row, lane >> 1) + 8 * (lane & 1);
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + kTileBytes), "r"(lo[0]), "r"(lo[1]) : "memory");
+                    if (lane == 0) row_unscale[row] = pow2i(e - 13);
                 }
             }
             fence_proxy_async_smem();
             mbar_arrive(&bars->q_full);
+            // the rows' sums: the 16 lanes (fp32: 32) of each of the 16 units, so
+            // that lane u ends with unit u's
+            float sum[kUnits];
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                if constexpr (kSplit) {
+                    sum[u] = (__uint_as_float(x[u].x) + __uint_as_float(x[u].y)) + (__uint_as_float(x[u].z) + __uint_as_float(x[u].w));
+                } else {
+                    const float2 a = h2_to_f2(x[u].x), b = h2_to_f2(x[u].y), c = h2_to_f2(x[u].z), d = h2_to_f2(x[u].w);
+                    sum[u] = ((a.x + a.y) + (b.x + b.y)) + ((c.x + c.y) + (d.x + d.y));
+                }
+            }
+#pragma unroll
+            for (int n = kUnits / 2; n; n >>= 1) {
+                const bool upper = lane & n;
+#pragma unroll
+                for (int u = 0; u < n; ++u) {
+                    const float keep = upper ? sum[u + n] : sum[u], give = upper ? sum[u] : sum[u + n];
+                    sum[u] = keep + __shfl_xor_sync(0xffffffffu, give, n);
+                }
+            }
+            if constexpr (kSplit) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 16);
+            if (!kSplit || lane < 16) row_sum[first + (lane & 15) * kPerUnit + (kSplit ? 0 : lane >> 4)] = sum[0];
+            asm volatile("bar.sync 1, 256;" ::: "memory");
         }
+        const float q_sum = row_sum[my_row], unscale = kSplit ? row_unscale[r] : 1.f;
         const int limit = valid ? row_keys(p, rt, row0 + my_row) : 0x7fffffff;  // a row that is none needs no mask
         const int step = turns ? 2 : 1;
         // O by f (rare, so in little code)
@@ -747,68 +764,74 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         __syncwarp();
         tc_fence_after();
         const float back = pow2i(E - 7);
-        const bool worked = j < items;  // this warpgroup had a tile
-        float *shared_o = reinterpret_cast<float *>(sm + kAtK);  // [dim][row] over K, V, now free
-        float *shared_ml = reinterpret_cast<float *>(sm);        // over Q
+        const bool direct = rt.splits == 1, merge = turns && items > 1;
         float mine = 1.f, other = 0.f;
-        if (turns) {
-            if (j == 1) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (!worked) break;
-                    uint32_t x[32];
-                    tmem_ld32(t_o + 32 * c, x);
-                    tmem_wait_ld(x);
-#pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        shared_o[(32 * c + k) * 128 + r] = fmaf(__uint_as_float(x[k]), back, z);
-                }
-                shared_ml[r] = m;
-                shared_ml[128 + r] = l;
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (j == 0 && items > 1) {
-                const float m1 = shared_ml[r], l1 = shared_ml[128 + r], mn = fmaxf(m, m1);
-                if (mn != -CUDART_INF_F) {
-                    mine = ex2(m - mn);
-                    other = ex2(m1 - mn);
-                }
-                l = l * mine + l1 * other;
-                m = mn;
-            }
-        }
-        if (!turns || j == 0) {
-            const size_t at = valid ? row_index(my_row) : 0;
-            const bool direct = rt.splits == 1, merge = turns && items > 1;
-            const float inv = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-            T *out = static_cast<T *>(p.out) + at * kHeadDim;
-            const size_t part = (size_t)split * p.total * p.hq + at;
-            if (!direct && valid) p.part_ml[part] = make_float2(m, l);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
+        // turns: warpgroup j ends with dims 64 j .. + 63 of all rows, the other
+        // half of its sums goes to the other one by shared memory, [dim][row]
+        // over K, now free
+        float *shared_o = reinterpret_cast<float *>(sm + kAtK);
+        if (merge) {
+            float *shared_ml = reinterpret_cast<float *>(sm);  // over Q
+#pragma unroll 1
+            for (int c = 2 - 2 * j; c < 4 - 2 * j; ++c) {
                 uint32_t x[32];
-                tmem_ld32(t_o + 32 * c, x);  // by whole warps: rows that are none are loaded, not stored
+                tmem_ld32(t_o + 32 * c, x);
                 tmem_wait_ld(x);
 #pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    float f[4];
+                for (int k = 0; k < 32; ++k) shared_o[(32 * c + k) * 128 + r] = fmaf(__uint_as_float(x[k]), back, z);
+            }
+            shared_ml[256 * j + r] = m;
+            shared_ml[256 * j + 128 + r] = l;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float m1 = shared_ml[256 * (j ^ 1) + r], l1 = shared_ml[256 * (j ^ 1) + 128 + r], mn = fmaxf(m, m1);
+            if (mn != -CUDART_INF_F) {
+                mine = ex2(m - mn);
+                other = ex2(m1 - mn);
+            }
+            l = l * mine + l1 * other;
+            m = mn;
+        }
+        // !merge with turns: a single tile, which was warpgroup 0's
+        const int c0 = merge ? 2 * j : 0, chunks = merge ? 2 : !turns || j == 0 ? 4 : 0;
+        const size_t at = valid ? row_index(my_row) : 0, part = (size_t)split * p.total * p.hq + at;
+        const float inv = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        if (!direct && valid && (!turns || j == 0)) p.part_ml[part] = make_float2(m, l);
+        // through shared memory (rows 16 bytes longer: no two of 8 lanes in a
+        // bank), then one bulk copy a row
+        const int size = direct ? (int)sizeof(T) : 4;
+        uint8_t *row = sm + (turns ? kAtV : kAtK) + my_row * (kHeadDim * size + 16);
+#pragma unroll 1
+        for (int c = c0; c < c0 + chunks; ++c) {
+            uint32_t x[32];
+            tmem_ld32(t_o + 32 * c, x);  // by whole warps: rows that are none are loaded, not stored
+            tmem_wait_ld(x);
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        f[d] = fmaf(__uint_as_float(x[k + d]), back, z);
-                        if (merge) f[d] = f[d] * mine + shared_o[(32 * c + k + d) * 128 + r] * other;
-                        f[d] *= inv;
-                    }
-                    if (valid) {
-                        if (direct)
-                            store_out4<T>(out + 32 * c + k, f[0], f[1], f[2], f[3]);
-                        else
-                            *reinterpret_cast<float4 *>(p.part_o + part * kHeadDim + 32 * c + k) =
-                                make_float4(f[0], f[1], f[2], f[3]);
-                    }
+            for (int k = 0; k < 32; k += 8) {
+                float f[8];
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    f[d] = fmaf(__uint_as_float(x[k + d]), back, z);
+                    if (merge) f[d] = f[d] * mine + shared_o[(32 * c + k + d) * 128 + r] * other;
+                    f[d] *= inv;
                 }
-                __syncwarp();
+                if (sizeof(T) == 2 && direct) {
+                    *reinterpret_cast<uint4 *>(row + 2 * (32 * c + k)) =
+                        make_uint4(pack_half(f[0], f[1]), pack_half(f[2], f[3]), pack_half(f[4], f[5]), pack_half(f[6], f[7]));
+                } else {
+                    *reinterpret_cast<float4 *>(row + 4 * (32 * c + k)) = make_float4(f[0], f[1], f[2], f[3]);
+                    *reinterpret_cast<float4 *>(row + 4 * (32 * c + k) + 16) = make_float4(f[4], f[5], f[6], f[7]);
+                }
             }
         }
+        fence_proxy_async_smem();  // before the copies read it
+        if (valid && chunks) {
+            uint8_t *to = direct ? static_cast<uint8_t *>(p.out) + at * (kHeadDim * sizeof(T))
+                                 : reinterpret_cast<uint8_t *>(p.part_o) + part * (kHeadDim * 4);
+            bulk_s2g(to + 32 * c0 * size, row + 32 * c0 * size, 32 * chunks * size);
+            bulk_commit();
+            bulk_wait_read_all();  // the writes are done when the grid is
+        }
+        __syncwarp();
         tc_fence_before();
     }
     __syncthreads();
@@ -1281,7 +1304,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
 // The first few_ctas CTAs take 8 of the up to 16 rows of a pair that was
 // attend_rows_kernel's, the others 8 of all rows.
 template <typename T>
-__global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_constant__ ChunkParams p, int tile_rows, int few_ctas) {
+__global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_constant__ ChunkParams p, int few_ctas) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool few = (int)blockIdx.x < few_ctas;
     bool late = false;  // the first part lies in its CTA's second place
@@ -1313,7 +1336,7 @@ __global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_consta
         }
         if (s >= 0 && sequence_tokens(p, s) * p.group > p.few_rows) {
             const int r = (t - p.q_start[s]) * p.group + h % p.group;  // among the rows of its pair
-            splits = row_tile(p, s, r / tile_rows, tile_rows, p.chunk).splits;
+            splits = row_tile(p, s, r / p.tile_rows, p.tile_rows, p.chunk).splits;
             at = row;
             step = (size_t)p.total * p.hq;
         }
@@ -1379,7 +1402,6 @@ int launch_beside(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaS
 // most 16 (few enough rows in all), or a single longer sequence.
 template <typename T, bool kSplit>
 int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
-    constexpr int tile_rows = kSplit ? 128 : 256;
     auto kern = attend_chunk_kernel<T, kSplit>;
     static std::atomic<bool> attr_done[kMaxDevices];
     if (ensure_smem_attr(attr_done, kern, kChunkSmem) != KVX_OK) return KVX_ECUDA;
@@ -1392,7 +1414,11 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     p.few_rows = few ? kFewRows : 0;
     const int tiles = key_tiles(p.max_pages);
     // row tiles: a sequence of more than 16 rows has one tile beside its whole ones
-    const long long grid_x = rows / tile_rows + (few ? std::min<long long>(p.batch, rows / (kFewRows + 1)) : p.batch);
+    auto row_tiles = [&](int tile_rows) {
+        return rows / tile_rows + (few ? std::min<long long>(p.batch, rows / (kFewRows + 1)) : p.batch);
+    };
+    p.tile_rows = kSplit || row_tiles(256) * p.hkv < 2 * sm_count() ? 128 : 256;
+    const long long grid_x = row_tiles(p.tile_rows);
     const long long most = chunk ? most_splits(grid_x * p.hkv, chunk_slots(), p.max_pages) : 1;
     p.chunk = (int)((tiles + most - 1) / most);
     const int splits = (tiles + p.chunk - 1) / p.chunk;
@@ -1406,7 +1432,7 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + (size_t)splits * all * kHeadDim);
     int rc = KVX_OK;
     if (chunk) {
-        const dim3 grid((unsigned)grid_x, (unsigned)p.hkv, (unsigned)splits);
+        const dim3 grid((unsigned)(grid_x * p.hkv), (unsigned)splits);
         kern<<<grid, kChunkThreads, kChunkSmem, st>>>(p);
         rc = launch_status();
     }
@@ -1422,7 +1448,7 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     if (rc != KVX_OK || (splits == 1 && !few)) return rc;
     const int few_grid = few ? p.batch * p.hkv * (kFewRows / 8) : 0;
     const unsigned grid = few_grid + (splits > 1 ? (unsigned)((all + 7) / 8) : 0);
-    return launch_beside(attend_combine_kernel<T>, dim3(grid), 256, 0, st, p, tile_rows, few_grid);
+    return launch_beside(attend_combine_kernel<T>, dim3(grid), 256, 0, st, p, few_grid);
 }
 
 }  // namespace
