@@ -10,30 +10,47 @@
 // one scalar per row.
 //
 // Rows: the new tokens of a sequence times the q-heads of a kv-head, token
-// major.  A CTA owns a tile of rows and a range of 128-key tiles (8 pages):
+// major.  A CTA owns a tile of 128 or 256 rows and a range of 128-key tiles
+// (8 pages); 5 warpgroups, registers dealt out with setmaxnreg:
 //  * loader warp: a bulk copy (TMA) per page and K|V, 2 KB of codes each, into
 //    staging slots;
-//  * 8 convert warps (4 for K, 4 for V): codes -> fp16 into the 128-byte-swizzled K and V tiles
-//    (K: the K-major B operand of Q K^T; V: the MN-major B operand of P V,
-//    the same bytes), two stages each;
-//  * MMA warp: one thread issues S = Q K^T (M 128, N 128, 8 steps of K 16)
-//    and O += P V with P read from tensor memory;
+//  * statistics warp: scales and middles of the next tiles, as the softmax
+//    takes them;
+//  * 2 convert warpgroups (K, V): codes -> fp16 into the 128-byte-swizzled
+//    tiles (K: the K-major B operand of Q K^T; V: the MN-major B operand of
+//    P V, the same bytes), two stages each;
+//  * MMA warp: one lane issues S = Q K^T (M 128, N 128, 8 steps of K 16) and
+//    O += P V with P read from tensor memory;
 //  * 2 softmax warpgroups, a thread per row: running maximum and sum in
 //    registers, P (fp16) written over the columns of S it came from; O stays in
 //    tensor memory and is rescaled only when a row's maximum has grown by
 //    more than 2^8 (p <= 2^8 until then).
 // The two warpgroups have an S and an O each (512 tensor-memory columns in
-// all), so one's MMAs run under the other's exponentials.  With more than 128
-// rows they own 128 rows each and share every key tile; up to 128 rows they
-// take turns at the key tiles of the same rows and are merged at the end.
+// all), so one's MMAs run under the other's exponentials.  With 256 rows they
+// own 128 each and share every key tile; with 128 they take turns at the key
+// tiles of the same rows and are merged at the end.
+//
+// What bounds it (4096 new tokens behind 28672, 24 q-heads on 8: 1.80 ms, 857
+// TFLOP/s of Q K^T and P V, 51 % of the measured bf16 rate): a step of 256
+// rows x 128 keys takes about 4600 cycles.  In it the tensor cores work 2050,
+// the exponential units 2050, shared memory about 2600 (Q and K read by
+// Q K^T, V by P V, codes copied in, read and written back as fp16), and a
+// warpgroup's own chain is maximum, exponentials, P V, the next Q K^T.  64-key
+// steps with two score buffers, which take the MMAs out of that chain, were
+// slower (2.19 ms: both warpgroups then want the exponentials at once), as was
+// handing P over by halves (1.85 ms).
 //
 // Sequences of at most 16 rows (a decode step, a few drafted tokens) would use
-// an eighth of those tiles: attend_rows_kernel takes them, on mma.sync.
+// an eighth of those tiles: attend_rows_kernel takes them, on mma.sync (8
+// sequences of 5 new tokens behind up to 8192 keys, 90 MB of codes: 35 us,
+// against 75 us in the tiles above).
 //
 // fp16 calls: P' = p s 2^(7 - E) with 2^E above the largest V scale so far: at
 // most 2^15 and normal in fp16 down to p s = 2^-21 of that scale, so a block
 // of small scale keeps its precision.  fp32 calls: q (scaled to 2^13) and P'
-// enter as fp16 high + low parts (22 bits), two MMAs for each product.
+// enter as fp16 high + low parts (22 bits), two MMAs for each product, and a
+// row tile is 128 rows (4 ragged sequences of up to 300 new tokens behind 4096,
+// 64 q-heads on 8: 176 us).
 #include <math_constants.h>
 
 #include <algorithm>
@@ -935,19 +952,29 @@ __device__ __forceinline__ int few_owner(const FewWork &w, int unit) {
     return unit < longer * (each + 1) ? unit / (each + 1) : (unit - longer) / each;
 }
 
-// Sequences of at most 16 rows: bound by the codes' bytes.  A CTA's 4 warps
-// take the pages of its range in turn.  The codes go from memory to the operands of mma.sync (m16n8k16) in registers:
-// the order of the dims within Q K^T, and of the keys and dims within P V, is
-// free as long as both operands agree, so with g = lane / 4, q = lane % 4
+// Sequences of at most 16 rows.  The warps of a CTA take the pages of its
+// range in turn; pages come by cp.async into the warp's own stages (no barrier
+// in the loop), two ahead (three: 36.0 against 35.3 us at the size below).  The
+// codes become the operands of mma.sync (m16n8k16) in registers: the order of
+// the dims within Q K^T, and of the keys and dims within P V, is free as long as
+// both operands agree, so with g = lane / 4, q = lane % 4
 //  * K: a lane reads dims 16 q .. + 15 and 64 + 16 q .. + 15 of key
 //    4 (g / 2) + g % 2 (+ 2 for the second n-tile); word s of those 32 bytes
 //    is its B fragment of k-step s.  Its scores are then keys 4 q .. 4 q + 3;
 //  * V: a lane reads dims 16 g .. + 15 of keys 4 q .. 4 q + 3, transposes them
 //    4 x 4 bytes at a time, and has its B fragments of the 16 n-tiles: n-tile
 //    t holds dims 16 n + t, so the lane ends with dims 32 q .. 32 q + 31 of O.
-// A page is one k-step of P V and has one V scale, which P takes.  Where a range
-// ends inside a (sequence, kv-head) the rows' partial results go to the
-// workspace; a CTA has two such ends at most.
+// A page is one k-step of P V and has one V scale, which P takes.  Where a
+// range ends inside a (sequence, kv-head) pair the rows' partial results go to
+// the workspace; a CTA has two such ends at most.
+//
+// 8 sequences of 5 new tokens behind up to 8192 keys, 24 q-heads on 8: 90 MB
+// of codes, 14 us at the copy rate; 28 us here (3.2 TB/s), and 7 us for the
+// launch of the empty tiles beside it and the combine.  Issue slots are half
+// full (about 450 instructions a page and warp, 4 warps a scheduler), the
+// start (lengths, page ids, first pages: three dependent reads) is a fifth.
+// 8 warps x 2 CTAs an SM against 4 x 4: 40.3 and 42.6 us at the time, for
+// fewer starts, ends and partial results.
 template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) attend_rows_kernel(const __grid_constant__ ChunkParams p) {
     constexpr int kWarps = kFewWarps<kSplit>;
@@ -1417,7 +1444,12 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     auto row_tiles = [&](int tile_rows) {
         return rows / tile_rows + (few ? std::min<long long>(p.batch, rows / (kFewRows + 1)) : p.batch);
     };
-    p.tile_rows = kSplit || row_tiles(256) * p.hkv < 2 * sm_count() ? 128 : 256;
+    // Rows of a CTA (fp16): 128 while CTAs of 256 would leave SMs idle, else
+    // 256, which converts each key tile for twice the rows.  24 q-heads on 8,
+    // 128 against 256 rows: 1001 tokens 28.5 against 32.7 us, 1500: 40.6
+    // against 56.6; 2600: 90 against 70, 5000: 249 against 203; behind 8000
+    // keys 500: 93 and 93, 3500: 572 against 580.
+    p.tile_rows = kSplit || row_tiles(256) * p.hkv <= sm_count() ? 128 : 256;
     const long long grid_x = row_tiles(p.tile_rows);
     const long long most = chunk ? most_splits(grid_x * p.hkv, chunk_slots(), p.max_pages) : 1;
     p.chunk = (int)((tiles + most - 1) / most);
