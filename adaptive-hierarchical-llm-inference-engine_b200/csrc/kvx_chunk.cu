@@ -30,19 +30,20 @@
 // own 128 each and share every key tile; with 128 they take turns at the key
 // tiles of the same rows and are merged at the end.
 //
-// What bounds it (4096 new tokens behind 28672, 24 q-heads on 8: 1.80 ms, 857
-// TFLOP/s of Q K^T and P V, 51 % of the measured bf16 rate): a step of 256
+// What bounds it (4096 new tokens behind 28672, 24 q-heads on 8: 1.63 ms, 948
+// TFLOP/s of Q K^T and P V, 56 % of the measured bf16 rate): a step of 256
 // rows x 128 keys takes about 4600 cycles.  In it the tensor cores work 2050,
 // the exponential units 2050, shared memory about 2600 (Q and K read by
 // Q K^T, V by P V, codes copied in, read and written back as fp16), and a
 // warpgroup's own chain is maximum, exponentials, P V, the next Q K^T.  64-key
 // steps with two score buffers, which take the MMAs out of that chain, were
-// slower (2.19 ms: both warpgroups then want the exponentials at once), as was
-// handing P over by halves (1.85 ms).
+// slower (2.19 against 1.80 ms: both warpgroups then want the exponentials at
+// once), as was handing P over by halves (1.85).  Splitting the row tiles of
+// the last, partly filled turn of the SMs gave 1.80 -> 1.63 (384 on 148 SMs).
 //
 // Sequences of at most 16 rows (a decode step, a few drafted tokens) would use
 // an eighth of those tiles: attend_rows_kernel takes them, on mma.sync (8
-// sequences of 5 new tokens behind up to 8192 keys, 90 MB of codes: 35 us,
+// sequences of 5 new tokens behind up to 8192 keys, 90 MB of codes: 37 us,
 // against 75 us in the tiles above).
 //
 // fp16 calls: P' = p s 2^(7 - E) with 2^E above the largest V scale so far: at
@@ -50,7 +51,7 @@
 // of small scale keeps its precision.  fp32 calls: q (scaled to 2^13) and P'
 // enter as fp16 high + low parts (22 bits), two MMAs for each product, and a
 // row tile is 128 rows (4 ragged sequences of up to 300 new tokens behind 4096,
-// 64 q-heads on 8: 176 us).
+// 64 q-heads on 8: 170 us).
 #include <math_constants.h>
 
 #include <algorithm>
@@ -78,7 +79,7 @@ struct TileStats {
     uint32_t known;           // bit i: page i is there
     uint32_t pad[2];
 };
-constexpr int kBarBytes = 288;
+constexpr int kBarBytes = 320;
 // shared memory: Q0, Q1 (staging slots 2, 3 when unused), K x 2, V x 2, staging x 2, the rest
 constexpr int kAtK = 2 * kTileBytes, kAtV = kAtK + 2 * kTileBytes, kAtStage = kAtV + 2 * kTileBytes,
               kAtMisc = kAtStage + 2 * kSlotBytes, kChunkSmem = 1024 + kAtMisc + kBarBytes + kStatSlots * (int)sizeof(TileStats) + 256 * 4;
@@ -91,34 +92,36 @@ struct ChunkParams {
     const int32_t *block_table, *q_start, *positions;
     const void *q;
     void *out;
-    float *part_o;     // [split][total * hq][128]
-    float2 *part_ml;   // [split][total * hq]
+    float *part_o;     // attend_chunk_kernel, split row tiles: [piece][tile_rows][128]
+    float2 *part_ml;   // [piece][tile_rows]
     float *few_o;      // attend_rows_kernel: [CTA][2][16][128]
     float2 *few_ml;    // [CTA][2][16]
     int32_t *error_flag;
     int batch, total, hq, hkv, group, max_pages, num_pages, causal;
-    int chunk;             // attend_chunk_kernel: key tiles of a split
-    int tile_rows;           // attend_chunk_kernel: rows of a CTA
+    int sms, max_pieces, max_splits;  // attend_chunk_kernel: pieces of split row tiles, of one of them
+    int tile_rows, tile_shift;  // attend_chunk_kernel: rows of a CTA (and log2 of it)
     int few_ctas, few_keys;  // attend_rows_kernel: CTAs; log2 of a unit's keys
     int few_rows;          // sequences of at most so many rows are attend_rows_kernel's (0: none)
     float scale_log2;
 };
-
-struct ChunkBars {
-    uint64_t ld_full[4], ld_empty[4], stat_full[kStatSlots], stat_empty[kStatSlots], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], q_full, done;
-    uint32_t tmem, gave_up;
-    uint32_t known[4];  // staging slot: bit i, page i was loaded
-    int seq, tile;
-};
-static_assert(sizeof(ChunkBars) <= kBarBytes);
 
 // Rows of one (sequence, row tile): what the kernel and the combine agree on.
 struct RowTile {
     int begin, n;      // packed rows of the sequence
     int pos, rows;     // rows in the tile
     int keys, tiles;   // keys the tile's last row sees, in 128-key tiles
-    int splits;
+    int splits, chunk; // pieces, key tiles of a piece
 };
+
+struct ChunkBars {
+    uint64_t ld_full[4], ld_empty[4], stat_full[kStatSlots], stat_empty[kStatSlots], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], q_full, done;
+    uint32_t tmem, gave_up;
+    uint32_t known[4];  // staging slot: bit i, page i was loaded
+    int seq, tile, kvh, split, part;
+    RowTile rt;
+};
+static_assert(sizeof(ChunkBars) <= kBarBytes);
+
 
 __device__ __forceinline__ int sequence_tokens(const ChunkParams &p, int s) {
     const int a = p.q_start[s], b = min(p.q_start[s + 1], p.total);
@@ -131,7 +134,9 @@ __device__ __forceinline__ int row_keys(const ChunkParams &p, const RowTile &t, 
     return (int)min(k, (long long)p.max_pages * kPageTokens);
 }
 
-__device__ __forceinline__ RowTile row_tile(const ChunkParams &p, int s, int tile, int tile_rows, int chunk) {
+constexpr int kMinChunk = 4;  // key tiles of a piece: below, a CTA's start and end outweigh its work
+
+__device__ __forceinline__ RowTile row_tile(const ChunkParams &p, int s, int tile, int tile_rows, int pieces) {
     RowTile t;
     t.begin = p.q_start[s];
     t.n = sequence_tokens(p, s);
@@ -140,8 +145,80 @@ __device__ __forceinline__ RowTile row_tile(const ChunkParams &p, int s, int til
     t.rows = min(tile_rows, all - tile * tile_rows);
     t.keys = row_keys(p, t, tile * tile_rows + t.rows - 1);
     t.tiles = (t.keys + kTileKeys - 1) / kTileKeys;
-    t.splits = max(1, (t.tiles + chunk - 1) / chunk);
+    t.splits = max(1, min(pieces, t.tiles / kMinChunk));
+    t.chunk = max(1, (t.tiles + t.splits - 1) / t.splits);
+    t.splits = max(1, (t.tiles + t.chunk - 1) / t.chunk);
     return t;
+}
+
+// The (row tile, kv-head) pairs by rank: kv-heads next to one another, the
+// last row tiles first (causal: they have the most keys).  A CTA, of which an
+// SM holds one, takes a pair, but those of the last, partly filled turn of
+// the SMs are split by keys so that the turn is filled: one pair in `pieces`.
+struct ChunkWork {
+    int tiles;   // row tiles of all sequences
+    int pairs;   // tiles * hkv
+    int whole;   // ranks below are not split
+    int pieces;  // of each of the others (at most: of at least kMinChunk key tiles each)
+};
+__device__ __forceinline__ int chunk_tiles(const ChunkParams &p, int s) {
+    const int rows = sequence_tokens(p, s) * p.group;
+    return rows > p.few_rows ? (rows + p.tile_rows - 1) >> p.tile_shift : 0;
+}
+// By a whole warp.  mine: the row tiles of sequence `lane`.
+__device__ __forceinline__ ChunkWork chunk_work(const ChunkParams &p, int *mine) {
+    const int lane = threadIdx.x & 31;
+    int tiles = 0;
+    unsigned longest = 0;  // key tiles
+    *mine = 0;
+    for (int s = lane; s < p.batch; s += 32) {
+        const int pos = p.positions[s], n = sequence_tokens(p, s), t = n * p.group > p.few_rows ? (n * p.group + p.tile_rows - 1) >> p.tile_shift : 0;
+        tiles += t;
+        if (s == lane) *mine = t;
+        if (t && pos >= 0)
+            longest = max(longest, ((unsigned)min((long long)pos + n, (long long)p.max_pages * kPageTokens) + kTileKeys - 1) / kTileKeys);
+    }
+    ChunkWork w;
+    w.tiles = __reduce_add_sync(0xffffffffu, tiles);
+    w.pairs = w.tiles * p.hkv;
+    const int rest = w.pairs % p.sms;
+    w.whole = w.pairs - rest;
+    w.pieces = 1;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (rest && longest >= 2 * kMinChunk) {
+        // turns x (key tiles + 3 for a CTA's start and end), least
+        const int most = min(min(p.max_splits, (int)longest / kMinChunk), p.max_pieces / rest);
+        unsigned best = 0xffffffffu, at = 1;
+        for (int n = 1 + lane; n <= most; n += 32) {
+            const unsigned cost = (unsigned)((rest * n + p.sms - 1) / p.sms) * ((longest + n - 1) / n + 3);
+            if (cost < best) best = cost, at = n;
+        }
+        w.pieces = (int)__reduce_min_sync(0xffffffffu, best == __reduce_min_sync(0xffffffffu, best) ? at : 0xffffffffu);
+    }
+    return w;
+}
+// By a whole warp: the sequence of row tile x, *x becomes its tile there (-1:
+// none).  mine as of chunk_work.
+__device__ __forceinline__ int chunk_sequence(const ChunkParams &p, int mine, int *x) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int s0 = 0; s0 < p.batch; s0 += 32) {
+        if (s0) mine = s0 + lane < p.batch ? chunk_tiles(p, s0 + lane) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, *x < before + sum);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            *x -= before + __shfl_sync(0xffffffffu, sum - mine, l);
+            return s0 + l;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return -1;
 }
 
 // ---- tcgen05
@@ -329,62 +406,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     TileStats *tile_stats = reinterpret_cast<TileStats *>(sm + kAtMisc + kBarBytes);
     float *row_sum = reinterpret_cast<float *>(tile_stats + kStatSlots), *row_unscale = row_sum + 128;  // [256]; fp32 calls: [128] each
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kvh = blockIdx.x % p.hkv, split = blockIdx.y;
 
     grid_dependents_launch();  // the combine may place its CTAs; it waits for this grid
-    // ---- which rows: the last tiles first (causal: they have the most keys)
+    // ---- which rows, which keys
     if (warp == 0) {
-        const int want = (gridDim.x - 1 - blockIdx.x) / p.hkv;
-        int before = 0, seq = -1, tile = 0;
-        for (int s0 = 0; s0 < p.batch && seq < 0; s0 += 32) {
-            const int s = s0 + lane;
-            const int rows = s < p.batch ? sequence_tokens(p, s) * p.group : 0;
-            const int mine = rows > p.few_rows ? (rows + tile_rows - 1) / tile_rows : 0;
-            int x = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            const uint32_t hit = __ballot_sync(0xffffffffu, want < before + x);
-            if (hit) {
-                const int l = __ffs(hit) - 1;
-                seq = s0 + l;
-                tile = want - before - __shfl_sync(0xffffffffu, x - mine, l);
-            }
-            before += __shfl_sync(0xffffffffu, x, 31);
-        }
+        int mine;
+        const ChunkWork work_of = chunk_work(p, &mine);
+        const int b = (int)blockIdx.x - work_of.whole;
+        const int rank = b < 0 ? (int)blockIdx.x : work_of.whole + b / work_of.pieces;
+        int tile = work_of.tiles - 1 - rank / p.hkv;
+        const int seq = rank < work_of.pairs ? chunk_sequence(p, mine, &tile) : -1;
         if (lane == 0) {
+            if (seq >= 0) bars->rt = row_tile(p, seq, tile, tile_rows, b < 0 ? 1 : work_of.pieces);
             bars->seq = seq;
             bars->tile = tile;
+            bars->kvh = rank % p.hkv;
+            bars->split = b < 0 ? 0 : b % work_of.pieces;
+            bars->part = b;
             bars->gave_up = 0;
         }
     }
-    __syncthreads();
-    const int seq = bars->seq, tile = bars->tile;
-    if (seq < 0) return;  // the grid is an upper bound
-    const RowTile rt = row_tile(p, seq, tile, tile_rows, p.chunk);
-    if (split >= rt.splits) return;
-    const int row0 = tile * tile_rows;
-    if (threadIdx.x == 0 && split == 0 && p.error_flag) {
-        if (rt.pos < 0) atomicOr(p.error_flag, 2);
-        if ((long long)rt.pos + rt.n > (long long)p.max_pages * kPageTokens) atomicOr(p.error_flag, 4);
-    }
-    auto row_index = [&](int r) {  // row of q / out: (token, q-head)
-        const int row = row0 + r;
-        return (size_t)(rt.begin + row / p.group) * p.hq + kvh * p.group + row % p.group;
-    };
-    if (rt.tiles == 0) {  // nothing to see
-        for (int i = threadIdx.x; i < rt.rows * (kHeadDim / 4); i += kChunkThreads)
-            store_out4<T>(static_cast<T *>(p.out) + row_index(i / (kHeadDim / 4)) * kHeadDim + 4 * (i % (kHeadDim / 4)), 0.f, 0.f,
-                          0.f, 0.f);
-        return;
-    }
-    const int t0 = split * p.chunk, tiles = min(p.chunk, rt.tiles - t0);  // this CTA's key tiles
-    const bool turns = kSplit || rt.rows <= 128;  // the warpgroups take turns at the key tiles
-    const int items = turns ? tiles : 2 * tiles;  // item w: warpgroup w % 2, key tile w or w / 2
-    const int slot_bits = turns && !kSplit ? 2 : 1, slot_mask = (1 << slot_bits) - 1;  // 4 or 2 staging slots
-    const int32_t *table = p.block_table + (size_t)seq * p.max_pages;
+    // ---- meanwhile barriers and tensor memory
     if (threadIdx.x == 32) {
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bars->ld_full[i], 1);
@@ -392,7 +434,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         }
         for (int i = 0; i < kStatSlots; ++i) {
             mbar_init(&bars->stat_full[i], 1);
-            mbar_init(&bars->stat_empty[i], turns ? 4 : 8);  // the softmax warps that look at a tile
+            mbar_init(&bars->stat_empty[i], 8);  // the softmax warps that look at a tile (turns: 4, twice each)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars->k_full[i], 4);
@@ -413,13 +455,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    auto release = [&] {
+        if (warp == kMmaWarp)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(bars->tmem) : "memory");
+    };
+    const int seq = bars->seq, tile = bars->tile, kvh = bars->kvh, split = bars->split;
+    const RowTile rt = bars->rt;
+    if (seq < 0 || split >= rt.splits) {  // the grid is an upper bound
+        release();
+        return;
+    }
+    const int row0 = tile * tile_rows;
+    if (threadIdx.x == 0 && split == 0 && p.error_flag) {
+        if (rt.pos < 0) atomicOr(p.error_flag, 2);
+        if ((long long)rt.pos + rt.n > (long long)p.max_pages * kPageTokens) atomicOr(p.error_flag, 4);
+    }
+    auto row_index = [&](int r) {  // row of q / out: (token, q-head)
+        const int row = row0 + r;
+        return (size_t)(rt.begin + row / p.group) * p.hq + kvh * p.group + row % p.group;
+    };
+    if (rt.tiles == 0) {  // nothing to see
+        for (int i = threadIdx.x; i < rt.rows * (kHeadDim / 4); i += kChunkThreads)
+            store_out4<T>(static_cast<T *>(p.out) + row_index(i / (kHeadDim / 4)) * kHeadDim + 4 * (i % (kHeadDim / 4)), 0.f, 0.f,
+                          0.f, 0.f);
+        release();
+        return;
+    }
+    const int t0 = split * rt.chunk, tiles = min(rt.chunk, rt.tiles - t0);  // this CTA's key tiles
+    const bool turns = kSplit || rt.rows <= 128;  // the warpgroups take turns at the key tiles
+    const int items = turns ? tiles : 2 * tiles;  // item w: warpgroup w % 2, key tile w or w / 2
+    const int slot_bits = turns && !kSplit ? 2 : 1, slot_mask = (1 << slot_bits) - 1;  // 4 or 2 staging slots
+    const int32_t *table = p.block_table + (size_t)seq * p.max_pages;
     // S0, S1, O0, O1: 128 columns each.  All 512 columns were asked for, so
     // they begin at 0 (were they to begin elsewhere, nothing is done).
     constexpr uint32_t tmem = 0;
     if (bars->tmem != 0) {
         if (threadIdx.x == 0 && p.error_flag) atomicOr(p.error_flag, 1);
-        if (warp == kMmaWarp)
-            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(bars->tmem) : "memory");
+        release();
         return;
     }
     auto slot_at = [&](int s) { return s < 2 ? kAtStage + s * kSlotBytes : kTileBytes + (s - 2) * kSlotBytes; };
@@ -479,8 +551,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 const float mid = fmaf(128.f, cur.z, cur.w), f = lane < 8 ? p.scale_log2 : pow2i(7 - E);
                 TileStats &t = tile_stats[i & (kStatSlots - 1)];
                 wait_or_give_up(&bars->stat_empty[i & (kStatSlots - 1)], (i / kStatSlots & 1) ^ 1, bars, p.error_flag);
+                // a K scale of zero becomes 1e-20: the -inf of a masked key stays
+                // one, and products below 2^27 of the others stay nothing
                 if (lane < 16)
-                    reinterpret_cast<float2 *>(&t.page[lane & 7])[lane >> 3] = make_float2(cur.z * f, lane < 8 ? mid * f : mid);
+                    reinterpret_cast<float2 *>(&t.page[lane & 7])[lane >> 3] =
+                        make_float2(lane < 8 && cur.z * f == 0.f ? 1e-20f : cur.z * f, lane < 8 ? mid * f : mid);
                 if (lane == 0) {
                     t.exponent = E;
                     t.known = known;
@@ -606,7 +681,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
 #pragma unroll
                     for (int k = 0; k < 4; ++k) big = max(big, __float_as_uint(fabsf(f[k])));
                     big = __reduce_max_sync(0xffffffffu, big);
-                    const int e = big > 0 && big < 0x7f800000u ? exponent_above(__uint_as_float(big)) : 13;
+                    const int e = big > 0 && big < 0x7f800000u ? max(exponent_above(__uint_as_float(big)), -37) : 13;
                     const float up = pow2i(13 - e);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
@@ -773,7 +848,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             tc_fence_before();
             mbar_arrive(&bars->p_full[j]);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->stat_empty[i & (kStatSlots - 1)]);
+            if (lane == 0) {
+                mbar_arrive(&bars->stat_empty[i & (kStatSlots - 1)]);
+                if (turns) mbar_arrive(&bars->stat_empty[i & (kStatSlots - 1)]);
+            }
         }
 
         // ---- O
@@ -810,7 +888,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         }
         // !merge with turns: a single tile, which was warpgroup 0's
         const int c0 = merge ? 2 * j : 0, chunks = merge ? 2 : !turns || j == 0 ? 4 : 0;
-        const size_t at = valid ? row_index(my_row) : 0, part = (size_t)split * p.total * p.hq + at;
+        const size_t at = valid ? row_index(my_row) : 0, part = (size_t)bars->part * tile_rows + my_row;
         const float inv = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         if (!direct && valid && (!turns || j == 0)) p.part_ml[part] = make_float2(m, l);
         // through shared memory (rows 16 bytes longer: no two of 8 lanes in a
@@ -1327,52 +1405,11 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
     grid_dependency_wait();  // the other kernel's rows are done when this grid is
 }
 
-// out[row] of the rows whose keys were split: one warp per row, 4 dims a lane.
-// The first few_ctas CTAs take 8 of the up to 16 rows of a pair that was
-// attend_rows_kernel's, the others 8 of all rows.
-template <typename T>
-__global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_constant__ ChunkParams p, int few_ctas) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const bool few = (int)blockIdx.x < few_ctas;
-    bool late = false;  // the first part lies in its CTA's second place
-    int splits = 1;
-    size_t row = 0, at = 0, step = 0;  // row of out; first part; between the parts
-    if (few) {
-        const int pair = blockIdx.x >> 1, r = (blockIdx.x & 1) * 8 + warp, s = pair / p.hkv, kvh = pair % p.hkv;
-        const int rows = sequence_tokens(p, s) * p.group;
-        int before;
-        const FewWork work_of = few_work(p, s, &before);
-        if (r < rows && rows <= p.few_rows) {
-            const int units = few_pair(p, s);
-            before += kvh * units;
-            const int first = few_owner(work_of, before + kFewStart);
-            splits = few_owner(work_of, before + units - 1) - first + 1;
-            late = few_begin(work_of, first) < before;
-            at = (size_t)first * 2 * kFewRows + r;
-            step = 2 * kFewRows;
-            row = (size_t)(p.q_start[s] + r / p.group) * p.hq + kvh * p.group + r % p.group;
-        }
-    } else {
-        row = (size_t)(blockIdx.x - few_ctas) * 8 + warp;
-        const int t = (int)(row / p.hq), h = (int)(row % p.hq);
-        int s = -1;
-        for (int s0 = 0; s0 < p.batch && s < 0 && t < p.total; s0 += 32) {
-            const int i = s0 + lane;
-            const uint32_t hit = __ballot_sync(0xffffffffu, i < p.batch && p.q_start[i] >= 0 && p.q_start[i] <= t && t < p.q_start[i + 1]);
-            if (hit) s = s0 + __ffs(hit) - 1;
-        }
-        if (s >= 0 && sequence_tokens(p, s) * p.group > p.few_rows) {
-            const int r = (t - p.q_start[s]) * p.group + h % p.group;  // among the rows of its pair
-            splits = row_tile(p, s, r / p.tile_rows, p.tile_rows, p.chunk).splits;
-            at = row;
-            step = (size_t)p.total * p.hq;
-        }
-    }
-    grid_dependency_wait();  // until here only the call's own arguments are read; every thread waits, so this grid ends last
-    if (splits == 1) return;
-    const float2 *part_ml = few ? p.few_ml : p.part_ml;
-    const float *part_o = few ? p.few_o : p.part_o;
-    auto part = [&](int c) { return at + c * step + (c == 0 && late ? kFewRows : 0); };
+// out[row] of one row whose keys were split: by a warp, 4 dims a lane.
+// part(c): the row of part_ml, part_o that holds piece c.
+template <typename T, typename Part>
+__device__ __forceinline__ void combine_row(T *out, const float *part_o, const float2 *part_ml, int splits, Part part) {
+    const int lane = threadIdx.x & 31;
     float M = -CUDART_INF_F;
     for (int c = lane; c < splits; c += 32) M = fmaxf(M, part_ml[part(c)].x);
 #pragma unroll
@@ -1388,19 +1425,62 @@ __global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_consta
         acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    store_out4<T>(static_cast<T *>(p.out) + row * kHeadDim + 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    store_out4<T>(out + 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
-constexpr int kMinChunk = 4;  // key tiles: below, a CTA's start and end outweigh its work
+// The first few_ctas CTAs take 8 of the up to 16 rows of a pair that was
+// attend_rows_kernel's, the others the rows of split row tiles in turn, one a warp.
+// Until grid_dependency_wait only the call's own arguments are read; every
+// thread waits, so this grid ends last.
+template <typename T>
+__global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_constant__ ChunkParams p, int few_ctas) {
+    const int warp = threadIdx.x >> 5;
+    T *out = static_cast<T *>(p.out);
+    if ((int)blockIdx.x < few_ctas) {
+        const int pair = blockIdx.x >> 1, r = (blockIdx.x & 1) * 8 + warp, s = pair / p.hkv, kvh = pair % p.hkv;
+        const int rows = sequence_tokens(p, s) * p.group;
+        int before, splits = 1, first = 0;
+        bool late = false;  // the first part lies in its CTA's second place
+        const FewWork work_of = few_work(p, s, &before);
+        if (r < rows && rows <= p.few_rows) {
+            const int units = few_pair(p, s);
+            before += kvh * units;
+            first = few_owner(work_of, before + kFewStart);
+            splits = few_owner(work_of, before + units - 1) - first + 1;
+            late = few_begin(work_of, first) < before;
+        }
+        grid_dependency_wait();
+        if (splits > 1)
+            combine_row<T>(out + ((size_t)(p.q_start[s] + r / p.group) * p.hq + kvh * p.group + r % p.group) * kHeadDim, p.few_o,
+                           p.few_ml, splits,
+                           [&](int c) { return (size_t)(2 * (first + c) + (c == 0 && late)) * kFewRows + r; });
+        return;
+    }
+    int mine;
+    const ChunkWork work_of = chunk_work(p, &mine);
+    const int rows = work_of.pieces > 1 ? (work_of.pairs - work_of.whole) << p.tile_shift : 0;
+    const int warps = (gridDim.x - few_ctas) * 8, first = (blockIdx.x - few_ctas) * 8 + warp;
+    grid_dependency_wait();
+#pragma unroll 1
+    for (int i = first; i < rows; i += warps) {
+        const int tail = i >> p.tile_shift, r = i & (p.tile_rows - 1), rank = work_of.whole + tail;
+        int tile = work_of.tiles - 1 - rank / p.hkv;
+        const int seq = chunk_sequence(p, mine, &tile);
+        const RowTile rt = row_tile(p, seq, tile, p.tile_rows, work_of.pieces);
+        if (r >= rt.rows || rt.splits == 1) continue;
+        const int row = tile * p.tile_rows + r;
+        combine_row<T>(out + ((size_t)(rt.begin + row / p.group) * p.hq + rank % p.hkv * p.group + row % p.group) * kHeadDim,
+                       p.part_o, p.part_ml, rt.splits,
+                       [&](int c) { return ((size_t)tail * work_of.pieces + c) * p.tile_rows + r; });
+    }
+}
 
 int key_tiles(int max_pages) { return (max_pages + kTilePages - 1) / kTilePages; }
 
-// Splits of the keys: one while `ctas` (an upper bound of the CTAs that have
-// rows) fill `slots`, else as many as fill them.
-long long most_splits(long long ctas, long long slots, int max_pages) {
-    return std::min<long long>(std::max<long long>(1, slots / ctas), std::max(1, key_tiles(max_pages) / kMinChunk));
-}
-long long chunk_slots() { return 2LL * sm_count(); }  // about two CTAs an SM (one is resident)
+// Pieces of one row tile, and of the row tiles of a call that are split: two
+// turns of the SMs where there are no more row tiles than SMs, else three.
+int most_splits(int max_pages) { return std::max(1, key_tiles(max_pages) / kMinChunk); }
+long long most_pieces(long long pairs) { return (pairs <= sm_count() ? 2LL : 3LL) * sm_count(); }
 int few_ctas(bool fp32) { return (fp32 ? kFewCtas<true> : kFewCtas<false>) * sm_count(); }
 
 // A launch that may start while the one before it in the stream runs.
@@ -1439,7 +1519,6 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     const long long rows = (long long)p.total * p.group;
     const bool chunk = rows > kFewRows, few = p.batch > 1 || rows <= kFewRows;
     p.few_rows = few ? kFewRows : 0;
-    const int tiles = key_tiles(p.max_pages);
     // row tiles: a sequence of more than 16 rows has one tile beside its whole ones
     auto row_tiles = [&](int tile_rows) {
         return rows / tile_rows + (few ? std::min<long long>(p.batch, rows / (kFewRows + 1)) : p.batch);
@@ -1450,22 +1529,29 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     // against 56.6; 2600: 90 against 70, 5000: 249 against 203; behind 8000
     // keys 500: 93 and 93, 3500: 572 against 580.
     p.tile_rows = kSplit || row_tiles(256) * p.hkv <= sm_count() ? 128 : 256;
-    const long long grid_x = row_tiles(p.tile_rows);
-    const long long most = chunk ? most_splits(grid_x * p.hkv, chunk_slots(), p.max_pages) : 1;
-    p.chunk = (int)((tiles + most - 1) / most);
-    const int splits = (tiles + p.chunk - 1) / p.chunk;
-    const size_t all = (size_t)p.total * p.hq, few_all = (size_t)few_ctas(kSplit) * 2 * kFewRows;
+    p.tile_shift = p.tile_rows == 256 ? 8 : 7;
+    const long long pairs = row_tiles(p.tile_rows) * p.hkv;  // at most
+    p.sms = sm_count();
+    p.max_splits = most_splits(p.max_pages);
+    // A prompt from (nearly) its start on more row tiles than SMs: its last
+    // turn are its shortest tiles, not worth a combine (1001 tokens, 24 q-heads
+    // on 8: 28 us, and 33 with the launches that may split them).
+    if (p.causal && p.batch == 1 && pairs > p.sms && (long long)p.max_pages * kPageTokens - p.total < 2 * kMinChunk * kTileKeys)
+        p.max_splits = 1;
+    p.max_pieces = (int)most_pieces(pairs);
+    // at most the whole pairs and the pieces, or all pairs in as many pieces as one may have
+    const long long grid_x = std::min(pairs * p.max_splits, pairs <= p.sms ? std::max(pairs, (long long)p.max_pieces) : pairs + p.max_pieces);
+    const size_t few_all = (size_t)few_ctas(kSplit) * 2 * kFewRows;
     p.few_ctas = few_ctas(kSplit);
     p.few_keys = kFewWarps<kSplit> == 8 ? 7 : 6;
     static_assert(kFewWarps<kSplit> == 8 || kFewWarps<kSplit> == 4);
     p.few_o = static_cast<float *>(workspace);
     p.few_ml = reinterpret_cast<float2 *>(p.few_o + few_all * kHeadDim);
     p.part_o = p.few_o + (few ? few_all * (kHeadDim + 2) : 0);
-    p.part_ml = reinterpret_cast<float2 *>(p.part_o + (size_t)splits * all * kHeadDim);
+    p.part_ml = reinterpret_cast<float2 *>(p.part_o + (size_t)std::min<long long>(pairs * p.max_splits, p.max_pieces) * p.tile_rows * kHeadDim);
     int rc = KVX_OK;
     if (chunk) {
-        const dim3 grid((unsigned)(grid_x * p.hkv), (unsigned)splits);
-        kern<<<grid, kChunkThreads, kChunkSmem, st>>>(p);
+        kern<<<(unsigned)grid_x, kChunkThreads, kChunkSmem, st>>>(p);
         rc = launch_status();
     }
     if (few && rc == KVX_OK) {
@@ -1477,9 +1563,10 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
             rc = launch_status();
         }
     }
-    if (rc != KVX_OK || (splits == 1 && !few)) return rc;
+    const bool split = chunk && p.max_splits > 1;
+    if (rc != KVX_OK || (!split && !few)) return rc;
     const int few_grid = few ? p.batch * p.hkv * (kFewRows / 8) : 0;
-    const unsigned grid = few_grid + (splits > 1 ? (unsigned)((all + 7) / 8) : 0);
+    const unsigned grid = few_grid + (split ? (unsigned)std::min<long long>(std::min<long long>(pairs, p.sms) * (p.tile_rows / 8), 4 * p.sms) : 0);
     return launch_beside(attend_combine_kernel<T>, dim3(grid), 256, 0, st, p, few_grid);
 }
 
@@ -1488,17 +1575,17 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
 
 using namespace kvx;
 
-// For every call of at most this many sequences, tokens and pages: splits *
-// row tiles * kv-heads stays below the slots, so the rows of the partial
-// results below slots * tile_rows; never more splits than one CTA would get.
+// For every call of at most this many sequences, tokens and pages: the pieces
+// of split row tiles, and a row tile and kv-head has at most 256 rows more
+// than its sequence.
 extern "C" KVX_API size_t kvx_attend_chunk_workspace_bytes(int32_t batch, int32_t total_tokens, int32_t num_q_heads,
                                                            int32_t num_kv_heads, int32_t max_pages) {
     if (batch <= 0 || total_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
         max_pages <= 0)
         return 0;
-    const long long splits = most_splits(num_kv_heads, chunk_slots(), max_pages);
     long long rows = 2LL * few_ctas(true) * kFewRows;
-    if (splits > 1) rows += std::min(splits * total_tokens * num_q_heads, chunk_slots() * 256);
+    const long long splits = most_splits(max_pages), padded = (long long)total_tokens * num_q_heads + 256LL * batch * num_kv_heads;
+    if (splits > 1) rows += std::min(splits * padded, 3LL * sm_count() * 256);
     return (size_t)rows * (kHeadDim + 2) * sizeof(float) + 16;
 }
 

@@ -449,9 +449,12 @@ KVX_API int kvx_rope_append(const kvx_paged *kv, const int32_t *block_table, int
  * kv-head h / (num_q_heads/num_kv_heads).  sm_scale <= 0 means 1/sqrt(128).
  * Pages outside the pool are left out (bit 1 of *error_flag), keys past the
  * block table too (bit 2), a sequence of negative position altogether (bit
- * 1); a query that sees no key gives a zero row.  Output rows outside every
- * sequence keep what they hold.  Accumulation and softmax in fp32; fp16
- * calls round the probabilities to fp16 for the second product.  workspace:
+ * 1); a query that sees no key gives a zero row.  Scales in the statistics
+ * are not negative.  Output rows outside every
+ * sequence keep what they hold; out may be q.  Accumulation and softmax in
+ * fp32; fp16 calls round the probabilities, times the V scales, to fp16 for
+ * the second product.  batch * num_kv_heads * (max_pages / 4 + 5) fits an int
+ * (else KVX_EUNSUPPORTED).  workspace:
  * kvx_attend_chunk_workspace_bytes(), 16-byte aligned, needs no
  * initialisation; calls that share one are ordered. */
 KVX_API size_t kvx_attend_chunk_workspace_bytes(int32_t batch, int32_t total_tokens,

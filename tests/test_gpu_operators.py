@@ -521,6 +521,47 @@ def test_attend_long_and_many(kvx, dtype, seed, ctx, new, hq, hkv):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("ctx,new,hq,hkv", [([3000], [801], 24, 8), ([2500, 40, 3001], [500, 2, 700], 16, 8), ([700] * 40, [20] * 40, 8, 2),
+                                            ([1100 + 7 * i for i in range(35)], [17 + i for i in range(35)], 16, 4),
+                                            ([9001, 0], [1, 260], 16, 8), ([5000], [130], 8, 1)])
+def test_attend_more_row_tiles_than_sms(kvx, dtype, ctx, new, hq, hkv):
+    """Whole row tiles and, behind them, split ones; more than 32 sequences."""
+    pool, stats, bt, start, q = attend_case(sum(new), ctx, new, hq, hkv, dtype)
+    for causal in (True, False):
+        out = kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), q, stats=stats, causal=causal)
+        assert_attended(out, attend64(pool, stats, bt, start, ctx, q, causal=causal))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("ctx,new", [([600], [2]), ([500, 77], [5, 40]), ([64], [300])])
+def test_attend_over_constant_pages(kvx, dtype, ctx, new):
+    """Pages of one value (their scale is zero), among pages of a tiny and of
+    a large range: values of 2^12 +- 2^-8 or 2^8 in V."""
+    pool, stats, bt, start, q = attend_case(61, ctx, new, 8, 2, dtype)
+    for i, page in enumerate(sorted({int(p) for row in bt for p in row if p >= 0})):
+        if i % 3 == 0:
+            stats[page, :, :, 2] = 0.0
+        elif i % 3 == 1:
+            stats[page, 1, :, 2:] *= 2.0 ** -9
+            stats[page, 1, :, 3] += 4096.0
+        else:
+            stats[page, 1, :, 2:] *= 2.0 ** 6
+    out = kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), q, stats=stats)
+    assert_attended(out, attend64(pool, stats, bt, start, ctx, q))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_attend_in_place(kvx, dtype):
+    """out may be q."""
+    ctx, new = [3000, 100, 513], [801, 4, 60]
+    pool, stats, bt, start, q = attend_case(62, ctx, new, 24, 8, dtype)
+    want = kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), q, stats=stats)
+    got = q.clone()
+    kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), got, stats=stats, out=got)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("ctx,new", [([600], [7]), ([64], [300])])
 def test_attend_over_pages_of_very_different_ranges(kvx, dtype, ctx, new):
     """Blocks whose scales differ by up to 2^20, keys far off zero."""
