@@ -48,10 +48,18 @@
 //
 // fp16 calls: P' = p s 2^(7 - E) with 2^E above the largest V scale so far: at
 // most 2^15 and normal in fp16 down to p s = 2^-21 of that scale, so a block
-// of small scale keeps its precision.  fp32 calls: q (scaled to 2^13) and P'
-// enter as fp16 high + low parts (22 bits), two MMAs for each product, and a
-// row tile is 128 rows (4 ragged sequences of up to 300 new tokens behind 4096,
-// 64 q-heads on 8: 170 us).
+// of small scale keeps its precision.
+//
+// fp32 calls: q (scaled to 2^13) and P' enter as fp16 high + low parts, 22 bits
+// or more, two MMAs for each product.  The high parts are on a grid (multiples
+// of 8 of q, of 2^-4 of P'), so their sums of products with the codes stay
+// below 2^24 grid steps and are exact although the tensor core truncates; the
+// low parts have sums of their own.  So a row tile is 128 rows, O takes 256
+// columns (high, low), S as many, and the two warpgroups take 64 keys each of
+// every tile, with one running maximum.  4 ragged sequences of up to 300 new
+// tokens behind 4096, 64 q-heads on 8: 235 us and an error of 4.3e-7; one sum
+// for both parts, the warpgroups taking turns, was 172 us and 3.4e-6 (fp32
+// products and sums of the plain form: 5850 us, 9.5e-7).
 #include <math_constants.h>
 
 #include <algorithm>
@@ -434,7 +442,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         }
         for (int i = 0; i < kStatSlots; ++i) {
             mbar_init(&bars->stat_full[i], 1);
-            mbar_init(&bars->stat_empty[i], 8);  // the softmax warps that look at a tile (turns: 4, twice each)
+            mbar_init(&bars->stat_empty[i], 8);  // the softmax warps that look at a tile (alternate: 4, twice each)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars->k_full[i], 4);
@@ -482,8 +490,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         return;
     }
     const int t0 = split * rt.chunk, tiles = min(rt.chunk, rt.tiles - t0);  // this CTA's key tiles
-    const bool turns = kSplit || rt.rows <= 128;  // the warpgroups take turns at the key tiles
-    const int items = turns ? tiles : 2 * tiles;  // item w: warpgroup w % 2, key tile w or w / 2
+    // the warpgroups take the same rows: whole key tiles in turn, or (fp32) both
+    // halves of each
+    const bool turns = kSplit || rt.rows <= 128, alternate = turns && !kSplit;
+    const int items = turns ? tiles : 2 * tiles;  // item w: warpgroup w % 2 (fp32: both), key tile w or w / 2
     const int slot_bits = turns && !kSplit ? 2 : 1, slot_mask = (1 << slot_bits) - 1;  // 4 or 2 staging slots
     const int32_t *table = p.block_table + (size_t)seq * p.max_pages;
     // S0, S1, O0, O1: 128 columns each.  All 512 columns were asked for, so
@@ -571,6 +581,41 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             const bool u_turns = uniform(turns);
             const int u_items = (int)uniform(items);
             wait_or_give_up(&bars->q_full, 0, bars, p.error_flag);
+            if constexpr (kSplit) {
+                // P V of a key tile, then the scores of the next; high and low
+                // parts have sums of their own
+#pragma unroll 1
+                for (int i = -1; i < u_items; ++i) {
+                    if (i >= 0) {
+                        wait_or_give_up(&bars->v_full[i & 1], (i >> 1) & 1, bars, p.error_flag);
+                        wait_or_give_up(&bars->p_full[0], i & 1, bars, p.error_flag);
+                        wait_or_give_up(&bars->p_full[1], i & 1, bars, p.error_flag);
+                        tc_fence_after();
+                        const uint32_t v = umma_desc_low(at + kAtV + (i & 1) * kTileBytes, kHalfBytes);
+#pragma unroll
+                        for (int part = 0; part < 2; ++part)
+#pragma unroll
+                            for (int ks = 0; ks < 8; ++ks)
+                                umma_f16_ts(issues, tmem + 256 + part * 128, tmem + ks * 16 + part * 8, v + (ks * 2048 >> 4), kIdescPV, i | ks);
+                        umma_commit(issues, &bars->v_empty[i & 1]);
+                    }
+                    if (i + 1 < u_items) {
+                        const int st = (i + 1) & 1;
+                        wait_or_give_up(&bars->k_full[st], ((i + 1) >> 1) & 1, bars, p.error_flag);
+                        tc_fence_after();
+                        const uint32_t q = umma_desc_low(at, 16), k = umma_desc_low(at + kAtK + st * kTileBytes, 16);
+#pragma unroll
+                        for (int part = 0; part < 2; ++part)
+#pragma unroll
+                            for (int ks = 0; ks < 8; ++ks) {
+                                const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                                umma_f16_ss(issues, tmem + part * 128, q + ((part * kTileBytes >> 4) + off), k + off, kIdescQK, ks);
+                            }
+                        umma_commit(issues, &bars->s_full[0]);
+                        umma_commit(issues, &bars->k_empty[st]);
+                    }
+                }
+            } else {
 #pragma unroll 1
             for (int w = -2; w < u_items; ++w) {  // P V of item w, then the scores of item w + 2
                 const int j = w & 1;
@@ -581,11 +626,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                     tc_fence_after();
                     const uint32_t v = umma_desc_low(at + kAtV + st * kTileBytes, kHalfBytes);
 #pragma unroll
-                    for (int part = 0; part < (kSplit ? 2 : 1); ++part)
-#pragma unroll
-                        for (int ks = 0; ks < 8; ++ks)  // a page: its P over its columns of S
-                            umma_f16_ts(issues, tmem + 256 + j * 128, tmem + j * 128 + ks * 16 + part * 8, v + (ks * 2048 >> 4),
-                                        kIdescPV, (w > 1) | part | ks);
+                    for (int ks = 0; ks < 8; ++ks)  // a page: its P over its columns of S
+                        umma_f16_ts(issues, tmem + 256 + j * 128, tmem + j * 128 + ks * 16, v + (ks * 2048 >> 4), kIdescPV, (w > 1) | ks);
                     if (u_turns || j) umma_commit(issues, &bars->v_empty[st]);
                 }
                 if (w + 2 < u_items) {
@@ -595,15 +637,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                     const uint32_t q = umma_desc_low(at + (u_turns ? 0 : j * kTileBytes), 16),
                                    k = umma_desc_low(at + kAtK + st * kTileBytes, 16);
 #pragma unroll
-                    for (int part = 0; part < (kSplit ? 2 : 1); ++part)
-#pragma unroll
-                        for (int ks = 0; ks < 8; ++ks) {
-                            const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
-                            umma_f16_ss(issues, tmem + j * 128, q + ((part * kTileBytes >> 4) + off), k + off, kIdescQK, part | ks);
-                        }
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                        umma_f16_ss(issues, tmem + j * 128, q + off, k + off, kIdescQK, ks);
+                    }
                     umma_commit(issues, &bars->s_full[j]);
                     if (u_turns || j) umma_commit(issues, &bars->k_empty[st]);
                 }
+            }
             }
             umma_commit(issues, &bars->done);
             __syncwarp();
@@ -650,7 +691,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         // ---- softmax: thread = row
         const int j = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t t_s = tmem + j * 128 + lanes, t_o = tmem + 256 + j * 128 + lanes;
+        // fp32: this warpgroup's half of the keys, high parts (the low ones 128 columns on)
+        const uint32_t t_s = tmem + j * (kSplit ? 64 : 128) + lanes, t_o = tmem + 256 + j * 128 + lanes;
         const int my_row = turns ? r : j * 128 + r;
         const bool valid = my_row < rt.rows;
         // Q: 16 loads of 512 contiguous bytes a warp, all in flight at once
@@ -675,7 +717,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 const uint32_t dst = base + (row >> 7) * kTileBytes;
                 if constexpr (!kSplit) {
                     if (row < rows_all) st_shared16(dst + tile_chunk(row & 127, lane & 15), x[u].x, x[u].y, x[u].z, x[u].w);
-                } else {  // 2^13 above the row's values, as high and low parts
+                } else {
+                    // Scaled to 2^13.  The high part is a multiple of 8, so its
+                    // product with the codes is below 2^24 eights: exact, however
+                    // the tensor core rounds.  The low part is the rest (to 2^-9).
                     const float f[4] = {__uint_as_float(x[u].x), __uint_as_float(x[u].y), __uint_as_float(x[u].z), __uint_as_float(x[u].w)};
                     uint32_t big = 0, hi[2], lo[2];
 #pragma unroll
@@ -686,7 +731,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const float a = f[2 * k] * up, b = f[2 * k + 1] * up;
-                        hi[k] = pack_half(a, b);
+                        hi[k] = pack_half(rintf(a * 0.125f) * 8.f, rintf(b * 0.125f) * 8.f);
                         const float2 h = h2_to_f2(hi[k]);
                         lo[k] = pack_half(a - h.x, b - h.y);
                     }
@@ -724,8 +769,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             asm volatile("bar.sync 1, 256;" ::: "memory");
         }
         const float q_sum = row_sum[my_row], unscale = kSplit ? row_unscale[r] : 1.f;
+        if (kSplit) asm volatile("bar.sync 1, 256;" ::: "memory");  // row_sum, row_unscale are free
         const int limit = valid ? row_keys(p, rt, row0 + my_row) : 0x7fffffff;  // a row that is none needs no mask
-        const int step = turns ? 2 : 1;
+        const int step = alternate ? 2 : 1;
         // O by f (rare, so in little code)
         auto scale_o = [&](float f) {
 #pragma unroll 1
@@ -738,23 +784,36 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 tmem_st16(t_o + 16 * c, o);
             }
         };
+        // pages c .. c + kStep - 1: 64 keys in x, or (fp32) 32 in x[0]
+        auto load_scores = [&](int c, uint32_t(&x)[2][32]) {
+            tmem_ld32(t_s + 16 * c, x[0]);
+            tmem_ld32(t_s + 16 * c + (kSplit ? 128 : 32), x[1]);
+            tmem_wait_ld(x[0], x[1]);
+            if constexpr (kSplit) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) x[0][k] = __float_as_uint(__uint_as_float(x[0][k]) + __uint_as_float(x[1][k]));
+            }
+        };
         float m = -CUDART_INF_F, l = 0.f, z = 0.f;  // maximum (log2), sum, sum of p mid
         int E = -100;
-        int i = turns ? j : 0;
-        for (int w = j; w < items; w += 2, i += step) {
+        constexpr int kPages = kSplit ? 4 : 8, kStep = kPages / 2;  // of an item; of those, at once
+        const int page0 = kSplit ? 4 * j : 0;
+        int i = alternate ? j : 0;
+        for (int w = kSplit ? 0 : j; w < items; w += kSplit ? 1 : 2, i += step) {
             const TileStats &ts = tile_stats[i & (kStatSlots - 1)];
             wait_or_give_up(&bars->stat_full[i & (kStatSlots - 1)], i / kStatSlots & 1, bars, p.error_flag);
-            const uint32_t known = ts.known;
-            const int e = ts.exponent, seen = limit - (t0 + i) * kTileKeys;  // the tile's keys that the row sees
-            const bool masked = __any_sync(0xffffffffu, seen < kTileKeys) || known != 0xffu;
+            const uint32_t known = kSplit ? ts.known >> page0 & 0xfu : ts.known;
+            const auto *stats = ts.page + page0;
+            const int e = ts.exponent, seen = limit - (t0 + i) * kTileKeys - page0 * kPageTokens;  // the item's keys that the row sees
+            const bool masked = __any_sync(0xffffffffu, seen < kPages * kPageTokens) || known != (1u << kPages) - 1;
             // a page this row sees nothing of: scores of -inf, whatever its statistics
             auto hidden = [&](int page) { return seen <= page * kPageTokens || !(known >> page & 1); };
-            wait_or_give_up(&bars->s_full[j], (w >> 1) & 1, bars, p.error_flag);
+            wait_or_give_up(&bars->s_full[kSplit ? 0 : j], (kSplit ? w : w >> 1) & 1, bars, p.error_flag);
             __syncwarp();
             tc_fence_after();
             if (masked) {  // few tiles: their scores are masked where they are
 #pragma unroll 1
-                for (int page = 0; page < kTilePages; ++page) {
+                for (int page = 0; page < kPages; ++page) {
                     uint32_t v[16];
                     tmem_ld16(t_s + 16 * page, v);
                     tmem_wait_ld(v);
@@ -770,16 +829,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             // together has to stay in the instruction cache.
             float top = -CUDART_INF_F;
 #pragma unroll 1
-            for (int c = 0; c < 4; c += 2) {
+            for (int c = 0; c < kPages; c += kStep) {
                 uint32_t x[2][32];
-                tmem_ld32(t_s + 32 * c, x[0]);
-                tmem_ld32(t_s + 32 * c + 32, x[1]);
-                tmem_wait_ld(x[0], x[1]);
+                load_scores(c, x);
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const int page = 2 * c + h;
+                for (int h = 0; h < kStep; ++h) {
+                    const int page = c + h;
                     uint32_t(&v)[32] = x[h >> 1];
-                    float2 ks = *reinterpret_cast<const float2 *>(&ts.page[page]);
+                    float2 ks = *reinterpret_cast<const float2 *>(&stats[page]);
                     ks.x *= unscale, ks.y *= q_sum;
                     if (masked && hidden(page)) ks = make_float2(1.f, 0.f);
                     float a = __uint_as_float(v[16 * (h & 1)]), b = __uint_as_float(v[16 * (h & 1) + 1]);
@@ -791,6 +848,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                     a = fmaxf(fmaxf(a, __uint_as_float(v[16 * (h & 1) + 14])), __uint_as_float(v[16 * (h & 1) + 15]));
                     top = fmaxf(top, fmaf(ks.x, fmaxf(a, b), ks.y));
                 }
+            }
+            if constexpr (kSplit) {  // of both halves of the keys (read before the next scores are asked for)
+                row_sum[128 * j + r] = top;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                top = fmaxf(top, row_sum[128 * (j ^ 1) + r]);
             }
             // the maximum in use may lag by kLazy; O follows where it catches
             // up, and where a larger V scale came
@@ -804,21 +866,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                     l *= f;
                     z *= f;
                 }
-                if (w >= 2) scale_o(E - e < -126 ? 0.f : f * pow2i(E - e));
+                if (w >= (kSplit ? 1 : 2)) scale_o(E - e < -126 ? 0.f : f * pow2i(E - e));
                 E = e;
             }
             const float m_use = m == -CUDART_INF_F ? 0.f : m;
 #pragma unroll 1
-            for (int c = 0; c < 4; c += 2) {
+            for (int c = 0; c < kPages; c += kStep) {
                 uint32_t x[2][32];
-                tmem_ld32(t_s + 32 * c, x[0]);
-                tmem_ld32(t_s + 32 * c + 32, x[1]);
-                tmem_wait_ld(x[0], x[1]);
+                load_scores(c, x);
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const int page = 2 * c + h;
+                for (int h = 0; h < kStep; ++h) {
+                    const int page = c + h;
                     uint32_t(&v)[32] = x[h >> 1];
-                    float4 st = ts.page[page];
+                    float4 st = stats[page];
                     st.x *= unscale;
                     st.y = fmaf(st.y, q_sum, -m_use);
                     if (masked && hidden(page)) st = make_float4(1.f, 0.f, 0.f, 0.f);
@@ -830,11 +890,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                         const float2 t = unpack2(fma2(aa, pack2(__uint_as_float(v[16 * (h & 1) + k]), __uint_as_float(v[16 * (h & 1) + k + 1])), bb));
                         const uint64_t e2 = pack2(ex2(t.x), ex2(t.y));
                         sum = add2(sum, e2);
-                        const float2 f = unpack2(mul2(e2, ss));
-                        hi[k / 2] = pack_half(f.x, f.y);
+                        const uint64_t p2 = mul2(e2, ss);
+                        const float2 f = unpack2(p2);
                         if constexpr (kSplit) {
+                            // the high part to a multiple of 2^-4 (11 bits of p s near its
+                            // largest): sums of its products are exact up to 2^20,
+                            // however the tensor core rounds
+                            constexpr float kRound = 1.5f * 524288.f;
+                            const float2 c = unpack2(add2(add2(p2, pack2(kRound, kRound)), pack2(-kRound, -kRound)));
+                            hi[k / 2] = pack_half(c.x, c.y);
                             const float2 g = h2_to_f2(hi[k / 2]);
                             lo[k / 2] = pack_half(f.x - g.x, f.y - g.y);
+                        } else {
+                            hi[k / 2] = pack_half(f.x, f.y);
                         }
                     }
                     const float2 both = unpack2(sum);
@@ -850,7 +918,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&bars->stat_empty[i & (kStatSlots - 1)]);
-                if (turns) mbar_arrive(&bars->stat_empty[i & (kStatSlots - 1)]);
+                if (alternate) mbar_arrive(&bars->stat_empty[i & (kStatSlots - 1)]);
             }
         }
 
@@ -859,7 +927,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         __syncwarp();
         tc_fence_after();
         const float back = pow2i(E - 7);
-        const bool direct = rt.splits == 1, merge = turns && items > 1;
+        const bool direct = rt.splits == 1, merge = alternate && items > 1;
         float mine = 1.f, other = 0.f;
         // turns: warpgroup j ends with dims 64 j .. + 63 of all rows, the other
         // half of its sums goes to the other one by shared memory, [dim][row]
@@ -886,8 +954,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             l = l * mine + l1 * other;
             m = mn;
         }
-        // !merge with turns: a single tile, which was warpgroup 0's
-        const int c0 = merge ? 2 * j : 0, chunks = merge ? 2 : !turns || j == 0 ? 4 : 0;
+        if constexpr (kSplit) {
+            float *shared_lz = reinterpret_cast<float *>(sm);  // over Q
+            shared_lz[256 * j + r] = l;
+            shared_lz[256 * j + 128 + r] = z;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            l += shared_lz[256 * (j ^ 1) + r];
+            z += shared_lz[256 * (j ^ 1) + 128 + r];
+        }
+        // alternate without merge: a single tile, which was warpgroup 0's
+        const int c0 = merge || kSplit ? 2 * j : 0, chunks = merge || kSplit ? 2 : !turns || j == 0 ? 4 : 0;
         const size_t at = valid ? row_index(my_row) : 0, part = (size_t)bars->part * tile_rows + my_row;
         const float inv = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         if (!direct && valid && (!turns || j == 0)) p.part_ml[part] = make_float2(m, l);
@@ -898,8 +974,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
 #pragma unroll 1
         for (int c = c0; c < c0 + chunks; ++c) {
             uint32_t x[32];
-            tmem_ld32(t_o + 32 * c, x);  // by whole warps: rows that are none are loaded, not stored
-            tmem_wait_ld(x);
+            // by whole warps: rows that are none are loaded, not stored
+            if constexpr (kSplit) {
+                uint32_t low[32];
+                tmem_ld32(tmem + 256 + lanes + 32 * c, x);
+                tmem_ld32(tmem + 384 + lanes + 32 * c, low);
+                tmem_wait_ld(x, low);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) + __uint_as_float(low[k]));
+            } else {
+                tmem_ld32(t_o + 32 * c, x);
+                tmem_wait_ld(x);
+            }
 #pragma unroll
             for (int k = 0; k < 32; k += 8) {
                 float f[8];
