@@ -883,6 +883,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                     st.y = fmaf(st.y, q_sum, -m_use);
                     if (masked && hidden(page)) st = make_float4(1.f, 0.f, 0.f, 0.f);
                     const uint64_t aa = pack2(st.x, st.x), bb = pack2(st.y, st.y), ss = pack2(st.z, st.z);
+                    // pages of a far smaller scale than the largest (2^6) keep 11 bits of their own
+                    const float grid = st.z >= 2.f ? 1.5f * 524288.f : 0.f;
+                    const uint64_t round = pack2(grid, grid), round_back = pack2(-grid, -grid);
                     uint64_t sum = 0;
                     uint32_t hi[8], lo[8];
 #pragma unroll
@@ -896,8 +899,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                             // the high part to a multiple of 2^-4 (11 bits of p s near its
                             // largest): sums of its products are exact up to 2^20,
                             // however the tensor core rounds
-                            constexpr float kRound = 1.5f * 524288.f;
-                            const float2 c = unpack2(add2(add2(p2, pack2(kRound, kRound)), pack2(-kRound, -kRound)));
+                            const float2 c = unpack2(add2(add2(p2, round), round_back));
                             hi[k / 2] = pack_half(c.x, c.y);
                             const float2 g = h2_to_f2(hi[k / 2]);
                             lo[k / 2] = pack_half(f.x - g.x, f.y - g.y);

@@ -551,6 +551,18 @@ def test_attend_over_constant_pages(kvx, dtype, ctx, new):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("ratio", [6, 9, 12, 15])
+def test_attend_rows_that_see_small_pages_only(kvx, dtype, ratio):
+    """The first rows see a page whose V scale is 2^-ratio of the next page's."""
+    ctx, new = [0, 0], [40, 300]
+    pool, stats, bt, start, q = attend_case(63 + ratio, ctx, new, 8, 2, dtype)
+    for row in bt:
+        stats[int(row[0]), 1, :, 2:] *= 2.0 ** -ratio
+    out = kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), q, stats=stats)
+    assert_attended(out, attend64(pool, stats, bt, start, ctx, q))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
 def test_attend_in_place(kvx, dtype):
     """out may be q."""
     ctx, new = [3000, 100, 513], [801, 4, 60]
