@@ -106,6 +106,7 @@ struct ChunkParams {
     float2 *few_ml;    // [CTA][2][16]
     int32_t *error_flag;
     int batch, total, hq, hkv, group, max_pages, num_pages, causal;
+    int followed;  // attend_chunk_kernel is not the call's last launch
     int sms, max_pieces, max_splits;  // attend_chunk_kernel: pieces of split row tiles, of one of them
     int tile_rows, tile_shift;  // attend_chunk_kernel: rows of a CTA (and log2 of it)
     int few_ctas, few_keys;  // attend_rows_kernel: CTAs; log2 of a unit's keys
@@ -415,7 +416,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     float *row_sum = reinterpret_cast<float *>(tile_stats + kStatSlots), *row_unscale = row_sum + 128;  // [256]; fp32 calls: [128] each
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    grid_dependents_launch();  // the combine may place its CTAs; it waits for this grid
+    // A launch of this call may place its CTAs; it waits for this grid.  The
+    // call's last launch lets nothing start: kvx_decode reads its queries and
+    // pages before it waits.
+    if (p.followed) grid_dependents_launch();
     // ---- which rows, which keys
     if (warp == 0) {
         int mine;
@@ -1637,6 +1641,8 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     p.few_ml = reinterpret_cast<float2 *>(p.few_o + few_all * kHeadDim);
     p.part_o = p.few_o + (few ? few_all * (kHeadDim + 2) : 0);
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + (size_t)std::min<long long>(pairs * p.max_splits, p.max_pieces) * p.tile_rows * kHeadDim);
+    const bool split = chunk && p.max_splits > 1;
+    p.followed = few || split;
     int rc = KVX_OK;
     if (chunk) {
         kern<<<(unsigned)grid_x, kChunkThreads, kChunkSmem, st>>>(p);
@@ -1651,7 +1657,6 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
             rc = launch_status();
         }
     }
-    const bool split = chunk && p.max_splits > 1;
     if (rc != KVX_OK || (!split && !few)) return rc;
     const int few_grid = few ? p.batch * p.hkv * (kFewRows / 8) : 0;
     const unsigned grid = few_grid + (split ? (unsigned)std::min<long long>(std::min<long long>(pairs, p.sms) * (p.tile_rows / 8), 4 * p.sms) : 0);

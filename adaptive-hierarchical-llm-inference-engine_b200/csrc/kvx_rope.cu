@@ -107,6 +107,7 @@ struct RopeAppendParams {
     int batch, total, hq, hkv, max_pages, num_pages, rotary, items;
     float amplitude;
     int kv_blocks, tokens_per_block;  // int8: CTAs that write pages, and the tokens each looks at
+    bool apart;                       // int8: q is rotated by a launch of its own
 };
 
 // The sequence that owns packed row t, or -1: all threads look at the
@@ -344,7 +345,9 @@ __global__ void __launch_bounds__(kRopeThreads, 2) rope_append_i8_kernel(const _
     __shared__ uint64_t bars[kRopeThreads / 32];
     __shared__ int slot, found;
     __shared__ int2 lead[kPageTokens];  // (sequence, packed row)
-    grid_dependents_launch();
+    // rope_append_q_kernel beside this one reads nothing that it writes; any
+    // other launch may (kvx_decode reads pages before it waits)
+    if (p.apart) grid_dependents_launch();
     if (blockIdx.x >= p.kv_blocks) {
         rope_append_rows<T, kHalf, kVec>(p, blockIdx.x - p.kv_blocks, false, cs, &slot);
         return;
@@ -455,9 +458,8 @@ int launch_rope_append(const RopeAppendParams &p, bool i8, bool half, bool vec, 
         // Many tokens: the CTAs that rotate q get a launch of their own, whose
         // few registers let 8 of them on an SM (with the other role's 128
         // registers it is 2, too few to keep the memory busy).
-        const bool apart = p.hq > 0 && p.tokens_per_block > 1;
-        kern<<<(unsigned)p.kv_blocks + (p.hq && !apart ? (unsigned)p.total : 0u), kRopeThreads, smem, st>>>(p);
-        if (!apart || launch_status() != KVX_OK) return launch_status();
+        kern<<<(unsigned)p.kv_blocks + (p.hq && !p.apart ? (unsigned)p.total : 0u), kRopeThreads, smem, st>>>(p);
+        if (!p.apart || launch_status() != KVX_OK) return launch_status();
         auto q_kern = half ? (vec ? rope_append_q_kernel<T, true, true> : rope_append_q_kernel<T, true, false>)
                            : (vec ? rope_append_q_kernel<T, false, true> : rope_append_q_kernel<T, false, false>);
         cudaLaunchConfig_t cfg{};
@@ -631,6 +633,7 @@ extern "C" KVX_API int kvx_rope_append(const kvx_paged *kv, const int32_t *block
     // 16 tokens a CTA once their pages alone fill the SMs
     p.tokens_per_block = total_tokens >= kPageTokens * sm_count() ? kPageTokens : 1;
     p.kv_blocks = (total_tokens + p.tokens_per_block - 1) / p.tokens_per_block * 2;
+    p.apart = p.hq > 0 && p.tokens_per_block > 1;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return io_dtype == KVX_F16 ? launch_rope_append<__half>(p, i8, half, vec, st)
                                : launch_rope_append<float>(p, i8, half, vec, st);

@@ -932,6 +932,52 @@ def test_a_serving_loop(kvx):
     assert err.item() == 0
 
 
+@pytest.mark.parametrize("prompt", [1, 9, 90])
+def test_calls_in_a_row_see_each_other(kvx, prompt):
+    """Appends, decodes (which start early and read their pages and queries
+    before the launch before them has ended), attention and forks on one
+    stream: the bits of the same calls with a wait after each."""
+    g, hq, hkv, layers, rows, max_pages = gen(55), 24, 8, 12, 32, 40
+    pool0 = torch.randint(-128, 128, (layers, rows * max_pages, 2, hkv, 16, 128), generator=g, dtype=torch.int8, device="cuda")
+    stats0 = torch.rand(layers, rows * max_pages, 2, hkv, 4, generator=g, device="cuda") * 0.02
+    packed = normal(g, layers, rows * prompt, hq + 2 * hkv, 128)
+    lens0 = [0 if prompt > 16 and i % 2 else 37 * i % 500 for i in range(rows)]
+    start, table = ints(range(0, rows * prompt + 1, prompt)), kvx.rope_table(128)
+    last = torch.arange(prompt - 1, rows * prompt, prompt, device="cuda")
+    results = []
+    for wait in (torch.cuda.synchronize, lambda: None):
+        pool, stats = pool0.clone(), stats0.clone()
+        pages = kvx.pages.Pages.empty(rows * max_pages, rows, max_pages, list(pool), list(stats))
+        pages.reserve(ints([n + prompt for n in lens0]))
+        ctx, outs = ints(lens0), []
+        after = ctx + prompt
+        qr = torch.empty(rows * prompt, hq, 128, dtype=F16, device="cuda")
+        torch.cuda.synchronize()
+        for layer in range(layers):
+            x = packed[layer]
+            kvx.rope_append(pool[layer], pages.block_table, start, ctx, x[:, hq:hq + hkv], x[:, hq + hkv:], q=x[:, :hq], q_out=qr,
+                            table=table, stats=stats[layer])
+            wait()
+            if prompt == 1:
+                outs.append(kvx.decode(pool[layer], pages.block_table, after, qr, stats=stats[layer]))
+                wait()
+            out = kvx.attend_chunk(pool[layer], pages.block_table, start, ctx, qr, stats=stats[layer])
+            wait()
+            outs.append(out)
+            outs.append(kvx.decode(pool[layer], pages.block_table, after, out if prompt == 1 else out[last], stats=stats[layer]))
+            wait()
+        pages.seq_lens += after
+        pages.free(ints([3]))
+        wait()
+        pages.fork(ints([0]), ints([3]))
+        wait()
+        outs.append(kvx.decode(pool[0], pages.block_table, pages.seq_lens, packed[0, :rows, :hq].contiguous(), stats=stats[0]))
+        torch.cuda.synchronize()
+        results.append(outs)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 def test_a_captured_decode_step(kvx):
     """One step (append, attend, reserve of the next) as a CUDA graph: replays
     give what eager calls give."""
