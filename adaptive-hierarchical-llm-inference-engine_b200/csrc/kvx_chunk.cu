@@ -57,7 +57,7 @@
 // low parts have sums of their own.  So a row tile is 128 rows, O takes 256
 // columns (high, low), S as many, and the two warpgroups take 64 keys each of
 // every tile, with one running maximum.  4 ragged sequences of up to 300 new
-// tokens behind 4096, 64 q-heads on 8: 235 us and an error of 4.3e-7; one sum
+// tokens behind 4096, 64 q-heads on 8: 217 us and an error of 4.3e-7; one sum
 // for both parts, the warpgroups taking turns, was 172 us and 3.4e-6 (fp32
 // products and sums of the plain form: 5850 us, 9.5e-7).
 #include <math_constants.h>
@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             mbar_init(&bars->k_empty[i], 1);
             mbar_init(&bars->v_full[i], 4);
             mbar_init(&bars->v_empty[i], 1);
-            mbar_init(&bars->s_full[i], 1);
+            mbar_init(&bars->s_full[i], kSplit && i == 1 ? 256 : 1);  // fp32: [1] says that the scores are read
             mbar_init(&bars->p_full[i], 128);
         }
         mbar_init(&bars->q_full, 256);
@@ -586,10 +586,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             const int u_items = (int)uniform(items);
             wait_or_give_up(&bars->q_full, 0, bars, p.error_flag);
             if constexpr (kSplit) {
-                // P V of a key tile, then the scores of the next; high and low
-                // parts have sums of their own
+                // P V of a key tile and the scores of the next; high and low parts
+                // have sums of their own.  The low scores' columns are free as
+                // soon as they are read: the next ones come under the exponentials.
+                const uint32_t q = umma_desc_low(at, 16);
 #pragma unroll 1
                 for (int i = -1; i < u_items; ++i) {
+                    const int st = (i + 1) & 1;
+                    const uint32_t k = umma_desc_low(at + kAtK + st * kTileBytes, 16);
+                    auto scores = [&](int part) {
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks) {
+                            const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                            umma_f16_ss(issues, tmem + part * 128, q + ((part * kTileBytes >> 4) + off), k + off, kIdescQK, ks);
+                        }
+                    };
+                    if (i + 1 < u_items) {
+                        wait_or_give_up(&bars->k_full[st], ((i + 1) >> 1) & 1, bars, p.error_flag);
+                        if (i >= 0) wait_or_give_up(&bars->s_full[1], i & 1, bars, p.error_flag);
+                        tc_fence_after();
+                        scores(1);
+                    }
                     if (i >= 0) {
                         wait_or_give_up(&bars->v_full[i & 1], (i >> 1) & 1, bars, p.error_flag);
                         wait_or_give_up(&bars->p_full[0], i & 1, bars, p.error_flag);
@@ -604,17 +621,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                         umma_commit(issues, &bars->v_empty[i & 1]);
                     }
                     if (i + 1 < u_items) {
-                        const int st = (i + 1) & 1;
-                        wait_or_give_up(&bars->k_full[st], ((i + 1) >> 1) & 1, bars, p.error_flag);
-                        tc_fence_after();
-                        const uint32_t q = umma_desc_low(at, 16), k = umma_desc_low(at + kAtK + st * kTileBytes, 16);
-#pragma unroll
-                        for (int part = 0; part < 2; ++part)
-#pragma unroll
-                            for (int ks = 0; ks < 8; ++ks) {
-                                const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
-                                umma_f16_ss(issues, tmem + part * 128, q + ((part * kTileBytes >> 4) + off), k + off, kIdescQK, ks);
-                            }
+                        scores(0);
                         umma_commit(issues, &bars->s_full[0]);
                         umma_commit(issues, &bars->k_empty[st]);
                     }
@@ -788,19 +795,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 tmem_st16(t_o + 16 * c, o);
             }
         };
-        // pages c .. c + kStep - 1: 64 keys in x, or (fp32) 32 in x[0]
+        // the 64 scores of pages c .. c + kStep - 1
         auto load_scores = [&](int c, uint32_t(&x)[2][32]) {
-            tmem_ld32(t_s + 16 * c, x[0]);
-            tmem_ld32(t_s + 16 * c + (kSplit ? 128 : 32), x[1]);
-            tmem_wait_ld(x[0], x[1]);
             if constexpr (kSplit) {
 #pragma unroll
-                for (int k = 0; k < 32; ++k) x[0][k] = __float_as_uint(__uint_as_float(x[0][k]) + __uint_as_float(x[1][k]));
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t low[32];
+                    tmem_ld32(t_s + 32 * h, x[h]);
+                    tmem_ld32(t_s + 32 * h + 128, low);
+                    tmem_wait_ld(x[h], low);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) x[h][k] = __float_as_uint(__uint_as_float(x[h][k]) + __uint_as_float(low[k]));
+                }
+            } else {
+                tmem_ld32(t_s + 16 * c, x[0]);
+                tmem_ld32(t_s + 16 * c + 32, x[1]);
+                tmem_wait_ld(x[0], x[1]);
             }
         };
         float m = -CUDART_INF_F, l = 0.f, z = 0.f;  // maximum (log2), sum, sum of p mid
         int E = -100;
-        constexpr int kPages = kSplit ? 4 : 8, kStep = kPages / 2;  // of an item; of those, at once
+        constexpr int kPages = kSplit ? 4 : 8, kStep = 4;  // of an item; of those, at once
         const int page0 = kSplit ? 4 * j : 0;
         int i = alternate ? j : 0;
         for (int w = kSplit ? 0 : j; w < items; w += kSplit ? 1 : 2, i += step) {
@@ -830,12 +845,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 tmem_wait_st();
             }
             // Two loops of two chunks of 32 keys each: the code of all warps
-            // together has to stay in the instruction cache.
+            // together has to stay in the instruction cache.  fp32: one chunk, held.
             float top = -CUDART_INF_F;
+            uint32_t held[2][32];
 #pragma unroll 1
             for (int c = 0; c < kPages; c += kStep) {
-                uint32_t x[2][32];
+                uint32_t fresh[2][32], (&x)[2][32] = kSplit ? held : fresh;
                 load_scores(c, x);
+                if constexpr (kSplit) {
+                    tc_fence_before();
+                    mbar_arrive(&bars->s_full[1]);
+                }
 #pragma unroll
                 for (int h = 0; h < kStep; ++h) {
                     const int page = c + h;
@@ -876,8 +896,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             const float m_use = m == -CUDART_INF_F ? 0.f : m;
 #pragma unroll 1
             for (int c = 0; c < kPages; c += kStep) {
-                uint32_t x[2][32];
-                load_scores(c, x);
+                uint32_t fresh[2][32], (&x)[2][32] = kSplit ? held : fresh;
+                if constexpr (!kSplit) load_scores(c, x);
 #pragma unroll
                 for (int h = 0; h < kStep; ++h) {
                     const int page = c + h;
