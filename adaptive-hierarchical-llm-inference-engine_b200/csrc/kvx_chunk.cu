@@ -994,7 +994,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         const float inv = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         if (!direct && valid && (!turns || j == 0)) p.part_ml[part] = make_float2(m, l);
         // through shared memory (rows 16 bytes longer: no two of 8 lanes in a
-        // bank), then one bulk copy a row
+        // bank)
         const int size = direct ? (int)sizeof(T) : 4;
         uint8_t *row = sm + (turns ? kAtV : kAtK) + my_row * (kHeadDim * size + 16);
 #pragma unroll 1
@@ -1030,15 +1030,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 }
             }
         }
-        fence_proxy_async_smem();  // before the copies read it
-        if (valid && chunks) {
-            uint8_t *to = direct ? static_cast<uint8_t *>(p.out) + at * (kHeadDim * sizeof(T))
-                                 : reinterpret_cast<uint8_t *>(p.part_o) + part * (kHeadDim * 4);
-            bulk_s2g(to + 32 * c0 * size, row + 32 * c0 * size, 32 * chunks * size);
-            bulk_commit();
-            bulk_wait_read_all();  // the writes are done when the grid is
-        }
         __syncwarp();
+        // 16 bytes a lane, whole stretches of rows together (a bulk copy a row
+        // took 1.2 us to issue, for all rows of the CTA)
+        const int shift = 31 - __clz(max(1, 32 * chunks * size / 16)), some = direct ? (int)at : (int)part;
+        const uint32_t rows_there = __ballot_sync(0xffffffffu, valid);
+        uint8_t *to = direct ? static_cast<uint8_t *>(p.out) : reinterpret_cast<uint8_t *>(p.part_o);
+        const uint8_t *from = row - lane * (kHeadDim * size + 16) + 32 * c0 * size;
+        if (chunks)
+#pragma unroll 4
+            for (int i = lane; i < 32 << shift; i += 32) {
+                const int of = i >> shift, byte = 16 * (i & ((1 << shift) - 1));
+                const int its = __shfl_sync(0xffffffffu, some, of);
+                if (rows_there >> of & 1)
+                    *reinterpret_cast<uint4 *>(to + (size_t)its * (kHeadDim * size) + 32 * c0 * size + byte) =
+                        *reinterpret_cast<const uint4 *>(from + of * (kHeadDim * size + 16) + byte);
+            }
         tc_fence_before();
     }
     __syncthreads();
