@@ -5,9 +5,11 @@
 // (cos, sin) pairs are worked out once into shared memory (rotary/2 sincospi
 // for heads * rotary/2 pairs), each thread keeps one item of a row -- a
 // 16-byte vector, or the two that pair up in the half layout -- with its
-// cosines in registers and walks the token's rows.  Backward of 8191 tokens x
-// 72 heads of 128 (64 rotated, interleaved, fp32, strided): 98 us, 6.2 TB/s
-// (0.95 of the measured copy rate); 64 tokens of 32 heads: 2.3 us, a launch.
+// cosines in registers and walks the token's rows, the first of which are
+// asked for before the cosines are worked out (afterwards: 98 against 93 us).
+// Backward of 8191 tokens x 72 heads of 128 (64 rotated, interleaved, fp32,
+// strided): 93 us, 6.5 TB/s, the measured copy rate; 64 tokens of 32 heads:
+// 2.3 us, a launch.
 #include <math.h>
 
 #include <algorithm>
@@ -23,6 +25,7 @@ namespace {
 constexpr int kMaxRopeDim = 1024;
 constexpr int kRopeThreads = 256;
 constexpr int kRowsInFlight = 4;  // rows whose loads a thread issues together
+constexpr int kRowsBeside = 2;    // the same, of rope_append_q_kernel (59 us at the size below; 4 and 2 CTAs an SM: 84; 1 and 5: 65)
 
 struct RopeTensor {
     const void *in;
@@ -49,24 +52,29 @@ __device__ __forceinline__ void fill_cs(float2 *cs, const uint64_t *turns, int p
     }
 }
 
-// Rows row0, row0 + step, ... < rows of the tensors, this thread's item of each.
-template <typename Item, typename T, typename Address>
-__device__ __forceinline__ void rope_rows(const Item &item, int row0, int step, int rows, Address at) {
-    for (int r = row0; r < rows; r += kRowsInFlight * step) {
-        typename Item::Data d[kRowsInFlight];
-        const T *src[kRowsInFlight];
-        T *dst[kRowsInFlight];
-        bool turn[kRowsInFlight];
+// Rows row0, row0 + step, ... < rows of the tensors, this thread's item of
+// each.  ready() runs once (in every thread, rows or not) when the first rows
+// have been asked for: the cosines are worked out while they are on their way.
+template <int kRows, typename Item, typename T, typename Address, typename Ready>
+__device__ __forceinline__ void rope_rows(const Item &item, int row0, int step, int rows, Address at, Ready ready) {
+    bool asked = false;
+    for (int r = row0; r < rows || !asked; r += kRows * step) {
+        typename Item::Data d[kRows];
+        const T *src[kRows];
+        T *dst[kRows];
+        bool turn[kRows];
 #pragma unroll
-        for (int u = 0; u < kRowsInFlight; ++u) {
+        for (int u = 0; u < kRows; ++u) {
             dst[u] = nullptr;
             if (r + u * step < rows) {
                 at(r + u * step, src[u], dst[u], turn[u]);
                 if (dst[u]) item.load(src[u], d[u]);
             }
         }
+        if (!asked) ready();
+        asked = true;
 #pragma unroll
-        for (int u = 0; u < kRowsInFlight; ++u)
+        for (int u = 0; u < kRows; ++u)
             if (dst[u]) {
                 if (turn[u]) item.turn(d[u]);
                 item.store(dst[u], d[u]);
@@ -78,19 +86,22 @@ template <typename T, bool kHalf, bool kVec>
 __global__ void __launch_bounds__(kVec ? kRopeThreads : kMaxRopeDim) rope_kernel(const __grid_constant__ RopeParams p) {
     __shared__ float2 cs[kMaxRopeDim / 2];
     const int64_t t = blockIdx.x;
-    fill_cs(cs, p.turns, p.rotary / 2, p.positions[t], p.amplitude, p.sine_sign);
-    __syncthreads();
     const int step = blockDim.x / p.items, row0 = threadIdx.x / p.items;
-    if (row0 >= step) return;  // threads left over by whole rows
-    const RopeItem<T, kHalf, kVec> item(threadIdx.x % p.items, p.rotary, cs);
-    rope_rows<RopeItem<T, kHalf, kVec>, T>(
-        item, row0, step, p.x[0].heads + p.x[1].heads, [&](int r, const T *&src, T *&dst, bool &turn) {
+    RopeItem<T, kHalf, kVec> item(threadIdx.x % p.items, p.rotary);
+    rope_rows<kRowsInFlight, RopeItem<T, kHalf, kVec>, T>(
+        item, row0, step, row0 < step ? p.x[0].heads + p.x[1].heads : 0,  // threads left over by whole rows: none
+        [&](int r, const T *&src, T *&dst, bool &turn) {
             const int which = r >= p.x[0].heads;
             const RopeTensor &x = p.x[which];
             const int64_t h = which ? r - p.x[0].heads : r;
             src = static_cast<const T *>(x.in) + t * x.in_token + h * x.in_head;
             dst = static_cast<T *>(x.out) + t * x.out_token + h * x.out_head;
             turn = true;
+        },
+        [&] {
+            fill_cs(cs, p.turns, p.rotary / 2, p.positions[t], p.amplitude, p.sine_sign);
+            __syncthreads();
+            item.cosines(cs);
         });
 }
 
@@ -124,16 +135,12 @@ __device__ __forceinline__ int find_sequence(const int32_t *q_start, int batch, 
 }
 
 // Token blockIdx: rotate q, and (fp16 / fp32 pools) rotate k and store k, v.
-template <typename T, bool kHalf, bool kVec>
+template <int kRows, typename T, bool kHalf, bool kVec>
 __device__ __forceinline__ void rope_append_rows(const RopeAppendParams &p, int t, bool with_kv, float2 *cs, int *slot) {
     const int s = find_sequence(p.q_start, p.batch, t, slot);
     if (s < 0) return;
     const int off = t - p.q_start[s];
     const long long pos = (long long)p.positions[s] + off;
-    if (p.turns) {
-        fill_cs(cs, p.turns, p.rotary / 2, pos, p.amplitude, 1.f);
-        __syncthreads();
-    }
     T *page_row = nullptr;  // K row of head 0 at the token's slot
     if (with_kv) {
         const long long lp = pos >> 4;
@@ -144,11 +151,10 @@ __device__ __forceinline__ void rope_append_rows(const RopeAppendParams &p, int 
             atomicOr(p.error_flag, 2);
     }
     const int step = blockDim.x / p.items, row0 = threadIdx.x / p.items;
-    if (row0 >= step) return;
-    const RopeItem<T, kHalf, kVec> item(threadIdx.x % p.items, p.rotary, cs);
+    RopeItem<T, kHalf, kVec> item(threadIdx.x % p.items, p.rotary);
     const bool turning = p.turns != nullptr;
-    rope_rows<RopeItem<T, kHalf, kVec>, T>(
-        item, row0, step, p.hq + (page_row ? 2 * p.hkv : 0), [&](int r, const T *&src, T *&dst, bool &turn) {
+    rope_rows<kRows, RopeItem<T, kHalf, kVec>, T>(
+        item, row0, step, row0 < step ? p.hq + (page_row ? 2 * p.hkv : 0) : 0, [&](int r, const T *&src, T *&dst, bool &turn) {
             turn = turning;
             if (r < p.hq) {
                 src = static_cast<const T *>(p.q) + (int64_t)t * p.q_stride + r * kHeadDim;
@@ -163,6 +169,12 @@ __device__ __forceinline__ void rope_append_rows(const RopeAppendParams &p, int 
                 src = static_cast<const T *>(p.v) + (int64_t)t * p.v_stride + (r - p.hkv) * kHeadDim;
                 turn = false;
             }
+        },
+        [&] {
+            if (!turning) return;
+            fill_cs(cs, p.turns, p.rotary / 2, pos, p.amplitude, 1.f);
+            __syncthreads();
+            item.cosines(cs);
         });
 }
 
@@ -172,7 +184,7 @@ template <typename T, bool kHalf, bool kVec>
 __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_constant__ RopeAppendParams p) {
     __shared__ float2 cs[kHeadDim / 2];
     __shared__ int slot;
-    rope_append_rows<T, kHalf, kVec>(p, blockIdx.x, true, cs, &slot);
+    rope_append_rows<kRowsInFlight, T, kHalf, kVec>(p, blockIdx.x, true, cs, &slot);
 }
 
 // ---- int8 pages
@@ -334,9 +346,9 @@ __device__ __forceinline__ void append_block_i8(const T *src, int64_t stride, ui
 // among its tokens_per_block packed rows: one token a CTA while tokens are few
 // (a decode step, where every token leads), 16 when they fill the GPU anyway.
 // 32 sequences x 1 token (24 q-heads on 8): 4.2 us, three dependent reads and
-// a launch.  6 chunks of up to 2731 tokens (64 q-heads on 8, fp16): 113 us for
-// 476 MB, 43 of them the pages (bound by instructions: unpack, turn, range,
-// quantise, about 40 % of the issue slots at 2 CTAs an SM) and 70 the q rows.
+// a launch.  6 chunks of up to 2731 tokens (64 q-heads on 8, fp16): 102 us for
+// 410 MB, 43 of them the pages (bound by instructions: unpack, turn, range,
+// quantise, about 40 % of the issue slots at 2 CTAs an SM) and 59 the q rows.
 //
 // A warp with more than kDirectRows rows brings them to shared memory first,
 // a bulk copy (TMA) a row, all in flight together; fewer are read in place,
@@ -355,7 +367,7 @@ __global__ void __launch_bounds__(kRopeThreads, 2) rope_append_i8_kernel(const _
     // other launch may (kvx_decode reads pages before it waits)
     if (p.apart) grid_dependents_launch();
     if (blockIdx.x >= p.kv_blocks) {
-        rope_append_rows<T, kHalf, kVec>(p, blockIdx.x - p.kv_blocks, false, cs, &slot);
+        rope_append_rows<kRowsInFlight, T, kHalf, kVec>(p, blockIdx.x - p.kv_blocks, false, cs, &slot);
         return;
     }
     const bool is_v = blockIdx.x & 1;
@@ -437,10 +449,10 @@ __global__ void __launch_bounds__(kRopeThreads, 2) rope_append_i8_kernel(const _
 // The q rows of many tokens, beside the CTAs that write their pages: placed
 // while those run (nothing here depends on them), done when they are done.
 template <typename T, bool kHalf, bool kVec>
-__global__ void __launch_bounds__(kRopeThreads) rope_append_q_kernel(const __grid_constant__ RopeAppendParams p) {
+__global__ void __launch_bounds__(kRopeThreads, 4) rope_append_q_kernel(const __grid_constant__ RopeAppendParams p) {
     __shared__ float2 cs[kHeadDim / 2];
     __shared__ int slot;
-    rope_append_rows<T, kHalf, kVec>(p, blockIdx.x, false, cs, &slot);
+    rope_append_rows<kRowsBeside, T, kHalf, kVec>(p, blockIdx.x, false, cs, &slot);
     grid_dependency_wait();
 }
 
@@ -462,8 +474,8 @@ int launch_rope_append(const RopeAppendParams &p, bool i8, bool half, bool vec, 
         static std::atomic<bool> attr_done[4][kMaxDevices];
         if (smem && ensure_smem_attr(attr_done[2 * half + vec], kern, smem) != KVX_OK) return KVX_ECUDA;
         // Many tokens: the CTAs that rotate q get a launch of their own, whose
-        // few registers let 8 of them on an SM (with the other role's 128
-        // registers it is 2, too few to keep the memory busy).
+        // 64 registers let 4 of them on an SM (with the other role's 128 it is
+        // 2, too few to keep the memory busy).
         kern<<<(unsigned)p.kv_blocks + (p.hq && !p.apart ? (unsigned)p.total : 0u), kRopeThreads, smem, st>>>(p);
         if (!p.apart || launch_status() != KVX_OK) return launch_status();
         auto q_kern = half ? (vec ? rope_append_q_kernel<T, true, true> : rope_append_q_kernel<T, true, false>)

@@ -81,22 +81,23 @@ struct RopeItem {
     bool turns;
     float2 cs[kPairs];
 
-    // cs_row: (cos, sin) of the token's pairs, in shared memory
-    __device__ __forceinline__ RopeItem(int item, int rotary, const float2 *cs_row) {
+    __device__ __forceinline__ RopeItem(int item, int rotary) {
         const int half = rotary / 2;
         const int turning = kHalf ? half / E : (kVec ? rotary / E : half);
         turns = item < turning;
         if (turns) {
             first = kHalf ? item * E : (kVec ? item * E : 2 * item);
             second = kHalf ? first + half : first + 1;
-#pragma unroll
-            for (int k = 0; k < kPairs; ++k) cs[k] = cs_row[(kHalf ? first : first / 2) + k];
         } else {
             first = rotary + (item - turning) * E;
             second = -1;
-#pragma unroll
-            for (int k = 0; k < kPairs; ++k) cs[k] = make_float2(1.f, 0.f);
         }
+    }
+    // cs_row: (cos, sin) of the token's pairs, in shared memory
+    __device__ __forceinline__ void cosines(const float2 *cs_row) {
+        if (turns)
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) cs[k] = cs_row[(kHalf ? first : first / 2) + k];
     }
 
     struct Data {
