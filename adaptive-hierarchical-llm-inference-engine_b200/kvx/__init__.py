@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -112,7 +113,7 @@ class RopeRows(C.Structure):
 
 _i64 = C.c_int64
 lib.kvx_rope_frequencies.argtypes = [C.POINTER(RopeConfig), _vp, C.POINTER(C.c_float)]
-lib.kvx_rope.argtypes = [C.POINTER(RopeTableC), _vp, _i32, _i32, _i32, C.POINTER(RopeRows), _i32, _i32, _vp]
+lib.kvx_rope.argtypes = [C.POINTER(RopeTableC), _vp, _i32, _i32, _i32, _vp, _i32, _i32, _vp]  # RopeRows, or their bytes
 lib.kvx_rope_append.argtypes = [C.POINTER(KvPaged), _vp, _i32, _vp, _vp, _i32, _i32, C.POINTER(RopeTableC), _i32, _vp, _i64,
                                 _vp, _i32, _vp, _i64, _vp, _i64, _vp, _vp]
 lib.kvx_attend_chunk_workspace_bytes.restype = _sz
@@ -482,7 +483,7 @@ def _runtime():
     global _rt
     torch = _torch()
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
-    _rt = (torch.float16, torch.float32, torch.int32, raw, torch.cuda.current_device)
+    _rt = (torch.float16, torch.float32, torch.int32, raw, getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device))
     return _rt
 
 
@@ -537,6 +538,7 @@ class RopeTable:
     def __init__(self, turns, rotary_dim, layout, amplitude):
         self.turns, self.rotary_dim, self.layout, self.amplitude = turns, rotary_dim, layout, amplitude
         self.c = RopeTableC(turns.data_ptr(), rotary_dim, ROPE_LAYOUT[layout], amplitude)
+        self.ref = C.byref(self.c)
 
 
 def rope_frequencies(rotary_dim, base=10000.0, scaling="none", factor=1.0, low=1.0, high=4.0, original_context=8192.0):
@@ -561,8 +563,13 @@ def rope_table(rotary_dim, base=10000.0, layout="half", scaling="none", factor=1
     return RopeTable(torch.tensor(signed, dtype=torch.int64).to(device), rotary_dim, layout, amplitude)
 
 
+# kvx_rope_rows as bytes, one and two of them: a quarter of the time that
+# ctypes takes to make the structures
+_ROWS = {n: struct.Struct("@" + "QQi4xqqqq" * n) for n in (1, 2)}
+
+
 def _rope_rows(x, out, what):
-    """The RopeRows of a tensor [tokens][heads][dim] and its output."""
+    """The fields of the RopeRows of a tensor [tokens][heads][dim] and its output."""
     sx, so = x.stride(), out.stride()
     shape = x.shape
     if len(shape) != 3 or (shape[2] > 1 and (sx[2] != 1 or so[2] != 1)):
@@ -571,7 +578,7 @@ def _rope_rows(x, out, what):
         raise ValueError(what + "_out: shape and dtype of its input")
     if (so[0] == 0 and shape[0] > 1) or (so[1] == 0 and shape[1] > 1):
         raise ValueError(what + "_out: strides without overlap")
-    return RopeRows(x.data_ptr(), out.data_ptr(), shape[1], sx[0], sx[1], so[0], so[1])
+    return x.data_ptr(), out.data_ptr(), shape[1], sx[0], sx[1], so[0], so[1]
 
 
 def rope(q, k, positions, table, q_out=None, k_out=None, inverse=False, stream=None):
@@ -581,21 +588,21 @@ def rope(q, k, positions, table, q_out=None, k_out=None, inverse=False, stream=N
     Returns (q_out, k_out)."""
     if q_out is None:
         q_out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
-    rows = (RopeRows * 2)()
-    rows[0] = _rope_rows(q, q_out, "q")
+    rows = _rope_rows(q, q_out, "q")
     tokens, _, dim = q.shape
     n = 1
     if k is not None:
         if k_out is None:
             k_out = _torch().empty(k.shape, dtype=k.dtype, device=k.device)
-        rows[1] = _rope_rows(k, k_out, "k")
+        rows += _rope_rows(k, k_out, "k")
         n = 2
         if k.shape[0] != tokens or k.shape[2] != dim or k.dtype != q.dtype:
             raise ValueError("k: tokens, dim and dtype of q")
     _vector(positions, tokens, "positions")
     code = _io_code(q, "q")
     dev = _one_device(q, q_out, k, k_out, positions, table.turns)
-    rc = _launch(dev, stream, lib.kvx_rope, C.byref(table.c), positions.data_ptr(), tokens, dim, code, rows, n, 1 if inverse else 0)
+    rc = _launch(dev, stream, lib.kvx_rope, table.ref, positions.data_ptr(), tokens, dim, code, _ROWS[n].pack(*rows), n,
+                 1 if inverse else 0)
     if rc:
         raise KvxError("kvx_rope", rc)
     return q_out, k_out
@@ -664,7 +671,7 @@ def rope_append(pool, block_table, q_start, positions, k, v, q=None, q_out=None,
     dev = _one_device(k, v, q, q_out, block_table, q_start, positions, error_flag, tensor, stats,
                       None if table is None else table.turns)
     rc = _launch(dev, stream, lib.kvx_rope_append, C.byref(kv), block_table.data_ptr(), max_pages, q_start.data_ptr(),
-                 positions.data_ptr(), batch, tokens, None if table is None else C.byref(table.c), code, q_ptr, qs, out_ptr, hq,
+                 positions.data_ptr(), batch, tokens, None if table is None else table.ref, code, q_ptr, qs, out_ptr, hq,
                  k.data_ptr(), ks, v.data_ptr(), vs, _flag(error_flag))
     if rc:
         raise KvxError("kvx_rope_append", rc)
