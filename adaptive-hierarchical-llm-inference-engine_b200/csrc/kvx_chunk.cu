@@ -107,7 +107,7 @@ struct ChunkParams {
     int32_t *error_flag;
     int batch, total, hq, hkv, group, max_pages, num_pages, causal;
     int followed;  // attend_chunk_kernel is not the call's last launch
-    int sms, max_pieces, max_splits;  // attend_chunk_kernel: pieces of split row tiles, of one of them
+    int sms, max_tiles, max_pieces, max_splits;  // attend_chunk_kernel: row tiles, pieces of split ones, of one of them
     int tile_rows, tile_shift;  // attend_chunk_kernel: rows of a CTA (and log2 of it)
     int few_ctas, few_keys;  // attend_rows_kernel: CTAs; log2 of a unit's keys
     int few_rows;          // sequences of at most so many rows are attend_rows_kernel's (0: none)
@@ -188,7 +188,8 @@ __device__ __forceinline__ ChunkWork chunk_work(const ChunkParams &p, int *mine)
             longest = max(longest, ((unsigned)min((long long)pos + n, (long long)p.max_pages * kPageTokens) + kTileKeys - 1) / kTileKeys);
     }
     ChunkWork w;
-    w.tiles = __reduce_add_sync(0xffffffffu, tiles);
+    // a q_start that does not ascend may claim more rows than there are
+    w.tiles = min(__reduce_add_sync(0xffffffffu, tiles), p.max_tiles);
     w.pairs = w.tiles * p.hkv;
     const int rest = w.pairs % p.sms;
     w.whole = w.pairs - rest;
@@ -1649,7 +1650,8 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     // keys 500: 93 and 93, 3500: 572 against 580.
     p.tile_rows = kSplit || row_tiles(256) * p.hkv <= sm_count() ? 128 : 256;
     p.tile_shift = p.tile_rows == 256 ? 8 : 7;
-    const long long pairs = row_tiles(p.tile_rows) * p.hkv;  // at most
+    p.max_tiles = (int)row_tiles(p.tile_rows);
+    const long long pairs = (long long)p.max_tiles * p.hkv;  // at most
     p.sms = sm_count();
     p.max_splits = most_splits(p.max_pages);
     // A prompt from (nearly) its start on more row tiles than SMs: its last

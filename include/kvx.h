@@ -410,14 +410,15 @@ KVX_API int kvx_rope(const kvx_rope_table *table, const int32_t *positions, int3
                      int32_t inverse, void *stream);
 
 /* Rotate and append a ragged batch.  Tokens of all sequences lie packed:
- * sequence s owns rows q_start[s] .. q_start[s+1]-1 (device int32
- * [batch + 1], ascending), its first token at position positions[s] (device
- * int32 [batch]).  Rows outside every sequence are neither read nor written.
- * q (NULL with num_q_heads 0): [total_tokens][num_q_heads][128] is rotated
- * into q_out (contiguous; q_out may be q when q is contiguous); k, v:
- * [total_tokens][num_kv_heads][128]; k is rotated, then k and v are stored in
- * the pages of the block table.  *_stride: elements between tokens (at least
- * heads * 128); every row 16-byte aligned.  table NULL: no rotation.
+ * sequence s owns rows q_start[s] .. q_start[s+1]-1 (device int32 [batch + 1],
+ * ascending; otherwise results are undefined, memory stays safe), its first
+ * token at position positions[s] (device int32 [batch]).  Rows outside every
+ * sequence are neither read nor written. q (NULL with num_q_heads 0):
+ * [total_tokens][num_q_heads][128] is rotated into q_out (contiguous; q_out may
+ * be q when q is contiguous); k, v: [total_tokens][num_kv_heads][128]; k is
+ * rotated, then k and v are stored in the pages of the block table.  *_stride:
+ * elements between tokens (at least heads * 128); every row 16-byte aligned.
+ * table NULL: no rotation.
  *
  * KVX_F16 / KVX_F32 pools (io_dtype the pool's): the bits of kvx_rope, then
  * kvx_append.  KVX_I8 pools (io_dtype KVX_F16 or KVX_F32; kv->stats is

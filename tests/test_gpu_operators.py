@@ -563,6 +563,21 @@ def test_attend_rows_that_see_small_pages_only(kvx, dtype, ratio):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
+def test_attend_with_starts_that_do_not_ascend(kvx, dtype):
+    """Ranges that overlap claim more rows than there are: no result is
+    promised, but the workspace's end holds and every row is a number."""
+    rows, hq, hkv = 400, 16, 8
+    start = [0, 400, 2, 390, 1, 400, 5, 400]
+    ctx = [1500] * (len(start) - 1)
+    pool, stats, bt, _, _ = attend_case(64, ctx, [400] * len(ctx), hq, hkv, dtype)
+    q = normal(gen(65), rows, hq, 128, dtype=dtype)
+    ws = kvx.attend_chunk_workspace(len(ctx), rows, hq, hkv, bt.shape[1])
+    guarded = torch.full((ws.numel() + 4096,), 171, dtype=torch.uint8, device="cuda")
+    out = kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), q, stats=stats, workspace=guarded[: ws.numel()])
+    assert (guarded[ws.numel():] == 171).all() and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
 def test_attend_in_place(kvx, dtype):
     """out may be q."""
     ctx, new = [3000, 100, 513], [801, 4, 60]
