@@ -577,6 +577,34 @@ def test_attend_with_starts_that_do_not_ascend(kvx, dtype):
     assert (guarded[ws.numel():] == 171).all() and torch.isfinite(out).all()
 
 
+def test_attend_two_at_once(kvx):
+    """Calls of two streams, a workspace each: the bits of the same calls
+    alone.  Mixed lengths, both types, the dense attention beside them (it
+    takes tensor memory too)."""
+    cases = []
+    for seed, dtype in ((66, F16), (67, F32)):
+        ctx, new = [2000, 40, 700], [5, 300, 40]
+        pool, stats, bt, start, q = attend_case(seed, ctx, new, 16, 4, dtype)
+        args = (pool, ints(bt), ints(start), ints(ctx), q)
+        cases.append((args, dict(stats=stats, workspace=kvx.attend_chunk_workspace(3, len(q), 16, 4, bt.shape[1]))))
+    want = [kvx.attend_chunk(*args, **kw) for args, kw in cases]
+    x = normal(gen(68), 512, 128, dtype=F32)
+    dense = kvx.attention_dense(x, x, x)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (args, kw) in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(kvx.attend_chunk(*args, **kw))
+        with torch.cuda.stream(streams[2]):
+            again = kvx.attention_dense(x, x, x)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+    assert torch.equal(again, dense)
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_attend_in_place(kvx, dtype):
     """out may be q."""
