@@ -196,11 +196,18 @@ __device__ __forceinline__ ChunkWork chunk_work(const ChunkParams &p, int *mine)
     w.pieces = 1;
     longest = __reduce_max_sync(0xffffffffu, longest);
     if (rest && longest >= 2 * kMinChunk) {
-        // turns x (key tiles + 3 for a CTA's start and end), least
+        // Least of turns x (key tiles + a CTA's start and end, 10 us), and for
+        // partial results their writing and reading (64 pieces: a key tile's
+        // time) and the combine, in 64ths of a key tile.  Against 3 key tiles
+        // for a CTA and nothing for the rest: 2600 tokens behind 2000 (24 q-heads
+        // on 8) 147 and 190 us, 1001 behind 3000 (64 on 8) 160 and 198, 3500
+        // behind 30000 (24 on 8) 1515 and 1493.
+        const unsigned start = p.tile_rows == 256 ? 6 : 8;
         const int most = min(min(p.max_splits, (int)longest / kMinChunk), p.max_pieces / rest);
         unsigned best = 0xffffffffu, at = 1;
         for (int n = 1 + lane; n <= most; n += 32) {
-            const unsigned cost = (unsigned)((rest * n + p.sms - 1) / p.sms) * ((longest + n - 1) / n + 3);
+            const unsigned cost =
+                64u * ((rest * n + p.sms - 1) / p.sms) * ((longest + n - 1) / n + start) + (n > 1 ? rest * n + 128 : 0);
             if (cost < best) best = cost, at = n;
         }
         w.pieces = (int)__reduce_min_sync(0xffffffffu, best == __reduce_min_sync(0xffffffffu, best) ? at : 0xffffffffu);
@@ -1112,7 +1119,7 @@ template <bool kSplit> struct FewShared {
 // lengths (which the host does not know).  It is counted in units of a page
 // for each warp of a CTA (p.few_keys keys).  A pair is kFewStart empty units, then its
 // own: what the start and end of a pair cost a CTA, so that one whose range
-// holds two ends has less to read.
+// holds two ends has less to read (8 x 5 tokens: 35.4 us, with 2 units 37.2).
 constexpr int kFewStart = 4;
 struct FewWork {
     int units;  // of all
