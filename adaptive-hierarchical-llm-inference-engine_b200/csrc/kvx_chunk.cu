@@ -143,6 +143,8 @@ __device__ __forceinline__ int row_keys(const ChunkParams &p, const RowTile &t, 
     return (int)min(k, (long long)p.max_pages * kPageTokens);
 }
 
+// A CTA's start and end, in key tiles.
+__host__ __device__ constexpr int piece_start(int tile_rows) { return tile_rows == 256 ? 6 : 8; }
 constexpr int kMinChunk = 4;  // key tiles of a piece: below, a CTA's start and end outweigh its work
 
 __device__ __forceinline__ RowTile row_tile(const ChunkParams &p, int s, int tile, int tile_rows, int pieces) {
@@ -202,7 +204,7 @@ __device__ __forceinline__ ChunkWork chunk_work(const ChunkParams &p, int *mine)
         // for a CTA and nothing for the rest: 2600 tokens behind 2000 (24 q-heads
         // on 8) 147 and 190 us, 1001 behind 3000 (64 on 8) 160 and 198, 3500
         // behind 30000 (24 on 8) 1515 and 1493.
-        const unsigned start = p.tile_rows == 256 ? 6 : 8;
+        const unsigned start = piece_start(p.tile_rows);
         const int most = min(min(p.max_splits, (int)longest / kMinChunk), p.max_pieces / rest);
         unsigned best = 0xffffffffu, at = 1;
         for (int n = 1 + lane; n <= most; n += 32) {
@@ -1650,12 +1652,26 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     auto row_tiles = [&](int tile_rows) {
         return rows / tile_rows + (few ? std::min<long long>(p.batch, rows / (kFewRows + 1)) : p.batch);
     };
-    // Rows of a CTA (fp16): 128 while CTAs of 256 would leave SMs idle, else
-    // 256, which converts each key tile for twice the rows.  24 q-heads on 8,
-    // 128 against 256 rows: 1001 tokens 28.5 against 32.7 us, 1500: 40.6
-    // against 56.6; 2600: 90 against 70, 5000: 249 against 203; behind 8000
-    // keys 500: 93 and 93, 3500: 572 against 580.
-    p.tile_rows = kSplit || row_tiles(256) * p.hkv <= sm_count() ? 128 : 256;
+    // Rows of a CTA (fp16): 256, which converts each key tile for twice the
+    // rows (2.4 us a key tile, 128: 1.4), or 128, which fills the SMs better.
+    // Behind many keys (four times the new tokens, as far as the block table
+    // tells) the lesser cost by the model that also splits the row tiles;
+    // prompts have tiles of all lengths: 128 while CTAs of 256 would leave SMs
+    // idle.  24 q-heads on 8, 128 against 256: 1001 tokens 28.4 and 33.6 us,
+    // 1500: 40.6 and 43.5, 2600: 90 and 70; behind 8000 500: 97 and 82, 1500:
+    // 215 and 197; 100 behind 30000: 75 and 88.
+    auto cost = [&](int tile_rows) {
+        const long long pairs = row_tiles(tile_rows) * p.hkv, rest = pairs % sm_count(), keys = key_tiles(p.max_pages);
+        long long tail = rest ? 64 * (keys + piece_start(tile_rows)) : 0;
+        const long long most = rest ? std::min<long long>({most_splits(p.max_pages), most_pieces(pairs) / rest, 32}) : 1;  // an estimate
+        for (long long n = 2; n <= most; ++n)
+            tail = std::min(tail, 64 * ((rest * n + sm_count() - 1) / sm_count()) * ((keys + n - 1) / n + piece_start(tile_rows)) +
+                                      rest * n + 128);
+        return (tile_rows == 256 ? 12 : 7) * (64 * (pairs / sm_count()) * (keys + piece_start(tile_rows)) + tail);
+    };
+    const long long wide = row_tiles(256) * p.hkv;
+    const bool far = (long long)p.max_pages * kPageTokens >= 4LL * p.total / p.batch;
+    p.tile_rows = kSplit || (wide <= 2LL * sm_count() && (far ? cost(128) < cost(256) : wide <= sm_count())) ? 128 : 256;
     p.tile_shift = p.tile_rows == 256 ? 8 : 7;
     p.max_tiles = (int)row_tiles(p.tile_rows);
     const long long pairs = (long long)p.max_tiles * p.hkv;  // at most
