@@ -9,6 +9,10 @@
 // so a score costs one multiply-add on the accumulator, and the second sum is
 // one scalar per row.
 //
+// A block of one value is stored as scale 1, codes -128, zero point = the value:
+// its mid is 128 off what it holds, and a sum of rounded weights times -128
+// would not take that back.  block_values() gives such a block scale 0 instead.
+//
 // Rows: the new tokens of a sequence times the q-heads of a kv-head, token
 // major.  A CTA owns a tile of 128 or 256 rows and a range of 128-key tiles
 // (8 pages); 5 warpgroups, registers dealt out with setmaxnreg:
@@ -131,6 +135,12 @@ struct ChunkBars {
 };
 static_assert(sizeof(ChunkBars) <= kBarBytes);
 
+
+// {scale, zero point} of a block's statistics {min, max, scale, zero point};
+// scale 0 for a block of one value (stored with scale 1).
+__device__ __forceinline__ float2 block_values(const float4 &st) {
+    return make_float2(st.x == st.y && st.z == 1.f && st.w == st.x ? 0.f : st.z, st.w);
+}
 
 __device__ __forceinline__ int sequence_tokens(const ChunkParams &p, int s) {
     const int a = p.q_start[s], b = min(p.q_start[s + 1], p.total);
@@ -565,21 +575,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             float4 stat = stat_of(id);
             for (int i = 0; i < tiles; ++i) {
                 const uint32_t known = __ballot_sync(0xffffffffu, id >= 0 && id < p.num_pages) & 0xffu;
-                const float4 cur = stat;
+                const float2 cur = block_values(stat);
                 id = id_next;
                 stat = stat_of(id);
                 id_next = page_of(i + 2);
                 // scales that are no numbers do not count
-                const int e = lane >= 8 && lane < 16 && fabsf(cur.z) < CUDART_INF_F ? exponent_above(cur.z) : -100;
+                const int e = lane >= 8 && lane < 16 && fabsf(cur.x) < CUDART_INF_F ? exponent_above(cur.x) : -100;
                 E = max(E, __reduce_max_sync(0xffffffffu, e));
-                const float mid = fmaf(128.f, cur.z, cur.w), f = lane < 8 ? p.scale_log2 : pow2i(7 - E);
+                const float mid = fmaf(128.f, cur.x, cur.y), f = lane < 8 ? p.scale_log2 : pow2i(7 - E);
                 TileStats &t = tile_stats[i & (kStatSlots - 1)];
                 wait_or_give_up(&bars->stat_empty[i & (kStatSlots - 1)], (i / kStatSlots & 1) ^ 1, bars, p.error_flag);
                 // a K scale of zero becomes 1e-20: the -inf of a masked key stays
                 // one, and products below 2^27 of the others stay nothing
                 if (lane < 16)
                     reinterpret_cast<float2 *>(&t.page[lane & 7])[lane >> 3] =
-                        make_float2(lane < 8 && cur.z * f == 0.f ? 1e-20f : cur.z * f, lane < 8 ? mid * f : mid);
+                        make_float2(lane < 8 && cur.x * f == 0.f ? 1e-20f : cur.x * f, lane < 8 ? mid * f : mid);
                 if (lane == 0) {
                     t.exponent = E;
                     t.known = known;
@@ -1355,7 +1365,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
                 stage = stage == kFewStages - 1 ? 0 : stage + 1;
                 continue;
             }
-            const float2 ks = make_float2(f.ks.z, f.ks.w), vs = make_float2(f.vs.z, f.vs.w);  // {scale, zero point}
+            const float2 ks = block_values(f.ks), vs = block_values(f.vs);
             uint4 kw[2][2];
 #pragma unroll
             for (int j = 0; j < 2; ++j)
