@@ -26,7 +26,8 @@
 //  * MMA warp: one lane issues S = Q K^T (M 128, N 128, 8 steps of K 16) and
 //    O += P V with P read from tensor memory;
 //  * 2 softmax warpgroups, a thread per row: running maximum and sum in
-//    registers, P (fp16) written over the columns of S it came from; O stays in
+//    registers, P (fp16 high and low parts) written over the columns of S it
+//    came from; O stays in
 //    tensor memory and is rescaled only when a row's maximum has grown by
 //    more than 2^8 (p <= 2^8 until then).
 // The two warpgroups have an S and an O each (512 tensor-memory columns in
@@ -50,12 +51,18 @@
 // sequences of 5 new tokens behind up to 8192 keys, 90 MB of codes: 37 us,
 // against 75 us in the tiles above).
 //
-// fp16 calls: P' = p s 2^(7 - E) with 2^E above the largest V scale so far: at
-// most 2^15 and normal in fp16 down to p s = 2^-21 of that scale, so a block
-// of small scale keeps its precision.
+// P' = p s 2^(7 - E) with 2^E above the largest V scale so far: at most 2^15
+// and normal in fp16 down to p s = 2^-21 of that scale, so a block of small
+// scale keeps its precision.  It enters P V as fp16 high + low parts, as in
+// kvx_decode: the weights multiply a block's whole range, and one rounding of
+// them costs up to 2^-12 of it, which in a block with outliers is far more than
+// the output's own rounding (1 % of V a hundred times the rest, 2 to 33 keys:
+// off by up to 0.09).  fp16 calls add both parts to the same sums.  The second
+// MMA costs 1.62 -> 2.02 ms (4096 new tokens behind 28672), 28.0 -> 30.2 us (a
+// prompt of 1001), 38.8 -> 41.2 us (8 x 5 tokens).
 //
-// fp32 calls: q (scaled to 2^13) and P' enter as fp16 high + low parts, 22 bits
-// or more, two MMAs for each product.  The high parts are on a grid (multiples
+// fp32 calls: q (scaled to 2^13) enters as high + low parts too, 22 bits or
+// more, two MMAs for each product.  The high parts are on a grid (multiples
 // of 8 of q, of 2^-4 of P'), so their sums of products with the codes stay
 // below 2^24 grid steps and are exact although the tensor core truncates; the
 // low parts have sums of their own.  So a row tile is 128 rows, O takes 256
@@ -657,8 +664,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                     tc_fence_after();
                     const uint32_t v = umma_desc_low(at + kAtV + st * kTileBytes, kHalfBytes);
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)  // a page: its P over its columns of S
-                        umma_f16_ts(issues, tmem + 256 + j * 128, tmem + j * 128 + ks * 16, v + (ks * 2048 >> 4), kIdescPV, (w > 1) | ks);
+                    for (int ks = 0; ks < 16; ++ks)  // a page: its P, high and low, over its columns of S
+                        umma_f16_ts(issues, tmem + 256 + j * 128, tmem + j * 128 + ks * 8, v + ((ks >> 1) * 2048 >> 4), kIdescPV, (w > 1) | ks);
                     if (u_turns || j) umma_commit(issues, &bars->v_empty[st]);
                 }
                 if (w + 2 < u_items) {
@@ -948,14 +955,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                             const float2 g = h2_to_f2(hi[k / 2]);
                             lo[k / 2] = pack_half(f.x - g.x, f.y - g.y);
                         } else {
-                            hi[k / 2] = pack_half(f.x, f.y);
+                            // high part cut to 11 bits, so that the rest is exact
+                            const float a = __uint_as_float(__float_as_uint(f.x) & 0xffffe000u), b = __uint_as_float(__float_as_uint(f.y) & 0xffffe000u);
+                            hi[k / 2] = pack_half(a, b);
+                            const float2 g = unpack2(fma2(pack2(a, b), pack2(-1.f, -1.f), p2));
+                            lo[k / 2] = pack_half(g.x, g.y);
                         }
                     }
                     const float2 both = unpack2(sum);
                     l += both.x + both.y;
                     z = fmaf(both.x + both.y, st.w, z);
                     tmem_st8(t_s + 16 * page, hi);  // over the page's own scores
-                    if constexpr (kSplit) tmem_st8(t_s + 16 * page + 8, lo);
+                    tmem_st8(t_s + 16 * page + 8, lo);
                 }
             }
             tmem_wait_st();
@@ -1333,7 +1344,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
         }
         __syncthreads();
 
-        float o[16][4];  // n-tile t: two dims of row g, of row g + 8; times 2^-v_exp
+        float o[16][4];  // n-tile t: two dims of row g, of row g + 8; times 2^(7 - v_exp)
 #pragma unroll
         for (int t = 0; t < 16; ++t)
 #pragma unroll
@@ -1412,8 +1423,9 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
                         top[r] = fmaxf(top[r], x);
                     }
             }
-            // P V takes p times the page's scale: as fp16 that keeps its 11 bits
-            // while the scale is near 2^v_exp.  v_exp goes down no further than
+            // P V takes p times the page's scale times 2^(7 - v_exp), as fp16 high
+            // and low parts that keep 22 bits while the scale is near 2^v_exp (p <=
+            // 2^8: at most 2^15).  v_exp goes down no further than
             // 60 below the largest so far, so that the sums stay finite.
             const float v_abs = fabsf(vs.x);
             const int e_v = v_abs > 0.f && v_abs < CUDART_INF_F ? max(min(exponent_above(v_abs), 126), v_top - 60) : v_exp;
@@ -1438,7 +1450,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
                     }
                 }
             }
-            const float v_scale = vs.x * pow2i(-v_exp);
+            const float v_scale = vs.x * pow2i(7 - v_exp);
             uint4 ph, pl;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -1458,11 +1470,9 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
                 const uint32_t a = pack_half(e4[0], e4[1]), b = pack_half(e4[2], e4[3]);
                 (r ? ph.y : ph.x) = a;
                 (r ? ph.w : ph.z) = b;
-                if constexpr (kSplit) {
-                    const float2 x = h2_to_f2(a), y = h2_to_f2(b);
-                    (r ? pl.y : pl.x) = pack_half(e4[0] - x.x, e4[1] - x.y);
-                    (r ? pl.w : pl.z) = pack_half(e4[2] - y.x, e4[3] - y.y);
-                }
+                const float2 x = h2_to_f2(a), y = h2_to_f2(b);
+                (r ? pl.y : pl.x) = pack_half(e4[0] - x.x, e4[1] - x.y);
+                (r ? pl.w : pl.z) = pack_half(e4[2] - y.x, e4[3] - y.y);
             }
             uint4 vw[4];
 #pragma unroll
@@ -1483,7 +1493,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
                 for (int i = 0; i < 4; ++i) {
                     const uint2 v = codes_to_half(col[i]);
                     mma_f16(o[4 * w + i], ph, v.x, v.y);
-                    if constexpr (kSplit) mma_f16(o[4 * w + i], pl, v.x, v.y);
+                    mma_f16(o[4 * w + i], pl, v.x, v.y);
                 }
             }
         }
@@ -1491,7 +1501,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
         __syncwarp();
 
         // ---- the quad's sums, then the warps
-        const float v_unit = pow2i(v_exp);
+        const float v_unit = pow2i(v_exp - 7);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
 #pragma unroll

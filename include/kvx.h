@@ -453,8 +453,8 @@ KVX_API int kvx_rope_append(const kvx_paged *kv, const int32_t *block_table, int
  * 1); a query that sees no key gives a zero row.  Scales in the statistics
  * are not negative.  Output rows outside every
  * sequence keep what they hold; out may be q.  Accumulation and softmax in
- * fp32; fp16 calls round the probabilities, times the V scales, to fp16 for
- * the second product.  batch * num_kv_heads * (max_pages / 4 + 5) fits an int
+ * fp32; the probabilities, times the V scales, enter the second product as
+ * fp16 high + low parts, 22 bits.  batch * num_kv_heads * (max_pages / 4 + 5) fits an int
  * (else KVX_EUNSUPPORTED).  workspace:
  * kvx_attend_chunk_workspace_bytes(), 16-byte aligned, needs no
  * initialisation; calls that share one are ordered. */

@@ -60,3 +60,77 @@ def test_attend_over_keys_of_one_value(kvx, dtype, ctx, new):
         pool[::step, 0] = -128
         out = kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), q * 16, stats=stats)
         assert_attended(out, attend64(pool, as_scale_zero(stats), bt, start, ctx, q * 16))
+
+
+# ------------------------------------------------- precision of P V ---
+
+def one_hot_q(g, rows, hq, dtype):
+    """Queries with one element, a power of two: a score has no more than a
+    few roundings, so that those of P V show."""
+    q = torch.zeros(rows, hq, 128, dtype=dtype, device="cuda")
+    at = torch.randint(0, 128, (rows, hq, 1), generator=g, device="cuda")
+    size = torch.exp2(torch.randint(-2, 4, (rows, hq, 1), generator=g, device="cuda").float())
+    sign = torch.randint(0, 2, (rows, hq, 1), generator=g, device="cuda") * 2 - 1
+    return q.scatter_(2, at, (size * sign).to(dtype))
+
+
+def assert_attended_closely(got, ref, floor=0.0):
+    """With one_hot_q.  A score: two products, a sum, the maximum taken from
+    it, each half a step of 2^-23 of what it adds up to (noise, twice with the
+    maximum; in powers of two 1.45 times that), and the exponential 2^-21;
+    once more through the sum.  A weight in high and low part is off by 2^-21,
+    the sum of the second product by 64 steps of 2^-23 (truncated, or a random
+    walk of more).  Then the output's rounding."""
+    out, size, noise = ref
+    eps = 16 * 2.0 ** -24 * noise + 2.0 ** -21
+    tol = (2 * eps + 64 * 2.0 ** -23 + 2.0 ** -21) * size + floor
+    tol = tol + ((E16 * (out.abs() + tol) + TINY16) if got.dtype == F16 else E32 * out.abs())
+    bad = ~((got.double() - out).abs() <= tol)
+    assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} elements off, worst {(got.double() - out).abs().max():.3e}, "
+                           f"{((got.double() - out).abs() / tol).max():.1f} of the bound")
+
+
+def outlier_case(seed, ctx, new, hq, hkv, dtype):
+    """1 % of V a hundred times the rest: the scale is the outliers'."""
+    def spread(g, pages, hkv):
+        s = torch.ones(pages, 2, hkv, 16, 128, device="cuda")
+        s[:, 1][torch.rand(pages, hkv, 16, 128, generator=g, device="cuda") < 0.01] = 100.0
+        return s
+    pool, stats, bt, start, _ = attend_case(seed, ctx, new, hq, hkv, dtype, spread)
+    return pool, stats, bt, start, one_hot_q(gen(seed), int(start[-1]), hq, dtype)
+
+
+CLOSE = [([0], [2]), ([1], [1]), ([31], [2]), ([127], [1]), ([500], [4]), ([0], [40]), ([100], [33]), ([500, 3], [128, 300]), ([2000], [100])]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (24, 8)])
+@pytest.mark.parametrize("ctx,new", CLOSE)
+def test_attend_over_blocks_with_outliers(kvx, dtype, ctx, new, hq, hkv):
+    pool, stats, bt, start, q = outlier_case(93 + sum(new), ctx, new, hq, hkv, dtype)
+    out = kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), q, stats=stats)
+    assert_attended_closely(out, attend64(pool, stats, bt, start, ctx, q))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (24, 8), (32, 2)])
+def test_attend_agrees_with_decode_over_outliers(kvx, dtype, hq, hkv):
+    """A token attended alone and as the last of 40: what the calls round, no
+    more; and decoded, within the decode's own bound."""
+    ctx = [0, 31, 100, 511, 2000]
+    pool, stats, bt, start, q = outlier_case(97, ctx, [1] * len(ctx), hq, hkv, dtype)
+    args = pool, ints(bt)
+    single = kvx.attend_chunk(*args, ints(start), ints(ctx), q, stats=stats)
+    decoded = kvx.decode(*args, ints([c + 1 for c in ctx]), q, stats=stats)
+    # the same token as the last of 40 (the others' queries do not matter)
+    group = [max(c - 39, 0) for c in ctx]
+    counts = [c + 1 - a for c, a in zip(ctx, group)]
+    many_start = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    many_q = torch.zeros(int(many_start[-1]), hq, 128, dtype=dtype, device="cuda")
+    last = torch.tensor(many_start[1:] - 1, dtype=torch.int64, device="cuda")
+    many_q[last] = q
+    many = kvx.attend_chunk(*args, ints(many_start), ints(group), many_q, stats=stats)[last]
+    ref = attend64(pool, stats, bt, start, ctx, q)
+    for got in (single, many):
+        assert_attended_closely(got, ref)
+        assert ((got - decoded).float().abs() <= 1e-2 + 1e-3 * decoded.float().abs()).all()
