@@ -61,16 +61,25 @@
 // MMA costs 1.62 -> 2.02 ms (4096 new tokens behind 28672), 28.0 -> 30.2 us (a
 // prompt of 1001), 38.8 -> 41.2 us (8 x 5 tokens).
 //
+// Sums: the tensor core cuts the sum that an MMA adds to, always towards zero,
+// so a sum of one sign loses a part that grows with its length: 2.9e-4 of it
+// over 30,000 keys, 7.2e-4 over 60,000 with both parts in one sum (measured, V
+// with an element at the top of its range in every token).  So O is moved out
+// of tensor memory every 32 key tiles of a warpgroup (fp32: 8; settle()), and
+// loses up to 1.2e-4 of it, less than an fp16 rounding (fp32: 3e-6 measured).
+// That costs 2.02 -> 2.15 ms and 217 -> 254 us at the sizes named here; every 16
+// and 4 tiles: 2.28 ms, 276 us, 64: 2.08 ms.  attend_rows_kernel adds each
+// page's part in fp32 registers (41.2 -> 43.3 us).
+//
 // fp32 calls: q (scaled to 2^13) enters as high + low parts too, 22 bits or
-// more, two MMAs for each product.  The high parts are on a grid (multiples
-// of 8 of q, of 2^-4 of P'), so their sums of products with the codes stay
-// below 2^24 grid steps and are exact although the tensor core truncates; the
-// low parts have sums of their own.  So a row tile is 128 rows, O takes 256
-// columns (high, low), S as many, and the two warpgroups take 64 keys each of
-// every tile, with one running maximum.  4 ragged sequences of up to 300 new
-// tokens behind 4096, 64 q-heads on 8: 217 us and an error of 4.3e-7; one sum
-// for both parts, the warpgroups taking turns, was 172 us and 3.4e-6 (fp32
-// products and sums of the plain form: 5850 us, 9.5e-7).
+// more, two MMAs for each product.  The high parts of q are on a grid (multiples
+// of 8), so their sums of products with the codes stay below 2^24 grid steps and
+// are exact although the tensor core cuts; the low parts of both products have
+// sums of their own.  So a row tile is 128 rows, O takes 256 columns (high,
+// low), S as many, and the two warpgroups take 64 keys each of every tile, with
+// one running maximum.  4 ragged sequences of up to 300 new tokens behind 4096,
+// 64 q-heads on 8: 254 us and an error of 5.0e-7 (fp32 products and sums of the
+// plain form: 5850 us, 6.2e-7).
 #include <math_constants.h>
 
 #include <algorithm>
@@ -103,6 +112,8 @@ constexpr int kBarBytes = 320;
 constexpr int kAtK = 2 * kTileBytes, kAtV = kAtK + 2 * kTileBytes, kAtStage = kAtV + 2 * kTileBytes,
               kAtMisc = kAtStage + 2 * kSlotBytes, kChunkSmem = 1024 + kAtMisc + kBarBytes + kStatSlots * (int)sizeof(TileStats) + 256 * 4;
 static_assert(kChunkSmem <= 227 * 1024, "chunk attention exceeds the shared memory of a CTA");
+// Key tiles of a warpgroup after which O is taken out of tensor memory.
+template <bool kSplit> constexpr int kSettle = kSplit ? 8 : 32;
 constexpr float kLazy = 8.f;  // log2 of the growth of a row's maximum that is let pass
 
 struct ChunkParams {
@@ -525,7 +536,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
     // halves of each
     const bool turns = kSplit || rt.rows <= 128, alternate = turns && !kSplit;
     const int items = turns ? tiles : 2 * tiles;  // item w: warpgroup w % 2 (fp32: both), key tile w or w / 2
-    const int slot_bits = turns && !kSplit ? 2 : 1, slot_mask = (1 << slot_bits) - 1;  // 4 or 2 staging slots
+    // 4 or 2 staging slots (two are Q1's place, which settle() takes in long runs)
+    const int slot_bits = alternate && tiles <= 2 * kSettle<kSplit> ? 2 : 1, slot_mask = (1 << slot_bits) - 1;
     const int32_t *table = p.block_table + (size_t)seq * p.max_pages;
     // S0, S1, O0, O1: 128 columns each.  All 512 columns were asked for, so
     // they begin at 0 (were they to begin elsewhere, nothing is done).
@@ -810,17 +822,112 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         if (kSplit) asm volatile("bar.sync 1, 256;" ::: "memory");  // row_sum, row_unscale are free
         const int limit = valid ? row_keys(p, rt, row0 + my_row) : 0x7fffffff;  // a row that is none needs no mask
         const int step = alternate ? 2 : 1;
+        // the columns of O that this thread looks after, 16 at a time: its own O's
+        // (fp32: its half of the dims, high parts, then low parts)
+        auto o_at = [&](int c) { return kSplit ? tmem + 256 + lanes + (c >> 2) * 128 + 64 * j + 16 * (c & 3) : t_o + 16 * c; };
         // O by f (rare, so in little code)
         auto scale_o = [&](float f) {
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
                 uint32_t o[16];
-                tmem_ld16(t_o + 16 * c, o);
+                tmem_ld16(o_at(c), o);
                 tmem_wait_ld(o);
 #pragma unroll
                 for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                tmem_st16(t_o + 16 * c, o);
+                tmem_st16(o_at(c), o);
             }
+        };
+        // The tensor core cuts every sum it adds to (about 2^-22 of it an MMA, and
+        // always towards zero), so every kSettle key tiles O moves on to the row's
+        // place in the output or in the partial results, times 1 / settled.  fp16
+        // rows there hold the nearest fp16 (of at most 2^15: |O| <= 2^14 l) and the
+        // rest, exact, stays in O; the second of two warpgroups with the same rows
+        // has Q1's place in shared memory.
+        float settled = 0.f;  // 0: nothing there yet
+        auto home = [&] {
+            return rt.splits == 1 ? static_cast<uint8_t *>(p.out) + row_index(my_row) * (kHeadDim * sizeof(T))
+                                  : reinterpret_cast<uint8_t *>(p.part_o + ((size_t)bars->part * tile_rows + my_row) * kHeadDim);
+        };
+        auto home_vec = [&](uint8_t *at, int k) {  // its 16-byte vector k
+            return reinterpret_cast<uint4 *>(alternate && j ? sm + kTileBytes + tile_chunk(r, k) : at + 16 * k);
+        };
+        constexpr int kVec = 16 / (int)sizeof(T);
+        auto vec_dims = [&](const uint4 &w, float *h) {
+            if constexpr (kSplit) {
+                h[0] = __uint_as_float(w.x), h[1] = __uint_as_float(w.y), h[2] = __uint_as_float(w.z), h[3] = __uint_as_float(w.w);
+            } else {
+                const float2 a = h2_to_f2(w.x), b = h2_to_f2(w.y), d = h2_to_f2(w.z), e = h2_to_f2(w.w);
+                h[0] = a.x, h[1] = a.y, h[2] = b.x, h[3] = b.y, h[4] = d.x, h[5] = d.y, h[6] = e.x, h[7] = e.y;
+            }
+        };
+        auto settle = [&](float l) {  // rows that are none have no home
+            uint8_t *at = home();
+            if constexpr (kSplit) {  // added in memory: nothing to wait for
+                const bool add = settled > 0x1p-60f;
+                const float times = add ? 1.f / settled : 1.f;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t o[16], low[16];
+                    tmem_ld16(o_at(c), o);
+                    tmem_ld16(o_at(c + 4), low);
+                    tmem_wait_ld(o);
+                    tmem_wait_ld(low);
+                    if (valid) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float4 *to = reinterpret_cast<float4 *>(at) + 16 * j + 4 * c + k;
+                            float f[4];
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) f[d] = (__uint_as_float(o[4 * k + d]) + __uint_as_float(low[4 * k + d])) * times;
+                            if (add) {
+                                asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]) : "memory");
+                            } else {
+                                const float4 old = settled != 0.f ? __ldcg(to) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                *to = make_float4(fmaf(old.x, settled, f[0]), fmaf(old.y, settled, f[1]), fmaf(old.z, settled, f[2]), fmaf(old.w, settled, f[3]));
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[k] = 0;
+                    tmem_st16(o_at(c), o);
+                    tmem_st16(o_at(c + 4), o);
+                }
+                if (!add) settled = 1.f;
+            } else {
+                const int e = min(exponent_above(l), 100);
+                const float down = pow2i(e - 1), up = pow2i(1 - e);
+#pragma unroll 1
+                for (int b = 0; b < 16; b += 8) {
+                    uint4 w[8];  // asked for together
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) w[k] = settled != 0.f && valid ? *home_vec(at, b + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[16], u[8];
+                        tmem_ld16(o_at(b / 2 + c), o);
+                        tmem_wait_ld(o);
+                        float h[16];
+                        vec_dims(w[2 * c], h);
+                        vec_dims(w[2 * c + 1], h + 8);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) h[k] = fmaf(h[k], settled, __uint_as_float(o[k]));
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            u[k] = pack_half(h[2 * k] * up, h[2 * k + 1] * up);
+                            const float2 g = h2_to_f2(u[k]);
+                            o[2 * k] = __float_as_uint(fmaf(g.x, -down, h[2 * k]));
+                            o[2 * k + 1] = __float_as_uint(fmaf(g.y, -down, h[2 * k + 1]));
+                        }
+                        if (valid) {
+                            *home_vec(at, b + 2 * c) = make_uint4(u[0], u[1], u[2], u[3]);
+                            *home_vec(at, b + 2 * c + 1) = make_uint4(u[4], u[5], u[6], u[7]);
+                        }
+                        tmem_st16(o_at(b / 2 + c), o);
+                    }
+                }
+                settled = down;
+            }
+            tmem_wait_st();
         };
         // the 64 scores of pages c .. c + kStep - 1
         auto load_scores = [&](int c, uint32_t(&x)[2][32]) {
@@ -854,9 +961,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             const bool masked = __any_sync(0xffffffffu, seen < kPages * kPageTokens) || known != (1u << kPages) - 1;
             // a page this row sees nothing of: scores of -inf, whatever its statistics
             auto hidden = [&](int page) { return seen <= page * kPageTokens || !(known >> page & 1); };
+            const int past = kSplit ? w : w >> 1;  // items in O, or moved on from it
             wait_or_give_up(&bars->s_full[kSplit ? 0 : j], (kSplit ? w : w >> 1) & 1, bars, p.error_flag);
             __syncwarp();
             tc_fence_after();
+            if (past && !(past & (kSettle<kSplit> - 1))) settle(l);
             if (masked) {  // few tiles: their scores are masked where they are
 #pragma unroll 1
                 for (int page = 0; page < kPages; ++page) {
@@ -917,7 +1026,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                     l *= f;
                     z *= f;
                 }
-                if (w >= (kSplit ? 1 : 2)) scale_o(E - e < -126 ? 0.f : f * pow2i(E - e));
+                f = E - e < -126 ? 0.f : f * pow2i(E - e);
+                if (w >= (kSplit ? 1 : 2)) scale_o(f);
+                settled *= f;
                 E = e;
             }
             const float m_use = m == -CUDART_INF_F ? 0.f : m;
@@ -934,9 +1045,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                     st.y = fmaf(st.y, q_sum, -m_use);
                     if (masked && hidden(page)) st = make_float4(1.f, 0.f, 0.f, 0.f);
                     const uint64_t aa = pack2(st.x, st.x), bb = pack2(st.y, st.y), ss = pack2(st.z, st.z);
-                    // pages of a far smaller scale than the largest (2^6) keep 11 bits of their own
-                    const float grid = st.z >= 2.f ? 1.5f * 524288.f : 0.f;
-                    const uint64_t round = pack2(grid, grid), round_back = pack2(-grid, -grid);
                     uint64_t sum = 0;
                     uint32_t hi[8], lo[8];
 #pragma unroll
@@ -947,11 +1055,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                         const uint64_t p2 = mul2(e2, ss);
                         const float2 f = unpack2(p2);
                         if constexpr (kSplit) {
-                            // the high part to a multiple of 2^-4 (11 bits of p s near its
-                            // largest): sums of its products are exact up to 2^20,
-                            // however the tensor core rounds
-                            const float2 c = unpack2(add2(add2(p2, round), round_back));
-                            hi[k / 2] = pack_half(c.x, c.y);
+                            hi[k / 2] = pack_half(f.x, f.y);
                             const float2 g = h2_to_f2(hi[k / 2]);
                             lo[k / 2] = pack_half(f.x - g.x, f.y - g.y);
                         } else {
@@ -990,13 +1094,38 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
         // half of its sums goes to the other one by shared memory, [dim][row]
         // over K, now free
         float *shared_o = reinterpret_cast<float *>(sm + kAtK);
+        // dims 32 c .. + 31 of the row's sums
+        auto sums = [&](int c, uint32_t(&x)[32]) {
+            if constexpr (kSplit) {
+                uint32_t low[32];
+                tmem_ld32(tmem + 256 + lanes + 32 * c, x);
+                tmem_ld32(tmem + 384 + lanes + 32 * c, low);
+                tmem_wait_ld(x, low);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) + __uint_as_float(low[k]));
+            } else {
+                tmem_ld32(t_o + 32 * c, x);
+                tmem_wait_ld(x);
+            }
+            if (settled != 0.f && valid) {
+                uint8_t *at = home();
+#pragma unroll
+                for (int n = 0; n < 32 / kVec; ++n) {
+                    float h[kVec];
+                    uint4 *from = home_vec(at, c * (32 / kVec) + n);
+                    vec_dims(kSplit ? __ldcg(from) : *from, h);
+#pragma unroll
+                    for (int k = 0; k < kVec; ++k)
+                        x[kVec * n + k] = __float_as_uint(fmaf(h[k], settled, __uint_as_float(x[kVec * n + k])));
+                }
+            }
+        };
         if (merge) {
             float *shared_ml = reinterpret_cast<float *>(sm);  // over Q
 #pragma unroll 1
             for (int c = 2 - 2 * j; c < 4 - 2 * j; ++c) {
                 uint32_t x[32];
-                tmem_ld32(t_o + 32 * c, x);
-                tmem_wait_ld(x);
+                sums(c, x);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) shared_o[(32 * c + k) * 128 + r] = fmaf(__uint_as_float(x[k]), back, z);
             }
@@ -1031,18 +1160,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
 #pragma unroll 1
         for (int c = c0; c < c0 + chunks; ++c) {
             uint32_t x[32];
-            // by whole warps: rows that are none are loaded, not stored
-            if constexpr (kSplit) {
-                uint32_t low[32];
-                tmem_ld32(tmem + 256 + lanes + 32 * c, x);
-                tmem_ld32(tmem + 384 + lanes + 32 * c, low);
-                tmem_wait_ld(x, low);
-#pragma unroll
-                for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) + __uint_as_float(low[k]));
-            } else {
-                tmem_ld32(t_o + 32 * c, x);
-                tmem_wait_ld(x);
-            }
+            sums(c, x);  // by whole warps: rows that are none are loaded, not stored
 #pragma unroll
             for (int k = 0; k < 32; k += 8) {
                 float f[8];
@@ -1492,8 +1610,13 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint2 v = codes_to_half(col[i]);
-                    mma_f16(o[4 * w + i], ph, v.x, v.y);
-                    mma_f16(o[4 * w + i], pl, v.x, v.y);
+                    // the page's part alone, then added: the tensor core cuts the
+                    // sum it adds to, always towards zero
+                    float d[4];
+                    mma_f16_zero(d, pl, v.x, v.y);
+                    mma_f16(d, ph, v.x, v.y);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[4 * w + i][e] += d[e];
                 }
             }
         }

@@ -134,3 +134,62 @@ def test_attend_agrees_with_decode_over_outliers(kvx, dtype, hq, hkv):
     for got in (single, many):
         assert_attended_closely(got, ref)
         assert ((got - decoded).float().abs() <= 1e-2 + 1e-3 * decoded.float().abs()).all()
+
+
+# ------------------------------------------------- sums over many keys ---
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("batch,ctx,new,hq,hkv", [(1, 30000, 1184, 16, 2), (1, 30000, 40, 16, 2), (300, 30000, 1, 8, 2), (150, 31000, 17, 8, 1),
+                                                       (1, 60000, 2368, 16, 2), (148, 120000, 16, 8, 1)])
+def test_attend_sums_of_one_sign(kvx, dtype, batch, ctx, new, hq, hkv):
+    """Flat scores and a V with one element at the top of its block's range in
+    every token, one at the bottom: sums that only grow, over 30,000 to 120,000
+    keys in one piece (as many row tiles as SMs; of 256 and of 128 rows), in
+    several, in the few rows' kernel."""
+    pages = (ctx + new + 15) // 16
+    g = gen(99)
+    pool = torch.randint(-128, 128, (pages, 2, hkv, 16, 128), generator=g, device="cuda", dtype=torch.int8)
+    pool[:, 1, ..., 0], pool[:, 1, ..., 1] = 127, -128
+    size = torch.rand(pages, 2, hkv, generator=g, device="cuda") / 4 + 0.75
+    stats = torch.stack((-size, size, 2 * size / 255, -size), -1).contiguous()
+    bt = ints(list(range(pages))).expand(batch, pages).contiguous()
+    q = torch.zeros(batch * new, hq, 128, dtype=dtype, device="cuda")
+    start = ints([new * i for i in range(batch + 1)])
+    out = kvx.attend_chunk(pool, bt, start, ints([ctx] * batch), q, stats=stats)
+    st = stats[:, 1].double()
+    v = st[..., 3, None, None] + (pool[:, 1].double() + 128) * st[..., 2, None, None]  # [pages][hkv][16][128]
+    v = v.permute(0, 2, 1, 3).reshape(-1, hkv, 128)[:ctx + new]
+    want = (v.cumsum(0) / torch.arange(1, len(v) + 1, device="cuda")[:, None, None])[ctx:]
+    want = want.repeat_interleave(hq // hkv, 1).repeat(batch, 1, 1)
+    # An MMA takes up to 2^-21 off the sum it adds to; off a sum that grows
+    # evenly, half of that on average: 2^-22 each.  Up to 32 (fp32: 8) key tiles
+    # of 128 go into one sum, 16 (fp32: 8) MMAs each.
+    off = 512 * 2.0 ** -22 if dtype == F16 else 64 * 2.0 ** -22
+    err = (out.double() - want).abs()
+    print(f"{dtype} {batch} x {new}: worst {err.max().item():.3e}, elements 0, 1: {err[..., :2].max().item():.3e}")
+    assert ((out >= (want - off).to(dtype)) & (out <= (want + off).to(dtype))).all(), f"worst {err.max():.3e}"
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("batch,ctx,new,hq,hkv", [(1, 9000, 1184, 16, 2), (1, 9000, 2368, 16, 2), (148, 12000, 16, 8, 1), (1, 70000, 100, 8, 2)])
+def test_attend_long_rows_in_place_with_rising_and_falling_scores(kvx, dtype, batch, ctx, new, hq, hkv):
+    """Sums that were moved on and then scaled down, by a little and by more
+    than a type holds, in the output's own place (out is q) and in pieces."""
+    pool, stats, bt, start, q = attend_case(100 + batch, [ctx], [new], hq, hkv, dtype)
+    pages = torch.tensor(bt[0][bt[0] >= 0], dtype=torch.int64, device="cuda")
+    for head in range(hkv):
+        ramp = torch.linspace(-3, 3, len(pages), device="cuda") * (1 if head == 0 else -1)
+        if head == 0:  # and one step up of hundreds, in the middle
+            ramp[len(pages) // 2:] += 200.0
+        stats[pages, 0, head, 3] += ramp
+    q = torch.cat([q] * batch)
+    q[:, :, 0] += 3  # the ramps count the same way in every row
+    bts, starts = np.concatenate([bt] * batch), np.arange(batch + 1, dtype=np.int32) * new
+    args = pool, ints(bts), ints(starts), ints([ctx] * batch)
+    out = kvx.attend_chunk(*args, q, stats=stats)
+    got = q.clone()
+    kvx.attend_chunk(*args, got, stats=stats, out=got)
+    assert torch.equal(got, out)
+    ref = attend64(pool, stats, bt, start, [ctx], q[:new])
+    for s in range(0, batch, 49):
+        assert_attended(out[s * new:(s + 1) * new], ref)
