@@ -78,7 +78,7 @@
 // sums of their own.  So a row tile is 128 rows, O takes 256 columns (high,
 // low), S as many, and the two warpgroups take 64 keys each of every tile, with
 // one running maximum.  4 ragged sequences of up to 300 new tokens behind 4096,
-// 64 q-heads on 8: 254 us and an error of 5.0e-7 (fp32 products and sums of the
+// 64 q-heads on 8: 257 us and an error of 5.0e-7 (fp32 products and sums of the
 // plain form: 5850 us, 6.2e-7).
 #include <math_constants.h>
 
@@ -99,6 +99,9 @@ constexpr int kSoftmaxRegs = 128, kConvertRegs = 72, kIssueRegs = 80;
 static_assert(2 * kSoftmaxRegs + 2 * kConvertRegs + kIssueRegs == 5 * 96, "the launch's registers, dealt out");
 constexpr int kTileBytes = 128 * kHeadDim * 2;  // an fp16 tile of Q, K or V: two halves of 64 dims
 constexpr int kHalfBytes = kTileBytes / 2, kSlotBytes = kTileKeys * kHeadDim;
+// fp32 calls: the low part of P' (at most 2^3, half a step of 2^15) enters times
+// 2^11, so that it stays normal in fp16 down to a P' of 2^-14 and below.
+constexpr float kLowUp = 2048.f;
 // What the softmax needs of a key tile's statistics.
 constexpr int kStatSlots = 4;
 struct TileStats {
@@ -878,7 +881,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                             float4 *to = reinterpret_cast<float4 *>(at) + 16 * j + 4 * c + k;
                             float f[4];
 #pragma unroll
-                            for (int d = 0; d < 4; ++d) f[d] = (__uint_as_float(o[4 * k + d]) + __uint_as_float(low[4 * k + d])) * times;
+                            for (int d = 0; d < 4; ++d) f[d] = fmaf(__uint_as_float(low[4 * k + d]), 1.f / kLowUp, __uint_as_float(o[4 * k + d])) * times;
                             if (add) {
                                 asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]) : "memory");
                             } else {
@@ -1057,7 +1060,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                         if constexpr (kSplit) {
                             hi[k / 2] = pack_half(f.x, f.y);
                             const float2 g = h2_to_f2(hi[k / 2]);
-                            lo[k / 2] = pack_half(f.x - g.x, f.y - g.y);
+                            lo[k / 2] = pack_half((f.x - g.x) * kLowUp, (f.y - g.y) * kLowUp);
                         } else {
                             // high part cut to 11 bits, so that the rest is exact
                             const float a = __uint_as_float(__float_as_uint(f.x) & 0xffffe000u), b = __uint_as_float(__float_as_uint(f.y) & 0xffffe000u);
@@ -1102,7 +1105,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 tmem_ld32(tmem + 384 + lanes + 32 * c, low);
                 tmem_wait_ld(x, low);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) + __uint_as_float(low[k]));
+                for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(fmaf(__uint_as_float(low[k]), 1.f / kLowUp, __uint_as_float(x[k])));
             } else {
                 tmem_ld32(t_o + 32 * c, x);
                 tmem_wait_ld(x);
@@ -1210,6 +1213,11 @@ constexpr int kFewRows = 16;
 // Warps of a CTA and CTAs on an SM: as many warps as the registers hold.
 template <bool kSplit> constexpr int kFewWarps = kSplit ? 4 : 8;
 template <bool kSplit> constexpr int kFewCtas = kSplit ? 3 : 2;
+// P' = p s 2^(kFewUp - v_exp) is at most 2^15: p may reach 2^kFewLazy before the
+// maximum in use follows.  fp32: little leeway, so that the weights of distant
+// keys are normal fp16 numbers (p of 2^-24: 2^-10, high and low part 2^-14 of it).
+template <bool kSplit> constexpr int kFewLazy = kSplit ? 1 : 8;
+template <bool kSplit> constexpr int kFewUp = 15 - kFewLazy<kSplit>;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -1462,7 +1470,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
         }
         __syncthreads();
 
-        float o[16][4];  // n-tile t: two dims of row g, of row g + 8; times 2^(7 - v_exp)
+        float o[16][4];  // n-tile t: two dims of row g, of row g + 8; times 2^(kFewUp - v_exp)
 #pragma unroll
         for (int t = 0; t < 16; ++t)
 #pragma unroll
@@ -1541,14 +1549,14 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
                         top[r] = fmaxf(top[r], x);
                     }
             }
-            // P V takes p times the page's scale times 2^(7 - v_exp), as fp16 high
-            // and low parts that keep 22 bits while the scale is near 2^v_exp (p <=
-            // 2^8: at most 2^15).  v_exp goes down no further than
+            // P V takes p times the page's scale times 2^(kFewUp - v_exp), as fp16
+            // high and low parts that keep 22 bits while the scale is near 2^v_exp.
+            // v_exp goes down no further than
             // 60 below the largest so far, so that the sums stay finite.
             const float v_abs = fabsf(vs.x);
             const int e_v = v_abs > 0.f && v_abs < CUDART_INF_F ? max(min(exponent_above(v_abs), 126), v_top - 60) : v_exp;
             const bool far = e_v > v_exp || e_v < v_exp - 4;
-            if (__any_sync(0xffffffffu, far || top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
+            if (__any_sync(0xffffffffu, far || top[0] > m[0] + kFewLazy<kSplit> || top[1] > m[1] + kFewLazy<kSplit>)) {
                 const float to = v_exp - e_v < -126 ? 0.f : far ? pow2i(v_exp - e_v) : 1.f;
                 if (far) v_exp = e_v;
                 v_top = max(v_top, v_exp);
@@ -1568,7 +1576,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
                     }
                 }
             }
-            const float v_scale = vs.x * pow2i(7 - v_exp);
+            const float v_scale = vs.x * pow2i(kFewUp<kSplit> - v_exp);
             uint4 ph, pl;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -1624,7 +1632,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
         __syncwarp();
 
         // ---- the quad's sums, then the warps
-        const float v_unit = pow2i(v_exp - 7);
+        const float v_unit = pow2i(v_exp - kFewUp<kSplit>);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
 #pragma unroll

@@ -136,6 +136,37 @@ def test_attend_agrees_with_decode_over_outliers(kvx, dtype, hq, hkv):
         assert ((got - decoded).float().abs() <= 1e-2 + 1e-3 * decoded.float().abs()).all()
 
 
+# ------------------------------------------------- distant keys ---
+
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("far,bits", [(13, 20), (24, 14), (30, 8)])
+def test_attend_distant_keys_count(kvx, new, far, bits):
+    """Key 0 takes nearly all of the weight and has a V of nearly nothing;
+    30,000 others have 2^-far of it each and V of 1.37.  Scores are exact; a
+    weight times the scale of V still has that many bits."""
+    ctx, hq, hkv = 30000, 8, 2
+    bt, num_pages, start = layout_of([ctx], [new], 7)
+    g = gen(98)
+    pool = torch.randint(-128, 128, (num_pages, 2, hkv, 16, 128), generator=g, device="cuda", dtype=torch.int8)
+    stats = torch.zeros(num_pages, 2, hkv, 4, device="cuda")
+    first = int(bt[0, 0])
+    pool[:, 0, :, :, 0] = -128  # K: element 0 is 0 but for key 0's
+    pool[first, 0, :, 0, 0] = 127
+    stats[:, 0] = torch.tensor([0.0, 2.55, 2.55 / 255, 0.0], device="cuda")
+    stats[first, 0] = torch.tensor([0.0, far, far / 255, 0.0], device="cuda")
+    pool[:, 1, :, :, :64] = 127
+    stats[:, 1] = torch.tensor([-1.37, 1.37, 2.74 / 255, -1.37], device="cuda")
+    stats[first, 1] *= 2.0 ** -20
+    q = torch.zeros(new, hq, 128, dtype=F32, device="cuda")
+    q[..., 0] = 1.0
+    out = kvx.attend_chunk(pool, ints(bt), ints([0, new]), ints([ctx]), q, stats=stats, sm_scale=math.log(2.0))
+    ref = attend64(pool, stats, bt, [0, new], [ctx], q, scale=math.log(2.0))
+    others = ctx * 2.0 ** -far
+    # key 0's own V, up to 1.37 * 2^-20, is 3.5 % of the others' 2^-30 * 30,000 * 1.37
+    assert ref[0][0, 0, 0].item() == pytest.approx(1.37 * others / (1 + others), rel=4e-2)
+    assert_attended_closely(out, ref, floor=2.0 ** -bits * ref[0][0, 0, 0].item())
+
+
 # ------------------------------------------------- sums over many keys ---
 
 @pytest.mark.parametrize("dtype", [F16, F32])
