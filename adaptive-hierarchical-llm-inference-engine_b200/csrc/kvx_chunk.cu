@@ -51,7 +51,8 @@
 // sequences of 5 new tokens behind up to 8192 keys, 90 MB of codes: 37 us,
 // against 75 us in the tiles above).
 //
-// P' = p s 2^(7 - E) with 2^E above the largest V scale so far: at most 2^15
+// P' = p s 2^(7 - E) with 2^E above the largest V scale that the row has seen (not
+// that of pages behind its last key, whose range is none of its): at most 2^15
 // and normal in fp16 down to p s = 2^-21 of that scale, so a block of small
 // scale keeps its precision.  It enters P V as fp16 high + low parts, as in
 // kvx_decode: the weights multiply a block's whole range, and one rounding of
@@ -105,7 +106,7 @@ constexpr float kLowUp = 2048.f;
 // What the softmax needs of a key tile's statistics.
 constexpr int kStatSlots = 4;
 struct TileStats {
-    float4 page[kTilePages];  // K: scale, mid (times the softmax scale, log2); V: scale 2^(7 - exponent), mid
+    float4 page[kTilePages];  // K: scale, mid (times the softmax scale, log2); V: scale, mid
     int exponent;             // 2^exponent is above every V scale up to this tile
     uint32_t known;           // bit i: page i is there
     uint32_t pad[2];
@@ -604,14 +605,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 // scales that are no numbers do not count
                 const int e = lane >= 8 && lane < 16 && fabsf(cur.x) < CUDART_INF_F ? exponent_above(cur.x) : -100;
                 E = max(E, __reduce_max_sync(0xffffffffu, e));
-                const float mid = fmaf(128.f, cur.x, cur.y), f = lane < 8 ? p.scale_log2 : pow2i(7 - E);
+                const float mid = fmaf(128.f, cur.x, cur.y), f = lane < 8 ? p.scale_log2 : 1.f;
                 TileStats &t = tile_stats[i & (kStatSlots - 1)];
                 wait_or_give_up(&bars->stat_empty[i & (kStatSlots - 1)], (i / kStatSlots & 1) ^ 1, bars, p.error_flag);
                 // a K scale of zero becomes 1e-20: the -inf of a masked key stays
                 // one, and products below 2^27 of the others stay nothing
                 if (lane < 16)
                     reinterpret_cast<float2 *>(&t.page[lane & 7])[lane >> 3] =
-                        make_float2(lane < 8 && cur.x * f == 0.f ? 1e-20f : cur.x * f, lane < 8 ? mid * f : mid);
+                        make_float2(lane < 8 && cur.x * f == 0.f ? 1e-20f : cur.x * f, mid * f);
                 if (lane == 0) {
                     t.exponent = E;
                     t.known = known;
@@ -960,7 +961,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
             wait_or_give_up(&bars->stat_full[i & (kStatSlots - 1)], i / kStatSlots & 1, bars, p.error_flag);
             const uint32_t known = kSplit ? ts.known >> page0 & 0xfu : ts.known;
             const auto *stats = ts.page + page0;
-            const int e = ts.exponent, seen = limit - (t0 + i) * kTileKeys - page0 * kPageTokens;  // the item's keys that the row sees
+            const int seen = limit - (t0 + i) * kTileKeys - page0 * kPageTokens;  // the item's keys that the row sees
             const bool masked = __any_sync(0xffffffffu, seen < kPages * kPageTokens) || known != (1u << kPages) - 1;
             // a page this row sees nothing of: scores of -inf, whatever its statistics
             auto hidden = [&](int page) { return seen <= page * kPageTokens || !(known >> page & 1); };
@@ -1017,10 +1018,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 top = fmaxf(top, row_sum[128 * (j ^ 1) + r]);
             }
+            // the largest V scale of the pages that the row has seen (both warpgroups
+            // of fp32 calls: of the whole tile); those behind its last key do not count
+            int e = ts.exponent;
+            const int in_tile = limit - (t0 + i) * kTileKeys;
+            if (kSplit ? __any_sync(0xffffffffu, in_tile < kTileKeys) || ts.known != 0xffu : masked) {
+                e = E;
+#pragma unroll 1
+                for (int page = 0; page < kTilePages; ++page) {
+                    const float v = ts.page[page].z;
+                    if (in_tile > page * kPageTokens && (ts.known >> page & 1) && fabsf(v) < CUDART_INF_F) e = max(e, exponent_above(v));
+                }
+            }
             // the maximum in use may lag by kLazy; O follows where it catches
             // up, and where a larger V scale came
             const bool lags = __any_sync(0xffffffffu, top > m + kLazy);
-            if (lags || e > E) {
+            if (lags || __any_sync(0xffffffffu, e > E)) {
                 float f = 1.f;
                 if (lags) {
                     const float mn = fmaxf(m, top);
@@ -1034,7 +1047,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 settled *= f;
                 E = e;
             }
-            const float m_use = m == -CUDART_INF_F ? 0.f : m;
+            const float m_use = m == -CUDART_INF_F ? 0.f : m, v_up = pow2i(7 - E);
 #pragma unroll 1
             for (int c = 0; c < kPages; c += kStep) {
                 uint32_t fresh[2][32], (&x)[2][32] = kSplit ? held : fresh;
@@ -1046,6 +1059,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                     float4 st = stats[page];
                     st.x *= unscale;
                     st.y = fmaf(st.y, q_sum, -m_use);
+                    st.z *= v_up;
                     if (masked && hidden(page)) st = make_float4(1.f, 0.f, 0.f, 0.f);
                     const uint64_t aa = pack2(st.x, st.x), bb = pack2(st.y, st.y), ss = pack2(st.z, st.z);
                     uint64_t sum = 0;

@@ -224,3 +224,22 @@ def test_attend_long_rows_in_place_with_rising_and_falling_scores(kvx, dtype, ba
     ref = attend64(pool, stats, bt, start, [ctx], q[:new])
     for s in range(0, batch, 49):
         assert_attended(out[s * new:(s + 1) * new], ref)
+
+
+# ------------------------------------------------- statistics far apart ---
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("ratio", [18, 24, 60])
+@pytest.mark.parametrize("ctx,new", [([0, 0, 0], [40, 300, 3]), ([14, 12], [4, 90])])
+def test_attend_larger_pages_behind_do_not_reach_a_row(kvx, dtype, ratio, ctx, new):
+    """Rows that see a page of V, and behind it, out of their sight, pages of
+    2^ratio times its range."""
+    pool, stats, bt, start, q = attend_case(63 + ratio, ctx, new, 8, 2, dtype)
+    for row in bt:
+        for page in row[1:]:
+            if page >= 0:
+                stats[int(page), 1, :, 2:] *= 2.0 ** ratio
+    out = kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), q, stats=stats)
+    ref = attend64(pool, stats, bt, start, ctx, q)
+    rows = torch.cat([torch.arange(int(a), min(int(a) + 16 - c, int(b))) for a, b, c in zip(start, start[1:], ctx)]).cuda()
+    assert_attended(out[rows], tuple(x[rows] for x in ref))
