@@ -608,11 +608,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) attend_chunk_kernel(const __
                 const float mid = fmaf(128.f, cur.x, cur.y), f = lane < 8 ? p.scale_log2 : 1.f;
                 TileStats &t = tile_stats[i & (kStatSlots - 1)];
                 wait_or_give_up(&bars->stat_empty[i & (kStatSlots - 1)], (i / kStatSlots & 1) ^ 1, bars, p.error_flag);
-                // a K scale of zero becomes 1e-20: the -inf of a masked key stays
-                // one, and products below 2^27 of the others stay nothing
+                // a K scale below 2^-70 becomes that: the -inf of a masked key stays
+                // one also times an fp32 row's 2^-50 (row_unscale), and products
+                // below 2^30 of the others stay nothing
                 if (lane < 16)
                     reinterpret_cast<float2 *>(&t.page[lane & 7])[lane >> 3] =
-                        make_float2(lane < 8 && cur.x * f == 0.f ? 1e-20f : cur.x * f, mid * f);
+                        make_float2(lane < 8 && cur.x * f < 0x1p-70f ? 0x1p-70f : cur.x * f, mid * f);
                 if (lane == 0) {
                     t.exponent = E;
                     t.known = known;

@@ -243,3 +243,18 @@ def test_attend_larger_pages_behind_do_not_reach_a_row(kvx, dtype, ratio, ctx, n
     ref = attend64(pool, stats, bt, start, ctx, q)
     rows = torch.cat([torch.arange(int(a), min(int(a) + 16 - c, int(b))) for a, b, c in zip(start, start[1:], ctx)]).cuda()
     assert_attended(out[rows], tuple(x[rows] for x in ref))
+
+
+# ------------------------------------------------- keys of tiny ranges ---
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("scale,size", [(2.0 ** -100, 1.0), (2.0 ** -100, 2.0 ** -45), (2.0 ** -70, 2.0 ** -60), (0.0, 2.0 ** -45), (2.0 ** -126, 1.0)])
+def test_attend_over_keys_of_tiny_ranges(kvx, dtype, scale, size):
+    """K blocks of a range next to nothing, and queries as small: the masked
+    keys of a page stay masked."""
+    ctx, new = [20, 300, 7], [60, 130, 3]
+    pool, stats, bt, start, q = attend_case(64, ctx, new, 8, 2, dtype)
+    stats[:, 0, :, 2] *= scale
+    q = (q.float() * size).to(dtype)
+    out = kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), q, stats=stats)
+    assert_attended(out, attend64(pool, stats, bt, start, ctx, q))
