@@ -8,6 +8,7 @@ status is not KVX_OK raises KvxError.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import struct
@@ -470,6 +471,10 @@ ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "llama3": 3, "yarn": 4}
 
 # These calls are made once per layer and step, so their checks are plain
 # comparisons and the message is only made when one fails.
+#
+# stream (None: the device's current one; a torch stream or its handle): where
+# the call's work goes, outputs and scratch that the call makes itself included,
+# which belong to it.  Order it with the streams of the other tensors.
 
 def _require(cond, what):
     if not cond:
@@ -496,6 +501,24 @@ def _launch(dev, stream, fn, *args):
         return fn(*args, rt[3](dev) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream)
     with _torch().cuda.device(dev):
         return fn(*args, rt[3](dev) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream)
+
+
+def _on(stream, like):
+    """Context for tensors that a call on `stream` makes itself: they belong to
+    that stream, so their memory is free when its work reaches the call, a fill
+    runs before the call's kernels, and memory given back is not taken by
+    another stream while those run."""
+    if stream is None or like.get_device() < 0:
+        return contextlib.nullcontext()
+    torch = _torch()
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=like.device) if isinstance(stream, int) else stream)
+
+
+def _empty_like(x, stream):
+    if stream is None:
+        return _torch().empty(x.shape, dtype=x.dtype, device=x.device)
+    with _on(stream, x):
+        return _torch().empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _one_device(first, *others):
@@ -587,13 +610,13 @@ def rope(q, k, positions, table, q_out=None, k_out=None, inverse=False, stream=N
     in place.  inverse=True turns back, which is the gradient of the rotation.
     Returns (q_out, k_out)."""
     if q_out is None:
-        q_out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = _empty_like(q, stream)
     rows = _rope_rows(q, q_out, "q")
     tokens, _, dim = q.shape
     n = 1
     if k is not None:
         if k_out is None:
-            k_out = _torch().empty(k.shape, dtype=k.dtype, device=k.device)
+            k_out = _empty_like(k, stream)
         rows += _rope_rows(k, k_out, "k")
         n = 2
         if k.shape[0] != tokens or k.shape[2] != dim or k.dtype != q.dtype:
@@ -662,7 +685,7 @@ def rope_append(pool, block_table, q_start, positions, k, v, q=None, q_out=None,
         if q.shape[0] != tokens or q.dtype != k.dtype:
             raise ValueError("q: tokens and dtype of k")
         if q_out is None:
-            q_out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = _empty_like(q, stream)
         if q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
             raise ValueError("q_out: contiguous, shape and dtype of q")
         q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
@@ -697,11 +720,13 @@ def attend_chunk(pool, block_table, q_start, positions, q, stats=None, out=None,
         raise ValueError("q: contiguous [tokens][hq][128]")
     tokens, hq, _ = q.shape
     if out is None:
-        out = _torch().zeros_like(q)
+        with _on(stream, q):
+            out = _torch().zeros_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("out: contiguous, shape and dtype of q")
     if workspace is None:
-        workspace = attend_chunk_workspace(batch, tokens, hq, kv.num_kv_heads, max_pages, q.device)
+        with _on(stream, q):
+            workspace = attend_chunk_workspace(batch, tokens, hq, kv.num_kv_heads, max_pages, q.device)
     elif not workspace.is_contiguous():
         raise ValueError("workspace: contiguous")
     dev = _one_device(q, out, block_table, q_start, positions, workspace, error_flag, tensor, stats)

@@ -258,3 +258,70 @@ def test_attend_over_keys_of_tiny_ranges(kvx, dtype, scale, size):
     q = (q.float() * size).to(dtype)
     out = kvx.attend_chunk(pool, ints(bt), ints(start), ints(ctx), q, stats=stats)
     assert_attended(out, attend64(pool, stats, bt, start, ctx, q))
+
+
+# ------------------------------------------------- streams ---
+
+LONG = 200_000_000  # cycles: 0.1 s on a stream
+
+
+def test_attend_output_on_an_explicit_stream(kvx):
+    """The rows that the call fills with zeros itself are filled before its
+    kernels, on their stream."""
+    ctx, new = [300, 10], [6, 50]
+    pool, stats, bt, start, q = attend_case(101, ctx, new, 8, 2, F16)
+    args = pool, ints(bt), ints(start), ints(ctx), q
+    want = kvx.attend_chunk(*args, stats=stats)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(LONG)
+    got = [kvx.attend_chunk(*args, stats=stats, stream=s) for s in (side, side.cuda_stream)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in got)
+
+
+def test_attend_scratch_of_two_explicit_streams(kvx, monkeypatch):
+    """Scratch that a call makes itself is not given to another stream while
+    the call may still use it."""
+    ctx, new = [300, 10], [6, 50]
+    pool, stats, bt, start, q = attend_case(102, ctx, new, 8, 2, F16)
+    args = pool, ints(bt), ints(start), ints(ctx), q
+    outs = [torch.zeros_like(q) for _ in range(3)]
+    at, real = [], kvx.attend_chunk_workspace
+
+    def noted(*a, **kw):
+        w = real(*a, **kw)
+        at.append((w.data_ptr(), w.numel()))
+        return w
+    monkeypatch.setattr(kvx, "attend_chunk_workspace", noted)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for s, o in zip(streams, outs):
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(LONG)
+        kvx.attend_chunk(*args, stats=stats, out=o, stream=s)
+    kvx.attend_chunk(*args, stats=stats, out=outs[2])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, outs[2]) for o in outs)
+    at.sort()
+    assert len(at) == 3 and all(a + n <= b for (a, n), (b, _) in zip(at, at[1:]))
+
+
+def test_rope_and_append_outputs_on_an_explicit_stream(kvx):
+    """Outputs that the calls make themselves do not lie in memory that
+    another stream's pending work still writes."""
+    q, k = normal(gen(103), 64, 24, 128), normal(gen(104), 64, 8, 128)
+    pos, table = ints(list(range(64))), kvx.rope_table(128)
+    pool = torch.zeros(4, 2, 8, 16, 128, dtype=torch.int8, device="cuda")
+    stats = torch.zeros(4, 2, 8, 4, device="cuda")
+    bt, start, first = ints([[0, 1, 2, 3]]), ints([0, 64]), ints([0])
+    want_q, want_k = kvx.rope(q, k, pos, table)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(LONG)
+    for x in (q, k, q):  # freed with their fill still to come
+        torch.empty_like(x).fill_(7.0)
+    got_q, got_k = kvx.rope(q, k, pos, table, stream=side)
+    got = kvx.rope_append(pool, bt, start, first, k, k, q=q, table=table, stats=stats, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(got_q, want_q) and torch.equal(got_k, want_k) and torch.equal(got, want_q)
