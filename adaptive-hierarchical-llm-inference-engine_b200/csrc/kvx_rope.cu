@@ -477,7 +477,8 @@ int launch_rope_append(const RopeAppendParams &p, bool i8, bool half, bool vec, 
         // 64 registers let 4 of them on an SM (with the other role's 128 it is
         // 2, too few to keep the memory busy).
         kern<<<(unsigned)p.kv_blocks + (p.hq && !p.apart ? (unsigned)p.total : 0u), kRopeThreads, smem, st>>>(p);
-        if (!p.apart || launch_status() != KVX_OK) return launch_status();
+        const int rc = launch_status();  // clears the error: asked once
+        if (!p.apart || rc != KVX_OK) return rc;
         auto q_kern = half ? (vec ? rope_append_q_kernel<T, true, true> : rope_append_q_kernel<T, true, false>)
                            : (vec ? rope_append_q_kernel<T, false, true> : rope_append_q_kernel<T, false, false>);
         cudaLaunchConfig_t cfg{};

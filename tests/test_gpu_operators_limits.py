@@ -325,3 +325,38 @@ def test_rope_and_append_outputs_on_an_explicit_stream(kvx):
     got = kvx.rope_append(pool, bt, start, first, k, k, q=q, table=table, stats=stats, stream=side)
     torch.cuda.synchronize()
     assert torch.equal(got_q, want_q) and torch.equal(got_k, want_k) and torch.equal(got, want_q)
+
+
+# ------------------------------------------------- a launch that fails ---
+
+@pytest.mark.parametrize("tokens", [3, 5000])
+def test_append_reports_a_launch_that_fails(kvx, tokens):
+    """Launches into a stream whose capture has been made invalid fail on the
+    host; the call says so, and works again afterwards."""
+    k = normal(gen(105), tokens, 1, 128)
+    q = normal(gen(106), tokens, 2, 128)
+    q_out = torch.empty_like(q)
+    pages = (tokens + 15) // 16
+    pool = torch.zeros(pages, 2, 1, 16, 128, dtype=torch.int8, device="cuda")
+    stats = torch.zeros(pages, 2, 1, 4, device="cuda")
+    bt, start, first = ints([list(range(pages))]), ints([0, tokens]), ints([0])
+    side = torch.cuda.Stream()
+
+    def call():
+        kvx.rope_append(pool, bt, start, first, k, k, q=q, q_out=q_out, stats=stats, stream=side)
+    call()
+    torch.cuda.synchronize()
+    rt = C.CDLL("libcudart.so.12")
+    stream, graph = C.c_void_p(side.cuda_stream), C.c_void_p()
+    assert rt.cudaStreamBeginCapture(stream, 2) == 0  # relaxed
+    try:
+        assert rt.cudaStreamSynchronize(stream) != 0  # not allowed: the capture is void
+        with pytest.raises(kvx.KvxError) as e:
+            call()
+        assert e.value.status == -3
+    finally:
+        rt.cudaStreamEndCapture(stream, C.byref(graph))
+        rt.cudaGetLastError()
+    call()
+    torch.cuda.synchronize()
+    assert torch.equal(q_out, q)
