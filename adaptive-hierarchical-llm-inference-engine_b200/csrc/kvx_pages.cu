@@ -49,6 +49,9 @@ PlanSpace plan_space(void *w, int num_pages, int num_rows) {
     return s;
 }
 
+// Pages of len tokens (len >= 0, up to the largest int).
+__device__ __forceinline__ int pages_of(int len) { return len / kPageTokens + (len % kPageTokens != 0); }
+
 // Exclusive prefix sum over the CTA's threads in thread order; *total gets
 // the sum.  red: 33 ints of shared memory.
 __device__ __forceinline__ int cta_prefix(int v, int *red, int *total) {
@@ -128,7 +131,7 @@ reserve_kernel(const kvx_pages t, const int32_t *new_tokens, PlanSpace w, int32_
                 bad = kErrLong;
             } else {
                 const int32_t *row = t.block_table + (size_t)r * t.max_pages;
-                for (int lp = (len + kPageTokens - 1) / kPageTokens + lane; lp < want; lp += 32) lack += row[lp] < 0;
+                for (int lp = pages_of(len) + lane; lp < want; lp += 32) lack += row[lp] < 0;
             }
         }
         lack = __reduce_add_sync(0xffffffffu, lack);
@@ -164,7 +167,7 @@ reserve_kernel(const kvx_pages t, const int32_t *new_tokens, PlanSpace w, int32_
         const int want = (int)(((long long)len + new_tokens[r] + kPageTokens - 1) / kPageTokens);
         int32_t *row = t.block_table + (size_t)r * t.max_pages;
         int next = w.rows_b[r];
-        for (int lp0 = (len + kPageTokens - 1) / kPageTokens; lp0 < want; lp0 += 32) {
+        for (int lp0 = pages_of(len); lp0 < want; lp0 += 32) {
             const int lp = lp0 + lane;
             const bool lacks = lp < want && row[lp] < 0;
             const uint32_t mask = __ballot_sync(0xffffffffu, lacks);
@@ -210,7 +213,7 @@ fork_plan_kernel(const kvx_pages t, const int32_t *parents, const int32_t *child
                 if (__ldcg(&w.rows_b[a])) bad |= kErrRows;  // a child of this call as a parent
                 if (len < 0) {
                     bad |= kErrRange;
-                } else if ((len + kPageTokens - 1) / kPageTokens > t.max_pages) {
+                } else if (pages_of(len) > t.max_pages) {
                     bad |= kErrLong;
                 } else if (len % kPageTokens) {
                     const int page = t.block_table[(size_t)a * t.max_pages + len / kPageTokens];

@@ -360,3 +360,17 @@ def test_append_reports_a_launch_that_fails(kvx, tokens):
     call()
     torch.cuda.synchronize()
     assert torch.equal(q_out, q)
+
+
+# ------------------------------------------------- lengths ---
+
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 16, 65])
+def test_pages_refuse_lengths_next_to_the_largest_int(kvx, length):
+    pages, pool = small(kvx)
+    pages.seq_lens[0] = length
+    before = [t.clone() for t in (pages.refcounts, pages.block_table, pages.seq_lens, pool)]
+    for what, args in (("fork", ([0], [1])), ("reserve", ([1, 0, 0, 0],))):
+        err = flag()
+        getattr(pages, what)(*(ints(a) for a in args), error_flag=err)
+        assert err.item() == 4
+        assert all(torch.equal(a, b) for a, b in zip(before, (pages.refcounts, pages.block_table, pages.seq_lens, pool)))
