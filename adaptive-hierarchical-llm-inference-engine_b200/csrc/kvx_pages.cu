@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kScanPer = 16;  // pages a thread looks at per step of a scan
+constexpr int kMostEntries = 0x7fffffff - 2 * kPlanThreads * kScanPer;
 constexpr int kErrRange = 2, kErrLong = 4, kErrPages = 8, kErrRows = 16;
 
 // Workspace: header, then the lists.
@@ -428,7 +429,8 @@ compact_apply_kernel(const kvx_pages t, PlanSpace w, const __grid_constant__ Cop
 int pages_status(const kvx_pages *t) {
     if (!t || !t->refcounts || !t->block_table || !t->seq_lens) return KVX_EINVAL;
     if (t->num_pages <= 0 || t->num_rows <= 0 || t->max_pages <= 0) return KVX_EINVAL;
-    if ((long long)t->num_rows * t->max_pages > 0x7fffffffLL) return KVX_EUNSUPPORTED;  // sums of entries fit an int
+    // sums of entries, and the steps of the loops over pages and entries, fit an int
+    if ((long long)t->num_rows * t->max_pages > kMostEntries || t->num_pages > kMostEntries) return KVX_EUNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(t->refcounts) | reinterpret_cast<uintptr_t>(t->block_table) |
          reinterpret_cast<uintptr_t>(t->seq_lens)) & 3)
         return KVX_EINVAL;
@@ -546,6 +548,7 @@ extern "C" KVX_API int kvx_pages_free(const kvx_pages *pages, const int32_t *row
     const int rc = pages_status(pages);
     if (rc != KVX_OK) return rc;
     if (n < 0) return KVX_EINVAL;
+    if (n > kMostEntries) return KVX_EUNSUPPORTED;
     if (n == 0) return KVX_OK;
     if (!rows) return KVX_EINVAL;
     free_kernel<<<(unsigned)std::min<long long>(n, (long long)sm_count() * 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(

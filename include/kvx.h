@@ -479,7 +479,9 @@ KVX_API int kvx_attend_chunk(const kvx_paged *kv, const int32_t *block_table, in
  * initialisation.  A refused call changes nothing and sets a bit of
  * *error_flag (device int32, may be NULL): bit 1 a row or page id out of
  * range, bit 2 more tokens than a block-table row holds, bit 3 too few free
- * pages, bit 4 a row given twice, or a child that is not empty. */
+ * pages, bit 4 a row given twice, or a child that is not empty.  num_pages,
+ * num_rows * max_pages and the rows of one call are below 2^31 - 2^15 (else
+ * KVX_EUNSUPPORTED). */
 typedef struct kvx_pages {
     int32_t *refcounts;   /* [num_pages] */
     int32_t *block_table; /* [num_rows][max_pages] */

@@ -196,6 +196,19 @@ def test_pages_refuse_tables(kvx, kw, status):
     assert kvx.lib.kvx_pages_compact(p, kv, 1, A, big, None, None, None) == status
 
 
+@pytest.mark.parametrize("kw", [dict(num_pages=2 ** 31 - 1), dict(num_pages=2 ** 31 - 20000), dict(num_rows=1, max_pages=2 ** 31 - 1),
+                                dict(num_rows=2 ** 31 - 1, max_pages=1)])
+def test_pages_refuse_sizes_next_to_the_largest_int(kvx, kw):
+    """A step past the end of such an array would not fit an int."""
+    import kvx.pages  # noqa: F401
+    p, kv, big = C.byref(books(**kw)), C.byref(pool(kvx, num_pages=kw.get("num_pages", 8))), 1 << 60
+    assert kvx.lib.kvx_pages_reserve(p, A, A, big, None, None) == EUNSUPPORTED
+    assert kvx.lib.kvx_pages_fork(p, kv, 1, A, A, 1, A, big, None, None) == EUNSUPPORTED
+    assert kvx.lib.kvx_pages_free(p, A, 1, None, None) == EUNSUPPORTED
+    assert kvx.lib.kvx_pages_compact(p, kv, 1, A, big, None, None, None) == EUNSUPPORTED
+    assert kvx.lib.kvx_pages_free(C.byref(books()), A, 2 ** 31 - 1, None, None) == EUNSUPPORTED
+
+
 def test_pages_refuse_arguments(kvx):
     import kvx.pages  # noqa: F401
     L, p, kv, big = kvx.lib, C.byref(books()), C.byref(pool(kvx)), 1 << 40
