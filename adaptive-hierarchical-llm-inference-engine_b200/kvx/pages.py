@@ -40,7 +40,25 @@ for _fn in ("kvx_pages_reserve", "kvx_pages_fork", "kvx_pages_free", "kvx_pages_
 ERR_RANGE, ERR_LONG, ERR_PAGES, ERR_ROWS = 2, 4, 8, 16  # bits of error_flag
 
 
+def _kept(name):
+    """A property whose object stays: x.name += y writes it in place, another
+    object is refused."""
+    held = "_" + name
+
+    def keep(self, value):
+        if value is not getattr(self, held):
+            raise AttributeError(f"{name}: written in place, not replaced (the calls hold its address)")
+    return property(lambda self: getattr(self, held), keep)
+
+
 class Pages:
+    """The three arrays, the pools and the scratch of one set of pages.  The
+    calls hold their addresses, so the tensors are written in place
+    (pages.seq_lens += n, pages.block_table.copy_(t)) and never replaced."""
+
+    refcounts, block_table, seq_lens = _kept("refcounts"), _kept("block_table"), _kept("seq_lens")
+    pools, stats = _kept("pools"), _kept("stats")
+
     def __init__(self, refcounts, block_table, seq_lens, pools, stats=None):
         torch = _torch()
         _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.is_contiguous(),
@@ -48,11 +66,11 @@ class Pages:
         _vector(refcounts, None, "refcounts")
         _vector(seq_lens, block_table.shape[0], "seq_lens")
         _require(stats is None or len(stats) == len(pools), "stats: one per pool")
-        self.refcounts, self.block_table, self.seq_lens = refcounts, block_table, seq_lens
-        self.pools, self.stats = list(pools), None if stats is None else list(stats)
-        described = [_pool(p, None if stats is None else stats[i]) for i, p in enumerate(self.pools)]
+        self._refcounts, self._block_table, self._seq_lens = refcounts, block_table, seq_lens
+        self._pools, self._stats = tuple(pools), None if stats is None else tuple(stats)
+        described = [_pool(p, None if stats is None else stats[i]) for i, p in enumerate(self._pools)]
         _require(all(kv.num_pages == refcounts.shape[0] for kv, _ in described), "refcounts: one per page of the pools")
-        self._device = _one_device(refcounts, block_table, seq_lens, *(t for _, t in described), *(self.stats or ()))
+        self._device = _one_device(refcounts, block_table, seq_lens, *(t for _, t in described), *(self._stats or ()))
         self._layers = (KvPaged * max(len(described), 1))(*(kv for kv, _ in described))
         self._pages = C.byref(PagesC(refcounts.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), refcounts.shape[0],
                                      block_table.shape[0], block_table.shape[1]))
@@ -77,7 +95,7 @@ class Pages:
 
     def reserve(self, new_tokens, error_flag=None, stream=None):
         """Pages for the next new_tokens[row] tokens of every row."""
-        _vector(new_tokens, self.block_table.shape[0], "new_tokens")
+        _vector(new_tokens, self._block_table.shape[0], "new_tokens")
         self._run(lib.kvx_pages_reserve, "kvx_pages_reserve", stream, (new_tokens, error_flag), self._pages, new_tokens.data_ptr(),
                   self._workspace.data_ptr(), self._bytes, _flag(error_flag))
 
@@ -87,7 +105,7 @@ class Pages:
         n = parents.shape[0]
         _vector(children, n, "children")
         self._run(lib.kvx_pages_fork, "kvx_pages_fork", stream, (parents, children, error_flag), self._pages, self._layers,
-                  len(self.pools), parents.data_ptr(), children.data_ptr(), n, self._workspace.data_ptr(), self._bytes,
+                  len(self._pools), parents.data_ptr(), children.data_ptr(), n, self._workspace.data_ptr(), self._bytes,
                   _flag(error_flag))
 
     def free(self, rows, error_flag=None, stream=None):
@@ -101,12 +119,12 @@ class Pages:
         if num_live is not None:
             _vector(num_live, 1, "num_live")
         self._run(lib.kvx_pages_compact, "kvx_pages_compact", stream, (num_live, error_flag), self._pages, self._layers,
-                  len(self.pools), self._workspace.data_ptr(), self._bytes, None if num_live is None else num_live.data_ptr(),
+                  len(self._pools), self._workspace.data_ptr(), self._bytes, None if num_live is None else num_live.data_ptr(),
                   _flag(error_flag))
 
     def copy(self, src, dst, error_flag=None, stream=None):
         """Page src[i] to page dst[i] in every layer."""
         _vector(src, None, "src")
         _vector(dst, src.shape[0], "dst")
-        self._run(lib.kvx_pages_copy, "kvx_pages_copy", stream, (src, dst, error_flag), self._layers, len(self.pools), src.data_ptr(),
+        self._run(lib.kvx_pages_copy, "kvx_pages_copy", stream, (src, dst, error_flag), self._layers, len(self._pools), src.data_ptr(),
                   dst.data_ptr(), src.shape[0], _flag(error_flag))

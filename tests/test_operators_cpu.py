@@ -209,6 +209,28 @@ def test_pages_refuse_sizes_next_to_the_largest_int(kvx, kw):
     assert kvx.lib.kvx_pages_free(C.byref(books()), A, 2 ** 31 - 1, None, None) == EUNSUPPORTED
 
 
+def test_pages_keep_their_tensors(kvx):
+    """The calls hold addresses: in-place writes go through, another tensor in
+    the place of one is refused."""
+    from kvx.pages import Pages
+    pages = object.__new__(Pages)
+    for name in ("refcounts", "block_table", "seq_lens"):
+        setattr(pages, "_" + name, torch.zeros(3, dtype=torch.int32))
+        t = getattr(pages, name)
+        exec(f"pages.{name} += 2")
+        assert getattr(pages, name) is t and t.tolist() == [2, 2, 2]
+        for other in (t + 1, t.clone(), t[:], None):
+            with pytest.raises(AttributeError):
+                setattr(pages, name, other)
+        with pytest.raises(AttributeError):
+            delattr(pages, name)
+        assert getattr(pages, name) is t
+    pages._pools, pages._stats = (torch.zeros(1),), None
+    for name in ("pools", "stats"):
+        with pytest.raises(AttributeError):
+            setattr(pages, name, (torch.zeros(1),))
+
+
 def test_pages_refuse_arguments(kvx):
     import kvx.pages  # noqa: F401
     L, p, kv, big = kvx.lib, C.byref(books()), C.byref(pool(kvx)), 1 << 40
