@@ -555,11 +555,24 @@ def _io_code(x, what):
     raise ValueError(what + ": float16 or float32")
 
 
+def _kept(name):
+    """A property whose object stays: x.name += y of a tensor writes it in place,
+    another object is refused."""
+    held = "_" + name
+
+    def keep(self, value):
+        if value is not getattr(self, held):
+            raise AttributeError(f"{name}: written in place, not replaced (the calls hold its address or value)")
+    return property(lambda self: getattr(self, held), keep)
+
+
 class RopeTable:
     """Frequencies of a rotary embedding on the device (see rope_table)."""
 
+    turns, rotary_dim, layout, amplitude = _kept("turns"), _kept("rotary_dim"), _kept("layout"), _kept("amplitude")
+
     def __init__(self, turns, rotary_dim, layout, amplitude):
-        self.turns, self.rotary_dim, self.layout, self.amplitude = turns, rotary_dim, layout, amplitude
+        self._turns, self._rotary_dim, self._layout, self._amplitude = turns, rotary_dim, layout, amplitude
         self.c = RopeTableC(turns.data_ptr(), rotary_dim, ROPE_LAYOUT[layout], amplitude)
         self.ref = C.byref(self.c)
 

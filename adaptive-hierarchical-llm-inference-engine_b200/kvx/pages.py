@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import ctypes as C
 
-from . import KvPaged, KvxError, _flag, _launch, _one_device, _pool, _require, _torch, _vector, lib
+from . import KvPaged, KvxError, _flag, _kept, _launch, _one_device, _pool, _require, _torch, _vector, lib
 
 _vp, _i32, _sz = C.c_void_p, C.c_int32, C.c_size_t
 
@@ -38,17 +38,6 @@ for _fn in ("kvx_pages_reserve", "kvx_pages_fork", "kvx_pages_free", "kvx_pages_
     getattr(lib, _fn).restype = C.c_int
 
 ERR_RANGE, ERR_LONG, ERR_PAGES, ERR_ROWS = 2, 4, 8, 16  # bits of error_flag
-
-
-def _kept(name):
-    """A property whose object stays: x.name += y writes it in place, another
-    object is refused."""
-    held = "_" + name
-
-    def keep(self, value):
-        if value is not getattr(self, held):
-            raise AttributeError(f"{name}: written in place, not replaced (the calls hold its address)")
-    return property(lambda self: getattr(self, held), keep)
 
 
 class Pages:

@@ -231,6 +231,17 @@ def test_pages_keep_their_tensors(kvx):
             setattr(pages, name, (torch.zeros(1),))
 
 
+def test_rope_table_keeps_its_values(kvx):
+    """Its C form is made once: an attribute that is replaced would not reach
+    the calls, and the turns in use would be freed."""
+    t = kvx.RopeTable(torch.zeros(64, dtype=torch.int64), 128, "half", 1.0)
+    for name, other in (("turns", torch.ones(64, dtype=torch.int64)), ("rotary_dim", 64), ("layout", "interleaved"), ("amplitude", 2.0)):
+        with pytest.raises(AttributeError):
+            setattr(t, name, other)
+    t.turns += 5
+    assert t.turns.data_ptr() == t.c.turns and t.c.rotary_dim == t.rotary_dim == 128 and t.c.amplitude == t.amplitude == 1.0
+
+
 def test_pages_refuse_arguments(kvx):
     import kvx.pages  # noqa: F401
     L, p, kv, big = kvx.lib, C.byref(books()), C.byref(pool(kvx)), 1 << 40
