@@ -572,6 +572,10 @@ class RopeTable:
     turns, rotary_dim, layout, amplitude = _kept("turns"), _kept("rotary_dim"), _kept("layout"), _kept("amplitude")
 
     def __init__(self, turns, rotary_dim, layout, amplitude):
+        _require(layout in ROPE_LAYOUT, f"layout: one of {sorted(ROPE_LAYOUT)}")
+        _require(rotary_dim >= 2 and rotary_dim % 2 == 0, "rotary_dim: even, at least 2")
+        _require(turns.dtype == _torch().int64 and turns.is_contiguous() and tuple(turns.shape) == (rotary_dim // 2,),
+                 "turns: contiguous int64 [rotary_dim / 2]")
         self._turns, self._rotary_dim, self._layout, self._amplitude = turns, rotary_dim, layout, amplitude
         self.c = RopeTableC(turns.data_ptr(), rotary_dim, ROPE_LAYOUT[layout], amplitude)
         self.ref = C.byref(self.c)

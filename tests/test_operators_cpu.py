@@ -231,6 +231,17 @@ def test_pages_keep_their_tensors(kvx):
             setattr(pages, name, (torch.zeros(1),))
 
 
+@pytest.mark.parametrize("turns,rotary_dim,layout", [
+    (torch.zeros(32, dtype=torch.int64), 128, "half"), (torch.zeros(65, dtype=torch.int64), 128, "half"),
+    (torch.zeros(64, dtype=torch.int32), 128, "half"), (torch.zeros(128, dtype=torch.int64)[::2], 128, "half"),
+    (torch.zeros(64, 1, dtype=torch.int64), 128, "half"), (torch.zeros(64, dtype=torch.int64), 129, "half"),
+    (torch.zeros(0, dtype=torch.int64), 0, "half"), (torch.zeros(64, dtype=torch.int64), 128, "other")])
+def test_rope_table_refuses(kvx, turns, rotary_dim, layout):
+    """The kernels read rotary_dim / 2 turns, whatever the tensor holds."""
+    with pytest.raises(ValueError):
+        kvx.RopeTable(turns, rotary_dim, layout, 1.0)
+
+
 def test_rope_table_keeps_its_values(kvx):
     """Its C form is made once: an attribute that is replaced would not reach
     the calls, and the turns in use would be freed."""
