@@ -625,7 +625,11 @@ def rope(q, k, positions, table, q_out=None, k_out=None, inverse=False, stream=N
     """Rotate q [tokens][hq][dim] and k [tokens][hk][dim] (k may be None) by
     positions [tokens] (int32); any token and head strides.  q_out = q rotates
     in place.  inverse=True turns back, which is the gradient of the rotation.
-    Returns (q_out, k_out)."""
+    Autograd records nothing here, so tensors that require a gradient are
+    refused while it records: call under torch.no_grad(), or from the forward
+    and backward of an autograd function.  Returns (q_out, k_out)."""
+    if (q.requires_grad or (k is not None and k.requires_grad)) and _torch().is_grad_enabled():
+        raise ValueError("q, k: a gradient would be lost here; call rope under torch.no_grad() or in an autograd function")
     if q_out is None:
         q_out = _empty_like(q, stream)
     rows = _rope_rows(q, q_out, "q")

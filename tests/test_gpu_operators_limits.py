@@ -10,8 +10,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_operators import (E16, E32, F16, F32, F64, TINY16, assert_attended, attend64, attend_case, flag, gen, ints,  # noqa: E402
-                                kvx, layout_of, normal, small)
+from test_gpu_operators import (E16, E32, F16, F32, F64, TINY16, assert_attended, assert_turned, attend64, attend_case,  # noqa: E402
+                                flag, gen, ints, kvx, layout_of, normal, small)
 
 assert kvx  # the fixture
 
@@ -374,3 +374,33 @@ def test_pages_refuse_lengths_next_to_the_largest_int(kvx, length):
         getattr(pages, what)(*(ints(a) for a in args), error_flag=err)
         assert err.item() == 4
         assert all(torch.equal(a, b) for a, b in zip(before, (pages.refcounts, pages.block_table, pages.seq_lens, pool)))
+
+
+# ------------------------------------------------- gradients ---
+
+class Turn(torch.autograd.Function):
+    """kvx.rope as an operation that autograd records."""
+
+    @staticmethod
+    def forward(ctx, q, k, rope, pos, table):
+        ctx.rope, ctx.pos, ctx.table = rope, pos, table
+        return rope(q, k, pos, table)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        return (*ctx.rope(gq, gk, ctx.pos, ctx.table, inverse=True), None, None, None)
+
+
+def test_rope_in_an_autograd_function(kvx):
+    """The documented way: grad mode is off in both directions.  The gradient
+    of a weighted sum against the formula's: R^T w, by the inverse."""
+    g = gen(107)
+    q, k = normal(g, 9, 4, 128, dtype=F32).requires_grad_(), normal(g, 9, 2, 128, dtype=F32).requires_grad_()
+    wq, wk = normal(g, 9, 4, 128, dtype=F32), normal(g, 9, 2, 128, dtype=F32)
+    pos, table = ints(list(range(100, 109))), kvx.rope_table(96, scaling="yarn", factor=4.0, high=32.0)
+    with pytest.raises(ValueError):
+        kvx.rope(q, k, pos, table)
+    yq, yk = Turn.apply(q, k, kvx.rope, pos, table)
+    ((yq * wq).sum() + (yk * wk).sum()).backward()
+    for x, w in ((q, wq), (k, wk)):
+        assert_turned(x.grad, w, pos, table, inverse=True)

@@ -307,3 +307,17 @@ def test_host_tensors_are_refused(kvx):
         kvx.rope_table(64, layout="other", device="cpu")
     with pytest.raises(ValueError):
         kvx.rope_table(64, scaling="other", device="cpu")
+
+
+def test_rope_does_not_lose_gradients(kvx):
+    """Recorded operations end here, so a tensor whose gradient is recorded is
+    refused; without recording it is a tensor like any other."""
+    x, y = (torch.zeros(4, 2, 128, dtype=torch.float16) for _ in range(2))
+    y.requires_grad_()
+    tab = kvx.RopeTable(torch.zeros(64, dtype=torch.int64), 128, "half", 1.0)
+    pos = torch.zeros(4, dtype=torch.int32)
+    for args in ((y, None), (x, y), (y * 2, x)):
+        with pytest.raises(ValueError, match="no_grad"):
+            kvx.rope(*args, pos, tab)
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):  # the next check
+            kvx.rope(*args, pos, tab)
