@@ -1407,7 +1407,7 @@ __global__ void __launch_bounds__(kFewWarps<kSplit> * 32, kFewCtas<kSplit>) atte
         const int32_t *table = p.block_table + (size_t)seq * p.max_pages;
         auto page_of = [&](int lp) { return lp < page1 ? table[lp] : -1; };
         const int key_a = 4 * (g >> 1) + (g & 1);  // key of this lane's column of Q K^T (+ 2 for the second n-tile)
-        // this warp's pages page0 + warp, + 4, ...: contents three ahead, ids of 32 at once
+        // this warp's pages page0 + warp, + kWarps, ...: contents kFewStages ahead, ids of 32 at once
         const int first = page0 + warp, count = first < page1 ? (page1 - first + kWarps - 1) / kWarps : 0;
         FewPage *page = sh.of[warp].page;
         int ids = page_of(first + lane * kWarps);

@@ -26,7 +26,6 @@ constexpr int kErrRange = 2, kErrLong = 4, kErrPages = 8, kErrRows = 16;
 struct PlanHeader {
     int32_t count;  // pairs in (src, dst): pages to copy
     int32_t ok;     // the call was accepted
-    int32_t live;   // compact: held pages
 };
 struct PlanSpace {
     PlanHeader *head;
@@ -399,7 +398,6 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const kvx_pa
     if (threadIdx.x == 0) {
         w.head->count = moving;
         w.head->ok = 1;
-        w.head->live = live;
         if (num_live) *num_live = live;
     }
 }

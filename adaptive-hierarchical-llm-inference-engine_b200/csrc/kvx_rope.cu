@@ -243,7 +243,7 @@ template <> struct Raw4<__half> {
 // One warp: the new rows (n from slot `slot0`) of one (page, K|V, head)
 // block.  Lane: elements 4 lane .. 4 lane + 3 of every row, in registers from
 // the range to the codes (read, unpacked and turned twice instead, the kernel
-// issued 2.5 times the instructions, and it is bound by them).  cs: (cos,
+// issued 2.5 times the instructions and took 55 us, not 43).  cs: (cos,
 // sin) of row i's pairs at cs + i * rotary/2, null for V and without a table.
 // kVec: partners in the half layout lie a multiple of 4 away.
 template <typename T, bool kHalf, bool kVec>
@@ -347,8 +347,10 @@ __device__ __forceinline__ void append_block_i8(const T *src, int64_t stride, ui
 // (a decode step, where every token leads), 16 when they fill the GPU anyway.
 // 32 sequences x 1 token (24 q-heads on 8): 4.2 us, three dependent reads and
 // a launch.  6 chunks of up to 2731 tokens (64 q-heads on 8, fp16): 102 us for
-// 410 MB, 43 of them the pages (bound by instructions: unpack, turn, range,
-// quantise, about 40 % of the issue slots at 2 CTAs an SM) and 59 the q rows.
+// 410 MB, 43 of them the pages and 59 the q rows.  The pages are 65 MB, 10 us at
+// the copy rate: with a block's rows in registers 16 warps fit on an SM, 42 % of
+// the issue slots are used, and the rest is latency (fixed waits, scoreboards and
+// barriers, 4.6 cycles an instruction) that so few warps do not hide.
 //
 // A warp with more than kDirectRows rows brings them to shared memory first,
 // a bulk copy (TMA) a row, all in flight together; fewer are read in place,
