@@ -35,21 +35,23 @@
 // own 128 each and share every key tile; with 128 they take turns at the key
 // tiles of the same rows and are merged at the end.
 //
-// What bounds it (4096 new tokens behind 28672, 24 q-heads on 8: 1.63 ms, 948
-// TFLOP/s of Q K^T and P V, 56 % of the measured bf16 rate): a step of 256
-// rows x 128 keys takes about 4600 cycles.  In it the tensor cores work 2050,
-// the exponential units 2050, shared memory about 2600 (Q and K read by
-// Q K^T, V by P V, codes copied in, read and written back as fp16), and a
-// warpgroup's own chain is maximum, exponentials, P V, the next Q K^T.  64-key
-// steps with two score buffers, which take the MMAs out of that chain, were
-// slower (2.19 against 1.80 ms: both warpgroups then want the exponentials at
-// once), as was handing P over by halves (1.85).  Splitting the row tiles of
-// the last, partly filled turn of the SMs gave 1.80 -> 1.63 (384 on 148 SMs).
+// What bounds it (4096 new tokens behind 28672, 24 q-heads on 8: 2.15 to 2.37
+// ms by box and clock, 650 to 720 TFLOP/s of Q K^T and P V counted once, 39 to
+// 43 % of the measured bf16 rate): a step of 256 rows x 128 keys takes about
+// 6000 cycles.  In it the tensor cores work 3070 (two thirds of it P V's
+// two parts), the exponential units 2050, shared memory about 3100 (Q and K
+// read by Q K^T, V twice by P V, codes copied in, read and written back as
+// fp16), and a warpgroup's own chain is maximum, exponentials, P V, the next
+// Q K^T.  Tried before the weights had a low part: 64-key steps with two score
+// buffers, which take the MMAs out of that chain (2.19 against 1.80 ms: both
+// warpgroups then want the exponentials at once), and P handed over by halves
+// (1.85).  Splitting the row tiles of the last, partly filled turn of the SMs
+// gave 1.80 -> 1.63 then (384 on 148 SMs).
 //
 // Sequences of at most 16 rows (a decode step, a few drafted tokens) would use
 // an eighth of those tiles: attend_rows_kernel takes them, on mma.sync (8
-// sequences of 5 new tokens behind up to 8192 keys, 90 MB of codes: 37 us,
-// against 75 us in the tiles above).
+// sequences of 5 new tokens behind up to 8192 keys, 90 MB of codes: 43 us; as
+// of one part a weight 37 us, against 75 us in the tiles above).
 //
 // P' = p s 2^(7 - E) with 2^E above the largest V scale that the row has seen (not
 // that of pages behind its last key, whose range is none of its): at most 2^15
@@ -79,7 +81,7 @@
 // sums of their own.  So a row tile is 128 rows, O takes 256 columns (high,
 // low), S as many, and the two warpgroups take 64 keys each of every tile, with
 // one running maximum.  4 ragged sequences of up to 300 new tokens behind 4096,
-// 64 q-heads on 8: 257 us and an error of 5.0e-7 (fp32 products and sums of the
+// 64 q-heads on 8: 265 us and an error of 5.0e-7 (fp32 products and sums of the
 // plain form: 5850 us, 6.2e-7).
 #include <math_constants.h>
 
@@ -234,8 +236,8 @@ __device__ __forceinline__ ChunkWork chunk_work(const ChunkParams &p, int *mine)
         // partial results their writing and reading (64 pieces: a key tile's
         // time) and the combine, in 64ths of a key tile.  Against 3 key tiles
         // for a CTA and nothing for the rest: 2600 tokens behind 2000 (24 q-heads
-        // on 8) 147 and 190 us, 1001 behind 3000 (64 on 8) 160 and 198, 3500
-        // behind 30000 (24 on 8) 1515 and 1493.
+        // on 8) 183 and 224 us, 1001 behind 3000 (64 on 8) 199 and 235, 3500
+        // behind 30000 (24 on 8) 2057 and 2045 to 2075.
         const unsigned start = piece_start(p.tile_rows);
         const int most = min(min(p.max_splits, (int)longest / kMinChunk), p.max_pieces / rest);
         unsigned best = 0xffffffffu, at = 1;
@@ -1283,7 +1285,8 @@ template <bool kSplit> struct FewShared {
 // lengths (which the host does not know).  It is counted in units of a page
 // for each warp of a CTA (p.few_keys keys).  A pair is kFewStart empty units, then its
 // own: what the start and end of a pair cost a CTA, so that one whose range
-// holds two ends has less to read (8 x 5 tokens: 35.4 us, with 2 units 37.2).
+// holds two ends has less to read (8 x 5 tokens: 43.2 us, with 2 units 42.8; as of
+// one part a weight 35.4 and 37.2).
 constexpr int kFewStart = 4;
 struct FewWork {
     int units;  // of all
@@ -1323,7 +1326,7 @@ __device__ __forceinline__ int few_owner(const FewWork &w, int unit) {
 
 // Sequences of at most 16 rows.  The warps of a CTA take the pages of its
 // range in turn; pages come by cp.async into the warp's own stages (no barrier
-// in the loop), two ahead (three: 36.0 against 35.3 us at the size below).  The
+// in the loop), two ahead (three: 43.9 against 43.2 us at the size below).  The
 // codes become the operands of mma.sync (m16n8k16) in registers: the order of
 // the dims within Q K^T, and of the keys and dims within P V, is free as long as
 // both operands agree, so with g = lane / 4, q = lane % 4
@@ -1338,9 +1341,9 @@ __device__ __forceinline__ int few_owner(const FewWork &w, int unit) {
 // the workspace; a CTA has two such ends at most.
 //
 // 8 sequences of 5 new tokens behind up to 8192 keys, 24 q-heads on 8: 90 MB
-// of codes, 14 us at the copy rate; 28 us here (3.2 TB/s), and 7 us for the
-// launch of the empty tiles beside it and the combine.  Issue slots are half
-// full (about 450 instructions a page and warp, 4 warps a scheduler), the
+// of codes, 14 us at the copy rate; 34 us here (2.7 TB/s), and 9 us for the
+// launch of the empty tiles beside it and the combine.  Issue slots are 54 %
+// full (about 800 instructions a page in all, 4 warps a scheduler), the
 // start (lengths, page ids, first pages: three dependent reads) is a fifth.
 // 8 warps x 2 CTAs an SM against 4 x 4: 40.3 and 42.6 us at the time, for
 // fewer starts, ends and partial results.
@@ -1819,13 +1822,15 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
         return rows / tile_rows + (few ? std::min<long long>(p.batch, rows / (kFewRows + 1)) : p.batch);
     };
     // Rows of a CTA (fp16): 256, which converts each key tile for twice the
-    // rows (2.4 us a key tile, 128: 1.4), or 128, which fills the SMs better.
+    // rows (3.6 us a key tile, 128: 2.0), or 128, which fills the SMs better.
     // Behind many keys (four times the new tokens, as far as the block table
     // tells) the lesser cost by the model that also splits the row tiles;
     // prompts have tiles of all lengths: 128 while CTAs of 256 would leave SMs
-    // idle.  24 q-heads on 8, 128 against 256: 1001 tokens 28.4 and 33.6 us,
-    // 1500: 40.6 and 43.5, 2600: 90 and 70; behind 8000 500: 97 and 82, 1500:
-    // 215 and 197; 100 behind 30000: 75 and 88.
+    // idle.  24 q-heads on 8, 128 against 256: 1001 tokens 32 and 40 us, 1500:
+    // 47 and 53, 2600: 105 and 85; behind 8000 500: 113 and 97, 1500: 273 and
+    // 261; 100 behind 30000: 89 and 105.  A block table wider than the lengths
+    // (2048 pages) makes a prompt count as one behind many keys: 1001 tokens 40
+    // us, 1500: 53, 2 x 700: 36 against 38.
     auto cost = [&](int tile_rows) {
         const long long pairs = row_tiles(tile_rows) * p.hkv, rest = pairs % sm_count(), keys = key_tiles(p.max_pages);
         long long tail = rest ? 64 * (keys + piece_start(tile_rows)) : 0;
@@ -1845,7 +1850,7 @@ int launch_attend(ChunkParams &p, void *workspace, cudaStream_t st) {
     p.max_splits = most_splits(p.max_pages);
     // A prompt from (nearly) its start on more row tiles than SMs: its last
     // turn are its shortest tiles, not worth a combine (1001 tokens, 24 q-heads
-    // on 8: 28 us, and 33 with the launches that may split them).
+    // on 8: 32 us, and 37 with the launches that may split them).
     if (p.causal && p.batch == 1 && pairs > p.sms && (long long)p.max_pages * kPageTokens - p.total < 2 * kMinChunk * kTileKeys)
         p.max_splits = 1;
     p.max_pieces = (int)most_pieces(pairs);
