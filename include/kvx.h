@@ -454,7 +454,9 @@ KVX_API int kvx_rope_append(const kvx_paged *kv, const int32_t *block_table, int
  * are not negative.  Output rows outside every
  * sequence keep what they hold; out may be q.  Accumulation and softmax in
  * fp32; the probabilities, times the V scales, enter the second product as
- * fp16 high + low parts, 22 bits.  batch * num_kv_heads * (max_pages / 4 + 5) fits an int
+ * fp16 high + low parts: 22 bits, down to 2^-32 (fp32 calls: 2^-39) of the
+ * largest that the row has seen.  While the call runs, the sequences' output
+ * rows may hold partial sums.  batch * num_kv_heads * (max_pages / 4 + 5) fits an int
  * (else KVX_EUNSUPPORTED).  workspace:
  * kvx_attend_chunk_workspace_bytes(), 16-byte aligned, needs no
  * initialisation; calls that share one are ordered. */
