@@ -404,3 +404,40 @@ def test_rope_in_an_autograd_function(kvx):
     ((yq * wq).sum() + (yk * wk).sum()).backward()
     for x, w in ((q, wq), (k, wk)):
         assert_turned(x.grad, w, pos, table, inverse=True)
+
+
+# ------------------------------------------------- documented use ---
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("ctx,new,hq,hkv", [([0], [1001], 24, 8), ([0, 0], [700, 700], 24, 8), ([0] + [600] * 9 + [0] * 6, [300] + [1] * 9 + [0] * 6, 16, 4)])
+@pytest.mark.parametrize("width", [64, 2048])
+def test_attend_with_a_table_wider_than_the_lengths(kvx, dtype, ctx, new, hq, hkv, width):
+    """A block table of the longest context, rows of sequences that are not
+    active among them: prompts, and a prompt beside single tokens."""
+    pool, stats, bt, start, q = attend_case(108, ctx, new, hq, hkv, dtype)
+    wide = np.full((len(ctx), width), -1, np.int32)
+    wide[:, :bt.shape[1]] = bt[:, :width]
+    err = flag()
+    out = kvx.attend_chunk(pool, ints(wide), ints(start), ints(ctx), q, stats=stats, error_flag=err)
+    assert err.item() == 0
+    assert_attended(out, attend64(pool, stats, bt, start, ctx, q))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_append_of_prompts_to_float_pools(kvx, dtype):
+    """Prompt-sized chunks behind other lengths, 64 q-heads: the bits of the
+    rotation, then of the append."""
+    ctx, new = [0, 37, 16], [2731, 700, 1]
+    bt, num_pages, start = layout_of(ctx, new, 9)
+    g = gen(109)
+    q, k, v = (normal(g, int(start[-1]), h, 128, dtype=dtype) for h in (64, 8, 8))
+    pool = normal(g, num_pages, 2, 8, 16, 128, dtype=dtype)
+    want = pool.clone()
+    table = kvx.rope_table(128, scaling="llama3", factor=8.0)
+    pos = torch.cat([torch.arange(c, c + n) for c, n in zip(ctx, new)]).int().cuda()
+    tq, tk = kvx.rope(q, k, pos, table)
+    for s, (c, n) in enumerate(zip(ctx, new)):
+        a, b = int(start[s]), int(start[s + 1])
+        kvx.append_chunk(want, ints(bt[s:s + 1]), ints([c]), tk[None, a:b].contiguous(), v[None, a:b].contiguous())
+    qo = kvx.rope_append(pool, ints(bt), ints(start), ints(ctx), k, v, q=q, table=table)
+    assert torch.equal(qo, tq) and torch.equal(pool, want)
